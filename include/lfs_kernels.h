@@ -57,6 +57,13 @@
  *                           (metadata :202-249; paged keys on a prefix-cache
  *                           hit, :231-237); math of model/attention/GQA.py:118-130
  *   lfs_prefill_attention_max_k  the same with the longest context as a hint
+ *   lfs_prefill_attention_window, lfs_paged_decode_window  the prefill and
+ *                           the decode attention over a sliding window with
+ *                           a few first keys that stay visible; no reference
+ *                           counterpart
+ *   lfs_copy_kv_blocks      blocks of the pool copied to others (forking a
+ *                           sequence, packing the pool); no reference
+ *                           counterpart
  *   lfs_fp8_index           fp8_index(q, q_s, k, k_s), the DSA indexer score,
  *                           model/attention/utils.py:175-250 (caller
  *                           model/attention/DSA.py:105)
@@ -65,6 +72,8 @@
  *                           its Exp(1) noise from Philox4x32-10
  *   lfs_sample_gumbel_split  the same sampler with each row cut into slices
  *                           (a caller workspace; same picks)
+ *   lfs_sample_filtered     a token by temperature, top-k, top-p and min-p from
+ *                           a given uniform number; no reference counterpart
  * Fused row kernels of the decode step around those calls (each replaces a
  * chain of torch ops of the reference model):
  *   lfs_add_rmsnorm         RMSNorm with fused residual add, model/utils.py:53-67
@@ -77,6 +86,9 @@
  *                           model/attention/GQA.py:80-95,
  *                           model/attention/utils.py:34-45
  *   lfs_qk_norm_rope_store_kv  the same, k and v in token order as well
+ *   lfs_qk_head_norm_rope_store  the same with every head normalised by itself
+ *                           and a rotation of a head's first dims; no
+ *                           reference counterpart
  *   lfs_moe_route           MoE gate, model/architecture/moe.py:45-90
  *   lfs_add_rmsnorm_route   ffn_norm + MoE gate in one launch (decode step)
  *   lfs_swiglu_quant        silu(w1 x) * w3 x, model/architecture/mlp.py:60-67,
@@ -107,7 +119,7 @@
 extern "C" {
 #endif
 
-#define LFS_ABI_VERSION 17
+#define LFS_ABI_VERSION 18
 
 /* argument errors (negative); launch errors are positive hipError_t values */
 #define LFS_EINVAL (-1)
@@ -368,6 +380,47 @@ int lfs_prefill_attention_max_k(const void* q, const void* k, const void* v, con
                           int32_t max_seqlen_q, int32_t max_seqlen_k, float scale, void* stream);
 
 /*
+ * The same over a sliding window with sinks: query position p sees key t
+ * where t <= p and (t > p - window or t < sinks); 0 where it sees none.
+ * Keys that no query of the call sees are never read: with a block table the
+ * entries of blocks that hold only such keys may be -1.  Of the keys that
+ * some query sees, V must be finite (a hidden one enters its tile's product
+ * with weight 0).  window >= 1, sinks >= 0.
+ */
+int lfs_prefill_attention_window(const void* q, const void* k, const void* v, const int32_t* cu_seqlens_q,
+                                 const int32_t* cu_seqlens_k, const int32_t* block_tables, int64_t bt_stride,
+                                 int32_t block_size, int64_t num_slots, void* out, int64_t B, int32_t num_q_heads,
+                                 int32_t num_kv_heads, int32_t head_dim, int32_t max_seqlen_q, int32_t window,
+                                 int32_t sinks, float scale, void* stream);
+
+/*
+ * lfs_paged_decode over a sliding window with sinks: with L =
+ * context_lens[b] tokens, the newest at L - 1, the tokens t < L with t >= L -
+ * window or t < sinks.  Hidden tokens are never read: the table entries of
+ * blocks that hold only such tokens may be -1.  workspace: at least
+ * lfs_paged_decode_window_workspace_bytes(...) bytes, sized on the device that
+ * runs the call.  q_out / q_scale as for lfs_paged_decode.  window >= 1,
+ * sinks >= 0.  The grid depends only on the shapes and the window.
+ */
+int64_t lfs_paged_decode_window_workspace_bytes(int64_t B, int32_t num_q_heads, int32_t head_dim);
+int lfs_paged_decode_window(const void* q, const void* k_cache, const void* v_cache, const int64_t* context_lens,
+                            const int32_t* block_tables, int64_t bt_stride, void* out, void* workspace,
+                            int64_t workspace_bytes, int64_t B, int32_t num_q_heads, int32_t num_kv_heads,
+                            int32_t head_dim, int32_t block_size, int64_t num_blocks, int32_t max_blocks,
+                            int32_t window, int32_t sinks, float scale, void* q_out, float* q_scale, void* stream);
+
+/*
+ * Blocks of a KV pool copied to other blocks, in each of `planes` planes of
+ * num_blocks blocks of block_bytes bytes (a pool bf16 [2, L, NB, BS, Hkv, D] has
+ * 2 L planes): block src[i] to block dst[i], i < n.  src and dst are HOST
+ * arrays, read before the call returns; a captured graph replays the pairs of
+ * its capture.  A destination may not appear twice, nor be a source.
+ * block_bytes is a multiple of 16.
+ */
+int lfs_copy_kv_blocks(void* pool, int64_t planes, int64_t num_blocks, int64_t block_bytes, const int32_t* src,
+                       const int32_t* dst, int64_t n, void* stream);
+
+/*
  * FP8 indexer score (DSA lightning indexer):
  *   o[b,m,n] = k_s[b][n] * sum_h relu(q[b,m,h,:] . k[b,n,:]) * q_s[b,m,h]
  * q: e4m3fn [B, M, H, D] contiguous; q_s fp32 [B, M, H]; k: e4m3fn rows of
@@ -403,6 +456,24 @@ int64_t lfs_sample_gumbel_workspace_bytes(int64_t B, int32_t vocab);
 int lfs_sample_gumbel_split(const void* logits, int64_t ld, const float* temperatures, int64_t B,
                             int32_t vocab, uint64_t seed, uint64_t offset, int64_t* out, float* noise_out,
                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * One token per row b of logits (bf16 [B, ld]) by temperature, top-k, top-p and
+ * min-p.  The row's tokens are ordered by logit, largest first, equal ones by
+ * index, with weights w_i = exp((x_i - x_max) / T[b]).  Kept are: the first
+ * top_k[b] of the order (<= 0: all); of those the shortest prefix whose weight
+ * reaches top_p[b] times theirs, at least one (>= 1 or NaN: all); of those the
+ * tokens with w_i >= min_p[b] and the first (<= 0 or NaN: all).  out[b] (int64)
+ * is the first token of the order at which the kept weight summed so far
+ * exceeds uniforms[b] (fp32, in [0, 1)) times all of it, logprob[b] (fp32, may
+ * be NULL) log(w / all of it).  top_k int32 [B], top_p and min_p fp32 [B]: NULL
+ * for none.  T <= 0 or NaN: the first of the order.  Tokens at -infinity or NaN
+ * are never drawn; a row of such tokens alone gives token 0 and -infinity.
+ * Weights and sums are held in 64 bits.
+ */
+int lfs_sample_filtered(const void* logits, int64_t ld, const float* temperatures, const float* uniforms,
+                        const int32_t* top_k, const float* top_p, const float* min_p, int64_t B, int32_t vocab,
+                        int64_t* out, float* logprob, void* stream);
 
 /*
  * add_rmsnorm, per row t of x: bf16 [T, d]:
@@ -458,6 +529,20 @@ int lfs_qk_norm_rope_store_kv(const void* qkv, int64_t ld, const float* q_weight
                               void* q_out, void* k_cache, void* v_cache, void* k_out, void* v_out, int64_t T,
                               int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int64_t num_slots,
                               int64_t max_positions, float eps, void* stream);
+
+/*
+ * lfs_qk_norm_rope_store_kv with every head of q and k normalised by itself
+ * (q_weight, k_weight fp32 [D]) and the first rotary_dim dims of a head rotated
+ * (cos_sin fp32 [max_positions, rotary_dim], half-split within them); fp32
+ * throughout, rounded to bf16 once.  k_out and v_out both or neither, caches
+ * and slot_mapping may be NULL.  D in {64, 128}; rotary_dim a multiple of 16,
+ * at most D.  Positions outside the table read its first or last row.
+ */
+int lfs_qk_head_norm_rope_store(const void* qkv, int64_t ld, const float* q_weight, const float* k_weight,
+                                const float* cos_sin, int32_t rotary_dim, const int64_t* positions,
+                                const int64_t* slot_mapping, void* q_out, void* k_cache, void* v_cache, void* k_out,
+                                void* v_out, int64_t T, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                int64_t num_slots, int64_t max_positions, float eps, void* stream);
 
 /*
  * moe_route, per token t of h: bf16 [T, d]:

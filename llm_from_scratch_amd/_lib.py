@@ -11,7 +11,7 @@ import ctypes
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "liblfs_kernels.so"
-ABI_VERSION = 17
+ABI_VERSION = 18
 # size of the library's static paged-decode workspace (LFS_DECODE_SCRATCH_BYTES)
 DECODE_SCRATCH_BYTES = 64 << 20
 
@@ -72,6 +72,19 @@ SIGNATURES = {
                                              _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_f, _c_p]),
     "lfs_prefill_attention_max_k": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_i64, _c_p,
                                                    _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_f, _c_p]),
+    "lfs_prefill_attention_window": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_i64, _c_p,
+                                                    _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_f,
+                                                    _c_p]),
+    "lfs_paged_decode_window_workspace_bytes": (ctypes.c_int64, [_c_i64, _c_i32, _c_i32]),
+    "lfs_paged_decode_window": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i64,
+                                               _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_f,
+                                               _c_p, _c_p, _c_p]),
+    "lfs_qk_head_norm_rope_store": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_p, _c_p, _c_i32, _c_p, _c_p, _c_p, _c_p, _c_p,
+                                                   _c_p, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i64, _c_i64, _c_f,
+                                                   _c_p]),
+    "lfs_sample_filtered": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_p,
+                                           _c_p]),
+    "lfs_copy_kv_blocks": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p]),
     "lfs_moe_align_tiles": (ctypes.c_int64, [_c_i64, _c_i32, _c_i32, _c_i32]),
     "lfs_moe_align": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_p,
                                      _c_p, _c_i64, _c_p]),

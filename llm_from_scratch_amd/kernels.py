@@ -17,6 +17,13 @@ Same names, arguments and return values as the reference's operators:
                          block_table=None) -> o
       varlen causal prefill attention, the call engine/model_runner.py:291-292
       names
+  sample_filtered(logits, temperatures, uniforms, top_k, top_p, min_p)
+      -> tokens
+      temperature, top-k, top-p and min-p sampling from given random numbers
+  copy_kv_blocks(kv_cache, src, dst)
+      blocks of the KV pool copied to others
+  qk_head_norm_rope_store(...) -> q
+      per-head norms, rotation and KV slot write
   sample_gumbel(logits, temperatures, seed, offset) -> tokens
       temperature + Gumbel-max sampling, utils/sampler.py:35-53
   fp8_index(q, q_s, k, k_s) -> index_score
@@ -30,6 +37,7 @@ from __future__ import annotations
 
 import math
 import numbers
+from array import array
 from typing import Optional, Tuple
 
 import torch
@@ -71,6 +79,18 @@ def _on_gpu(*ts: torch.Tensor) -> None:
             raise ValueError(f"tensor on {t.device}: the FP8/paged-KV kernels run on the GPU only")
         if t.device != dev:
             raise ValueError(f"tensors on different devices: {t.device} vs {dev}")
+
+
+def _launch(what: str, fn, on: torch.Tensor, *args) -> None:
+    """fn(*args, stream) on the device and current stream of ``on``, also
+    where that is not the current device."""
+    dev = on.get_device()
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _stream(on))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(on))
+    _lib.check(rc, what)
 
 
 def _dtype(t: torch.Tensor, dt: torch.dtype, name: str) -> None:
@@ -369,6 +389,40 @@ def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
     _lib.check(rc, "store_kvcache")
 
 
+def _block_ids(ids, name: str) -> array:
+    if isinstance(ids, torch.Tensor):
+        if ids.device.type != "cpu":
+            raise ValueError(f"{name} must be host data (a list or a CPU tensor), not on {ids.device}")
+        ids = ids.reshape(-1).tolist()
+    try:
+        return array("i", ids)
+    except OverflowError:
+        raise ValueError(f"{name}: block ids outside the pool") from None
+
+
+def copy_kv_blocks(kv_cache: torch.Tensor, src, dst) -> None:
+    """Copy whole blocks within a KV pool, in every layer's K and V:
+    kv_cache[..., dst[i], :, :, :] = kv_cache[..., src[i], :, :, :].
+
+    kv_cache: the engine's pool [2, L, num_blocks, block_size, Hkv, D], or any
+    contiguous tensor whose last four dimensions are those (one layer's k_cache,
+    say), of any type; a block's bytes a multiple of 16.  src and dst: equally
+    many block ids, host data (lists or CPU tensors), read before the call
+    returns.  One block may be copied to several, but a destination may not
+    appear twice, nor be a source (ValueError)."""
+    assert kv_cache.dim() >= 4 and kv_cache.is_contiguous(), "kv_cache must be contiguous [..., NB, BS, Hkv, D]"
+    _on_gpu(kv_cache)
+    s, d = _block_ids(src, "src"), _block_ids(dst, "dst")
+    assert len(s) == len(d), f"src and dst must have the same length, got {len(s)} and {len(d)}"
+    NB, BS, Hkv, D = kv_cache.shape[-4:]
+    block = BS * Hkv * D * kv_cache.element_size()
+    if not len(s):
+        return
+    planes = kv_cache.numel() * kv_cache.element_size() // max(1, NB * block)
+    _launch("copy_kv_blocks", _lib.load().lfs_copy_kv_blocks, kv_cache,
+            _ptr(kv_cache), planes, NB, block, s.buffer_info()[0], d.buffer_info()[0], len(s))
+
+
 BALANCED_MAX_BATCH = 8192  # the balanced split scans the batch's tile counts in LDS
 
 
@@ -447,10 +501,29 @@ def paged_decode_workspace_bytes(batch: int, num_q_heads: int, head_dim: int, ma
                                                             max_blocks, blocks_per_split))
 
 
+def paged_decode_window_workspace_bytes(batch: int, num_q_heads: int, head_dim: int) -> int:
+    return int(_lib.load().lfs_paged_decode_window_workspace_bytes(batch, num_q_heads, head_dim))
+
+
+MAX_WINDOW = 1 << 30  # a longer window, or more sinks, hide nothing of any context
+
+
+def _window_args(window: Optional[int], sinks: int) -> bool:
+    """Whether the attention is over a sliding window; raises on bad values."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks without a window hide nothing: give both, or neither")
+        return False
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be >= 1 and sinks >= 0, got {window} and {sinks}")
+    return True
+
+
 def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                            context_lens: torch.Tensor, block_tables: torch.Tensor,
                            scale: Optional[float] = None, blocks_per_split: Optional[int] = None,
-                           workspace: Optional[torch.Tensor] = None, quant: bool = False):
+                           workspace: Optional[torch.Tensor] = None, quant: bool = False,
+                           window: Optional[int] = None, sinks: int = 0):
     """One decode step of GQA attention over a paged KV pool.
 
     q: bf16 [B, Hq, D]; caches bf16 [num_blocks, block_size, Hkv, D];
@@ -468,7 +541,14 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     for the next FP8 linear and the call returns (o, codes e4m3fn
     [B, Hq*D], scales fp32 [B, Hq*D/128]), the codes equal to
     act_quant(o.view(B, -1)) bit for bit.
+    With ``window`` (>= 1) a token sees only the last ``window`` tokens of
+    its context, itself among them, and the first ``sinks`` ones; the others
+    are never read, and table entries of blocks that hold no visible token
+    may be -1.  The kernel then splits the work itself (``blocks_per_split``
+    must be None); a ``workspace`` takes
+    ``paged_decode_window_workspace_bytes`` bytes.
     """
+    windowed = _window_args(window, sinks)
     assert q.dim() == 3 and q.is_contiguous(), "q must be contiguous [B, Hq, D]"
     assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape == v_cache.shape
     assert k_cache.dim() == 4, "caches must be [num_blocks, block_size, Hkv, D]"
@@ -486,6 +566,21 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     max_blocks = block_tables.size(1)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
+    if windowed:
+        assert blocks_per_split is None, "blocks_per_split does not go with a window"
+        need = paged_decode_window_workspace_bytes(B, Hq, D)
+        if workspace is None:
+            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+        o = torch.empty_like(q)
+        oq = os_ = None
+        if quant:
+            oq = torch.empty(B, Hq * D, dtype=FP8, device=q.device)
+            os_ = torch.empty(B, Hq * D // 128, dtype=torch.float32, device=q.device)
+        _launch("paged_attention_decode", _lib.load().lfs_paged_decode_window, q,
+                _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(context_lens), _ptr(block_tables), block_tables.stride(0),
+                _ptr(o), _ptr(workspace), workspace.numel() * workspace.element_size(), B, Hq, Hkv, D, BS, NB, max_blocks,
+                min(window, MAX_WINDOW), min(sinks, MAX_WINDOW), float(scale), _ptr(oq), _ptr(os_))
+        return (o, oq, os_) if quant else o
     if blocks_per_split is None:
         bps = default_blocks_per_split(B, Hkv, max_blocks, BS, quant_values=(Hq // Hkv) * D if quant else 0)
     else:
@@ -635,7 +730,8 @@ def paged_attention_decode_noalloc(q: torch.Tensor, k_cache: torch.Tensor, v_cac
 def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                            cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor,
                            max_seqlen_q: int, max_seqlen_k: int, softmax_scale: Optional[float] = None,
-                           causal: bool = True, block_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+                           causal: bool = True, block_table: Optional[torch.Tensor] = None,
+                           window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """Varlen causal prefill attention, the call engine/model_runner.py:291-292
     of the reference names for its prefill step (same argument meaning).
 
@@ -646,7 +742,13 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     Hkv, D].  Queries of sequence i sit at the last lq positions of its lk
     keys and attend to keys up to their own position.  max_seqlen_k chooses the
     tiles and never the result: any value is taken.  softmax_scale
-    defaults to 1/sqrt(D).  Returns bf16 [total_q, Hq, D]."""
+    defaults to 1/sqrt(D).  Returns bf16 [total_q, Hq, D].
+
+    With ``window`` (>= 1) a query sees only the last ``window`` keys up to
+    its own position and the first ``sinks`` keys of its sequence.  Keys that
+    no query of the call sees are never read, and table entries of blocks
+    that hold only such keys may be -1; values of all others must be finite."""
+    windowed = _window_args(window, sinks)
     assert causal, "only causal prefill attention is provided"
     assert q.dim() == 3 and q.is_contiguous(), "q must be contiguous [total_q, Hq, D]"
     assert k.is_contiguous() and v.is_contiguous() and k.shape == v.shape
@@ -673,6 +775,15 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     assert Dk == D, "head_dim mismatch between q and k"
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
+    if windowed:
+        if q.numel() == 0 or k.numel() == 0:  # no query, or none that sees a key
+            return torch.zeros_like(q)
+        o = torch.empty_like(q)
+        _launch("flash_attn_varlen_func", _lib.load().lfs_prefill_attention_window, q,
+                _ptr(q), _ptr(k), _ptr(v), _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), bt_ptr, bt_stride, BS, num_slots,
+                _ptr(o), B, Hq, Hkv, D, int(max_seqlen_q), min(window, MAX_WINDOW), min(sinks, MAX_WINDOW),
+                float(softmax_scale))
+        return o
     # a hint only: whatever is not a whole number (None, a device scalar, whose
     # value would take a synchronisation) counts as "long"
     max_k = max(-1, min(int(max_seqlen_k), 2 ** 31 - 1)) if isinstance(max_seqlen_k, numbers.Integral) else 2 ** 31 - 1
@@ -745,6 +856,47 @@ def sample_gumbel(logits: torch.Tensor, temperatures: torch.Tensor, seed: int, o
                                    _ptr(noise) if noise is not None else None, _ptr(ws), ws.numel(), _stream(logits))
     _lib.check(rc, "sample_gumbel")
     return (out, noise) if return_noise else out
+
+
+def sample_filtered(logits: torch.Tensor, temperatures: torch.Tensor, uniforms: torch.Tensor,
+                    top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                    min_p: Optional[torch.Tensor] = None, return_logprob: bool = False):
+    """A token per row by temperature, top-k, top-p and min-p, from given
+    uniform numbers.
+
+    logits: bf16 [B, V] (unit column stride); temperatures fp32 [B] (<= 0: the
+    largest logit); uniforms fp32 [B] in [0, 1).  The row's tokens are ordered
+    by logit, largest first, equal ones by index, and weigh w = exp((x - x_max)
+    / T).  ``top_k`` (int32 [B]; <= 0: off) keeps the first k; ``top_p`` (fp32
+    [B]; >= 1: off) of those the shortest prefix whose weight reaches top_p of
+    theirs; ``min_p`` (fp32 [B]; <= 0: off) of those the tokens with w >= min_p.
+    The first token is always kept.  Drawn is the first token of the order at
+    which the kept weight summed so far exceeds u times all of it.  Tokens at
+    -infinity or NaN are never drawn (a row of them alone gives token 0).
+    Returns int64 [B], with ``return_logprob`` also the fp32 [B] logarithms of
+    the drawn tokens' shares of the kept weight."""
+    assert logits.dim() == 2 and logits.stride(1) == 1, "logits must be [B, V] with unit column stride"
+    _on_gpu(logits, temperatures, uniforms)
+    _dtype(logits, torch.bfloat16, "logits")
+    B, V = logits.shape
+    if logits.stride(0) < V:  # broadcast rows (an expanded view): give each row its own copy
+        logits = logits.contiguous()
+    rows = [temperatures, uniforms, top_k, top_p, min_p]
+    for i, (t, dt, n) in enumerate(zip(rows, _SAMPLE_TYPES, ("temperatures", "uniforms", "top_k", "top_p", "min_p"))):
+        if t is not None:
+            if t.get_device() != logits.get_device():
+                _on_gpu(logits, t)
+            _dtype(t, dt, n)
+            assert t.shape == (B,), f"{n} must be [B]"
+            rows[i] = t.contiguous()
+    out = torch.empty(B, dtype=torch.int64, device=logits.device)
+    logprob = torch.empty(B, dtype=torch.float32, device=logits.device) if return_logprob else None
+    _launch("sample_filtered", _lib.load().lfs_sample_filtered, logits,
+            _ptr(logits), logits.stride(0), *map(_ptr, rows), B, V, _ptr(out), _ptr(logprob))
+    return (out, logprob) if return_logprob else out
+
+
+_SAMPLE_TYPES = (torch.float32, torch.float32, torch.int32, torch.float32, torch.float32)
 
 
 # ------------------------------------------------- fused decode-step rows --
@@ -890,6 +1042,56 @@ def qk_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torc
         _ptr(slot_mapping), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k), _ptr(v), T, num_q_heads, num_kv_heads, D,
         num_slots, cos_sin.size(0), float(eps), _stream(qkv))
     _lib.check(rc, "qk_norm_rope_store")
+    return (q, k, v) if return_kv else q
+
+
+def qk_head_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                            cos_sin: torch.Tensor, positions: torch.Tensor, num_q_heads: int, num_kv_heads: int,
+                            eps: float, k_cache: Optional[torch.Tensor] = None,
+                            v_cache: Optional[torch.Tensor] = None,
+                            slot_mapping: Optional[torch.Tensor] = None, return_kv: bool = False):
+    """qk_norm_rope_store with every query and key head normalised by itself
+    (RMSNorm over its D values, weights fp32 [D] shared by the heads), in fp32
+    throughout, and the first R dims of a head rotated (half-split within
+    them; the others keep their norm).
+
+    qkv: bf16 [T, (Hq + 2 Hkv) * D] (rows may be strided), D 64 or 128;
+    cos_sin: fp32 [max_pos, R] = cat(cos, sin), R a multiple of 16, at most D;
+    positions int64 [T]; caches bf16 [NB, BS, Hkv, D] and slot_mapping int64
+    [T] (-1 = skip), or None.  Returns q: bf16 [T, Hq, D]; with ``return_kv``
+    (q, k, v), k and v bf16 [T, Hkv, D] as written to the slots."""
+    assert qkv.dim() == 2 and qkv.stride(1) == 1
+    T, width = qkv.shape
+    heads = num_q_heads + 2 * num_kv_heads
+    D = width // heads
+    assert width == heads * D, "qkv width mismatch"
+    _on_gpu(qkv, q_weight, k_weight, cos_sin, positions)
+    _dtype(qkv, torch.bfloat16, "qkv")
+    for t, n in ((q_weight, "q_weight"), (k_weight, "k_weight"), (cos_sin, "cos_sin")):
+        _dtype(t, torch.float32, n)
+        assert t.is_contiguous(), f"{n} must be contiguous"
+    assert q_weight.shape == (D,) and k_weight.shape == (D,), "q_weight and k_weight must be [D]"
+    assert cos_sin.dim() == 2, "cos_sin must be [max_pos, R]"
+    _dtype(positions, torch.int64, "positions")
+    assert positions.numel() == T and positions.is_contiguous(), "positions must be [T]"
+    num_slots = 0
+    if slot_mapping is not None:
+        _on_gpu(qkv, k_cache, v_cache, slot_mapping)
+        _dtype(slot_mapping, torch.int64, "slot_mapping")
+        for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+            _dtype(t, torch.bfloat16, n)
+            assert t.is_contiguous() and t.dim() == 4 and t.shape[2:] == (num_kv_heads, D), \
+                f"{n} must be [NB, BS, Hkv, D]"
+        assert v_cache.shape == k_cache.shape
+        assert slot_mapping.numel() == T and slot_mapping.is_contiguous()
+        num_slots = k_cache.shape[0] * k_cache.shape[1]
+    q = torch.empty(T, num_q_heads, D, dtype=torch.bfloat16, device=qkv.device)
+    k = torch.empty(T, num_kv_heads, D, dtype=torch.bfloat16, device=qkv.device) if return_kv else None
+    v = torch.empty_like(k) if return_kv else None
+    _launch("qk_head_norm_rope_store", _lib.load().lfs_qk_head_norm_rope_store, qkv,
+            _ptr(qkv), qkv.stride(0) if T > 1 else width, _ptr(q_weight), _ptr(k_weight), _ptr(cos_sin), cos_sin.size(1),
+            _ptr(positions), _ptr(slot_mapping), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k), _ptr(v), T, num_q_heads,
+            num_kv_heads, D, num_slots, cos_sin.size(0), float(eps))
     return (q, k, v) if return_kv else q
 
 

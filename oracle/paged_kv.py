@@ -145,3 +145,33 @@ def prefill_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, block_tables=N
         out[qs:qe] = sdpa(q[qs:qe].transpose(1, 0, 2), Kh, Vh, mask=mask, scale=scale,
                           dtype=dtype).transpose(1, 0, 2)
     return out
+
+
+def window_mask(positions, keys, window, sinks):
+    """[len(positions), keys]: whether the query at a position sees a key:
+    those up to itself that are among the last ``window`` or the first
+    ``sinks``."""
+    p = np.asarray(positions)[:, None]
+    j = np.arange(keys)[None, :]
+    return (j <= p) & ((j > p - window) | (j < sinks))
+
+
+def window_attention(q, K, V, positions, scale, window, sinks):
+    """One sequence over a sliding window with sinks, in 64 bits: q [lq, Hq, D]
+    at ``positions`` over K and V [lk, Hkv, D]; a query that sees no key gives
+    0, and hidden values take no part.  Returns (o, a): the output [lq, Hq, D]
+    and the same sum over |v|, by which a rounding of the weights moves it."""
+    q, K, V = (np.asarray(x, np.float64) for x in (q, K, V))
+    lq, Hq, D = q.shape
+    G = Hq // K.shape[1]
+    mask = window_mask(positions, K.shape[0], window, sinks)
+    seen = mask.any(0)
+    K, V, mask = K[seen], V[seen], mask[:, seen]
+    o, a = np.zeros_like(q), np.zeros_like(q)
+    for h in range(Hq):
+        s = np.where(mask, q[:, h] @ K[:, h // G].T * scale, -np.inf)
+        m = s.max(-1, keepdims=True, initial=-np.inf)
+        e = np.where(mask, np.exp(s - np.where(np.isfinite(m), m, 0)), 0)
+        w = e / np.maximum(e.sum(-1, keepdims=True), 1e-300)
+        o[:, h], a[:, h] = w @ V[:, h // G], w @ np.abs(V[:, h // G])
+    return o, a

@@ -73,3 +73,31 @@ def sample_gumbel(logits, temperatures, noise, dtype=np.float64):
     p = p / p.sum(axis=1, keepdims=True)
     score = p / np.maximum(np.asarray(noise, dtype), 1e-10)
     return score.argmax(axis=1), score
+
+
+def sample_filtered(logits, temperature, u, top_k=0, top_p=1.0, min_p=0.0):
+    """One row in 64 bits: (token, log of its share of the kept weight).  The
+    tokens are ordered by logit, largest first, equal ones by index; kept are
+    the first top_k, of those the shortest prefix that reaches top_p of their
+    weight, of those the ones with at least min_p of the largest weight; drawn
+    is the first at which the kept weight summed so far exceeds u of it."""
+    x = np.asarray(logits, np.float64)
+    valid = np.flatnonzero(x > -np.inf)  # no NaN either
+    if not len(valid):
+        return 0, -np.inf
+    order = valid[np.argsort(-x[valid], kind="stable")]
+    if not temperature > 0:
+        top_k, temperature = 1, 1.0
+    s = x[order]
+    with np.errstate(invalid="ignore"):
+        e = np.where(s == s[0], 0.0, (s - s[0]) / np.float64(temperature))
+    w = np.exp(np.where(np.isnan(e), -np.inf, e))
+    n = min(top_k, len(w)) if top_k > 0 else len(w)
+    c = np.cumsum(w[:n])
+    if top_p < 1:
+        n = max(1, int(np.count_nonzero(np.concatenate([[0.0], c[:-1]]) < top_p * c[-1])))
+    if min_p > 0:
+        n = max(1, min(n, int(np.count_nonzero(w >= min_p))))
+    c = np.cumsum(w[:n])
+    i = min(int(np.count_nonzero(c <= u * c[-1])), n - 1)
+    return int(order[i]), e[i] - np.log(c[-1])
