@@ -22,7 +22,7 @@ REPO = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "liblfs_kernels.so"
 SOURCES = ["capi.hip", "quant.hip", "fp8_gemm.hip", "paged_kv.hip", "fused.hip", "prefill.hip", "sampler.hip", "indexer.hip", "moe.hip",
-           "window.hip", "kv_blocks.hip", "head_norm.hip", "sample_filtered.hip"]
+           "paged_window.hip", "kv_blocks.hip", "head_norm.hip", "sample_filtered.hip"]
 # benchmark instrument (the decode's read ceiling), a library of its own that
 # nothing in the package loads: only bench.py does
 PROBE_PATH = PKG_DIR / "liblfs_probe.so"

@@ -212,12 +212,17 @@ __device__ __forceinline__ bool ranked_item(const int32_t* cu_q, const int32_t* 
   return true;
 }
 
-template <int D, bool PAGED>
+// WIN: a query at position p sees the keys t <= p with t > p - window or t <
+// sinks.  The workgroup walks the tiles of the sinks and those from its first
+// row's window on; keys in between, and within those tiles, that none of its
+// rows sees are never read (their blocks may be freed): their places hold a
+// visible key's row, masked.
+template <int D, bool PAGED, bool WIN>
 __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, const int32_t* __restrict__ bt,
     int64_t bt_stride, int64_t num_slots, uint16_t* __restrict__ out, Div dB, Div dHkv, Div G, Div dBS,
-    int rtiles, int xshift, float scale_log2) {
+    int rtiles, int xshift, float scale_log2, int window, int sinks) {
   constexpr int NDC = D / 16;            // 16-dim MFMA k steps of S
   constexpr int NDB = D / 32;            // 32-dim blocks of O^T
   constexpr int RB = 2 * D;              // bytes of a tile row
@@ -271,6 +276,19 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
                         ? -1 : __builtin_amdgcn_readfirstlane(off + (int)(min(r0 + RW * wave + RW - 1, rows - 1) / G));
   const int wlast = off + (int)(min(r0 + RW * NW - 1, rows - 1) / G);
   const int nkt = min(lk, wlast + 1) <= 0 ? 0 : (min(lk, wlast + 1) + KT - 1) / KT;
+  // WIN: the workgroup's hidden keys hlo .. hhi - 1, its tiles of sinks (0 ..
+  // ns - 1) and its window's first; a wave's rows all miss the keys to pmiss
+  int hlo = 0, hhi = 0, ns = 0, tw = 0, pmiss = 0;
+  if constexpr (WIN) {
+    hhi = max(0, off + (int)(r0 / G) - window + 1);
+    hlo = min(sinks, hhi);
+    if (hlo == hhi) hlo = hhi = 0;
+    tw = hhi / KT;
+    ns = min((hlo + KT - 1) / KT, tw);
+    pmiss = pfirst - window;
+  }
+  const int nt = WIN ? ns + max(0, nkt - tw) : nkt;
+  auto tile_key = [&](int j) { return (!WIN || j < ns ? j : j - ns + tw) * KT; };
   const int64_t rowb = (int64_t)Hkv * RB;  // bytes per token of k / v
   const uint8_t* kb = reinterpret_cast<const uint8_t*>(k) + (int64_t)kh * RB;
   const uint8_t* vb = reinterpret_cast<const uint8_t*>(v) + (int64_t)kh * RB;
@@ -295,25 +313,50 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
   // an invalid table entry reads slot 0.  The entry is loaded one tile ahead.
   const int hoff = (RPW * wave) & ~15;  // the wave's half within a tile
   int blk = 0, boff = 0, lblk = 0, loff = 0;  // block and offset of the half's first key, and of key lk - 1
-  if constexpr (PAGED) {
+  // WIN: the key in the place of the first of the half at key t: key hhi for a
+  // half that nobody sees
+  auto half_key = [&](int t) { return t >= lk ? max(lk - 1, 0) : t >= hlo && t + 16 <= hhi ? hhi : t; };
+  if constexpr (PAGED && !WIN) {
     boff = hoff;
     while (boff >= BS) boff -= BS, ++blk;
     lblk = (int)((unsigned)max(lk - 1, 0) / dBS), loff = max(lk - 1, 0) - lblk * BS;
   }
   auto entry = [&](int t) -> int {  // table entry of the half that starts at key t
-    int64_t e = (int64_t)i * bt_stride + min((int64_t)(t < lk ? blk : lblk), bt_stride - 1);
+    if constexpr (WIN) {
+      const int key = half_key(t);
+      blk = (int)((unsigned)key / dBS);
+      boff = key - blk * BS;
+    }
+    int64_t e = (int64_t)i * bt_stride + min((int64_t)(WIN || t < lk ? blk : lblk), bt_stride - 1);
     asm volatile("" : "+v"(e));  // a vector load: it returns before the barrier, with the copies
     return bt[e];
   };
   int next = 0;
-  if constexpr (PAGED) next = entry(hoff);
+  if constexpr (PAGED) next = entry(tile_key(0) + hoff);
   // copies of the K or V rows of the tile at key t0 into buffer buf (0 / 1;
   // V tiles are buffers 2 / 3); first: token or slot of its local row 0
   auto fetch = [&](const uint8_t* base, int64_t first, int t0, int buf, const unsigned (&rows16)[NC]) {
     const int valid = PAGED ? max(0, lk - 1 - (t0 + hoff)) : lk - 1 - t0;  // last local row that may be read
     const uint8_t* p = base + first * rowb;
     const unsigned dst = lbase + buf * TB + RPW * wave * RB;
-    if (valid >= (PAGED ? 15 : KT - 1)) {
+    const int th = t0 + hoff;  // the wave's first key
+    if (WIN && th < hhi && th + 16 > hlo) {
+      // hidden keys among the wave's 16, whose places take a visible row of
+      // theirs: the last sink's, else the window's first (a half that nobody
+      // sees has that as its row 0)
+      const int key0 = PAGED ? th : t0;  // of local row 0
+      const bool none = PAGED && th >= hlo && th + 16 <= hhi;
+      unsigned at[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int r = crow0 + RPC * c, key = key0 + r;
+        int to = min(r, valid);
+        if (none) to = 0;
+        else if (key >= hlo && key < hhi) to = (key0 < hlo ? hlo - 1 : hhi) - key0;
+        at[c] = rows16[c] + (unsigned)(to - r) * (unsigned)rowb;
+      }
+      copy_rows<NC>(p, at, dst);
+    } else if (valid >= (PAGED ? 15 : KT - 1)) {
       copy_rows<NC>(p, rows16, dst);
     } else {
       unsigned at[NC];
@@ -324,17 +367,19 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
     }
   };
   int64_t kfirst = 0;  // local row 0 of the K tile last fetched
-  auto fetch_k = [&](int t0, int buf) {
+  auto fetch_k = [&](int t0, int t1, int buf) {  // t1: key of the tile after it
     if constexpr (PAGED) {
       const int b = __builtin_amdgcn_readfirstlane(next);
-      kfirst = b < 0 || (int64_t)b * BS >= num_slots ? 0 : (int64_t)b * BS + (t0 + hoff < lk ? boff : loff);
-      boff += KT;
-      while (boff >= BS) boff -= BS, ++blk;
+      kfirst = b < 0 || (int64_t)b * BS >= num_slots ? 0 : (int64_t)b * BS + (WIN || t0 + hoff < lk ? boff : loff);
+      if constexpr (!WIN) {
+        boff += KT;
+        while (boff >= BS) boff -= BS, ++blk;
+      }
     } else {
       kfirst = (int64_t)k0 + t0;
     }
     fetch(kb, kfirst, t0, buf, krow);
-    if constexpr (PAGED) next = entry(t0 + KT + hoff);
+    if constexpr (PAGED) next = entry(t1 + hoff);
   };
 
   // Q^T (B operand): lane l supplies row l % 32, dims 16c + 8h .. +7
@@ -364,7 +409,8 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
   // position below 0), so that it ends as 0; else the running maximum, also
   // where that stays -infinity (every score overflowed), which makes the row
   // NaN, as a softmax over it is.
-  const float m_none = qp < 0 ? 0.f : -INFINITY;
+  // WIN: 0 until a visible key's score passes -infinity; the row ends as NaN if none does.
+  const float m_none = WIN || qp < 0 ? 0.f : -INFINITY;
   float m_exp = m_none;
   float alpha = 1.f;   // the tile's rescaling of O and of the sum
   // the causal mask, only where the tile reaches past the wave's first row;
@@ -372,12 +418,14 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
   auto mask_max = [&](v16f (&s)[NB], int t0) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) s[b] *= scale_log2;
-    if (t0 + KT - 1 > pfirst) {
+    if (t0 + KT - 1 > pfirst || (WIN && t0 <= plast - window && t0 + KT > sinks)) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (t0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4 > qp) s[b][r] = -INFINITY;
+        for (int r = 0; r < 16; ++r) {
+          const int key = t0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4;
+          if (key > qp || (WIN && key <= qp - window && key >= sinks)) s[b][r] = -INFINITY;
+        }
     }
     float mx = s[0][0];
 #pragma unroll
@@ -423,12 +471,12 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
   };
   constexpr int NS = NB * NDC, NP = KT / 16 * NDB;  // MFMAs of S^T and of O^T per tile
   constexpr int AH = 4;                             // operand reads ahead of them
-  if (nkt > 0) {
-    fetch_k(0, 0);
-    fetch(vb, kfirst, 0, 2, vrow);
+  if (nt > 0) {
+    fetch_k(tile_key(0), tile_key(1), 0);
+    fetch(vb, kfirst, tile_key(0), 2, vrow);
   }
-  for (int j = 0; j < nkt; ++j) {
-    const int t0 = j * KT, buf = j & 1;
+  for (int j = 0; j < nt; ++j) {
+    const int t0 = tile_key(j), buf = j & 1;
     // tile j is in LDS for every wave; every wave is done with tile j - 1,
     // whose buffers the next copies fill
     __builtin_amdgcn_s_waitcnt(0);
@@ -437,10 +485,11 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
 #pragma unroll
     for (int n = 0; n < AH; ++n) kf[n] = k_frag(n, buf);
     __builtin_amdgcn_sched_barrier(0);
-    if (j + 1 < nkt) {
-      fetch_k(t0 + KT, buf ^ 1);
-      fetch(vb, kfirst, t0 + KT, 2 + (buf ^ 1), vrow);
+    if (j + 1 < nt) {
+      fetch_k(tile_key(j + 1), tile_key(j + 2), buf ^ 1);
+      fetch(vb, kfirst, tile_key(j + 1), 2 + (buf ^ 1), vrow);
     }
+    if (WIN && t0 + KT - 1 <= pmiss && t0 >= sinks) continue;  // none of the wave's rows sees a key
     if (t0 > plast) continue;  // the wave's rows end before this tile (it still copies)
     v16f s[NB];
     uint32_t pw[NB][8];
@@ -482,7 +531,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
   __syncthreads();  // every wave is done with the K and V tiles
   const unsigned ob = lbase + wave * (RW * RB);
   {
-    const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+    const float inv = l_run > 0.f ? 1.f / l_run : !WIN || qp < 0 ? 0.f : NAN;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -775,6 +824,25 @@ inline bool prefill_short(bool paged, int64_t B, int Hq, int G, int D, int64_t m
   return G >= 2 && G <= 6 && w * t <= 2304;
 }
 
+// Grid of prefill_attention_kernel: row tiles of the longest prompt, kv heads
+// dealt to the XCDs.
+struct PrefillGrid {
+  int64_t rtiles;
+  int xshift;
+  dim3 grid;
+  bool ok;
+};
+inline PrefillGrid prefill_grid(int64_t B, int Hkv, int G, int64_t max_seqlen_q) {
+  PrefillGrid p;
+  p.rtiles = (max_seqlen_q * G + RW * NW - 1) / (RW * NW);
+  p.xshift = Hkv <= 8 && 8 % Hkv == 0 ? __builtin_ctz(8 / Hkv) : -1;
+  const int64_t nt = p.xshift > 0 ? (p.rtiles + (1 << p.xshift) - 1) >> p.xshift << p.xshift : p.rtiles;
+  p.ok = B * nt < ((1ll << 31) - kGridX) / Hkv && Hkv < 65536;
+  const int64_t wgs = B * nt * Hkv;
+  p.grid = dim3((unsigned)(wgs < kGridX ? wgs : kGridX), (unsigned)((wgs + kGridX - 1) / kGridX));
+  return p;
+}
+
 }  // namespace
 }  // namespace lfs
 
@@ -808,12 +876,8 @@ extern "C" int lfs_prefill_attention_max_k(const void* q, const void* k, const v
                 "prefill_attention: bad paged KV geometry (block_size must be a multiple of 16)");
   }
   const int G = Hq / Hkv;
-  const int64_t rtiles = ((int64_t)max_seqlen_q * G + RW * NW - 1) / (RW * NW);
-  const int xshift = Hkv <= 8 && 8 % Hkv == 0 ? __builtin_ctz(8 / Hkv) : -1;
-  const int64_t nt = xshift > 0 ? (rtiles + (1 << xshift) - 1) >> xshift << xshift : rtiles;
-  LFS_REQUIRE(B * nt < ((1ll << 31) - kGridX) / Hkv && Hkv < 65536, "prefill_attention: grid too large");
-  const int64_t wgs = B * nt * Hkv;
-  const dim3 grid((unsigned)(wgs < kGridX ? wgs : kGridX), (unsigned)((wgs + kGridX - 1) / kGridX));
+  const PrefillGrid pg = prefill_grid(B, Hkv, G, max_seqlen_q);
+  LFS_REQUIRE(pg.ok, "prefill_attention: grid too large");
   const float sl2 = scale * 1.4426950408889634f;
   hipStream_t st = (hipStream_t)stream;
   if (prefill_short(block_tables != nullptr, B, Hq, G, D, max_seqlen_q, max_seqlen_k)) {
@@ -841,10 +905,10 @@ extern "C" int lfs_prefill_attention_max_k(const void* q, const void* k, const v
   }
   const Div dBS = div_by(block_tables != nullptr ? block_size : 1);
 #define LFS_PF(DD, PG)                                                                                             \
-  hipLaunchKernelGGL((prefill_attention_kernel<DD, PG>), grid, dim3(64 * NW), 0, st, (const uint16_t*)q,        \
+  hipLaunchKernelGGL((prefill_attention_kernel<DD, PG, false>), pg.grid, dim3(64 * NW), 0, st, (const uint16_t*)q,        \
                      (const uint16_t*)k, (const uint16_t*)v, cu_seqlens_q, cu_seqlens_k, block_tables,             \
                      PG ? bt_stride : 0, num_slots, (uint16_t*)out, div_by((unsigned)B), div_by(Hkv), div_by(G),   \
-                     dBS, (int)rtiles, xshift, sl2)
+                     dBS, (int)pg.rtiles, pg.xshift, sl2, 0, 0)
   if (block_tables != nullptr) {
     if (D == 64) LFS_PF(64, true);
     else LFS_PF(128, true);
@@ -854,4 +918,45 @@ extern "C" int lfs_prefill_attention_max_k(const void* q, const void* k, const v
   }
 #undef LFS_PF
   return check_launch("prefill_attention");
+}
+
+extern "C" int lfs_prefill_attention_window(const void* q, const void* k, const void* v, const int32_t* cu_seqlens_q,
+                                            const int32_t* cu_seqlens_k, const int32_t* block_tables,
+                                            int64_t bt_stride, int32_t block_size, int64_t num_slots, void* out,
+                                            int64_t B, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                            int32_t max_seqlen_q, int32_t window, int32_t sinks, float scale,
+                                            void* stream) {
+  const int Hq = num_q_heads, Hkv = num_kv_heads, D = head_dim;
+  LFS_REQUIRE(B >= 0 && Hq > 0 && Hkv > 0 && max_seqlen_q >= 0, "prefill_attention_window: bad shape");
+  LFS_REQUIRE(D == 64 || D == 128, "prefill_attention_window: head_dim must be 64 or 128 (got %d)", D);
+  LFS_REQUIRE(Hq % Hkv == 0 && Hq / Hkv <= 8,
+              "prefill_attention_window: num_q_heads (%d) must be a multiple of num_kv_heads (%d), ratio <= 8", Hq, Hkv);
+  LFS_REQUIRE(window >= 1 && sinks >= 0, "prefill_attention_window: window must be >= 1 and sinks >= 0 (got %d, %d)",
+              window, sinks);
+  if (B == 0 || max_seqlen_q == 0) return 0;
+  LFS_REQUIRE(q && k && v && cu_seqlens_q && cu_seqlens_k && out, "prefill_attention_window: null pointer");
+  LFS_REQUIRE(((((uintptr_t)q) | ((uintptr_t)k) | ((uintptr_t)v) | ((uintptr_t)out)) & 15u) == 0,
+              "prefill_attention_window: q, k, v and out must be 16-byte aligned");
+  const bool paged = block_tables != nullptr;
+  if (paged)
+    LFS_REQUIRE(block_size > 0 && block_size % 16 == 0 && num_slots >= block_size && bt_stride > 0,
+                "prefill_attention_window: bad paged KV geometry (block_size must be a multiple of 16)");
+  const int G = Hq / Hkv;
+  const PrefillGrid pg = prefill_grid(B, Hkv, G, max_seqlen_q);
+  LFS_REQUIRE(pg.ok, "prefill_attention_window: grid too large");
+  const float sl2 = scale * 1.4426950408889634f;
+#define LFS_PW(DD, PG)                                                                                                \
+  hipLaunchKernelGGL((prefill_attention_kernel<DD, PG, true>), pg.grid, dim3(64 * NW), 0, (hipStream_t)stream,       \
+                     (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, cu_seqlens_q, cu_seqlens_k,          \
+                     block_tables, PG ? bt_stride : 0, num_slots, (uint16_t*)out, div_by((unsigned)B), div_by(Hkv),    \
+                     div_by(G), div_by(PG ? block_size : 1), (int)pg.rtiles, pg.xshift, sl2, window, sinks)
+  if (paged) {
+    if (D == 64) LFS_PW(64, true);
+    else LFS_PW(128, true);
+  } else {
+    if (D == 64) LFS_PW(64, false);
+    else LFS_PW(128, false);
+  }
+#undef LFS_PW
+  return check_launch("prefill_attention_window");
 }
