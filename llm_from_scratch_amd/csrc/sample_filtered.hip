@@ -31,7 +31,7 @@
 namespace lfs {
 namespace {
 
-constexpr int FNT = 1024;            // threads
+constexpr int FNT = 512;             // threads: 256 registers each, room for the row and the cuts
 constexpr int FNW = FNT / 64;
 constexpr int kBins = 65536;
 constexpr int kChunk = 128;          // bins of a chunk: two per lane
@@ -50,14 +50,29 @@ __device__ __forceinline__ int bin_of(uint32_t h) {
 __device__ __forceinline__ uint32_t bits_of(int d) { return d < 0x8000 ? 0x7FFFu - d : (uint32_t)d; }
 __device__ __forceinline__ double bin_value(int d) { return (double)bf16_to_f32(bits_of(d)); }
 
-// The weights of a row.
+// The weights of a row: 2^((x - x_max) log2(e) / T), by its Taylor series at
+// the exponent's nearest whole number (|f ln 2| <= 0.35: the first term left out
+// is below 2^-52).  Weights below 2^-1000 count as 0.
 struct Weights {
   int top;  // the largest logit's bin
-  double xmax, T;
+  double xmax, c;
   __device__ __forceinline__ double at(int d) const {
-    if (d == top) return 1.0;
-    const double w = exp((bin_value(d) - xmax) / T);
-    return w == w ? w : 0.0;  // infinite logit and temperature
+    const double t = (bin_value(d) - xmax) * c, n = rint(t), f = (t - n) * 0.6931471805599453;
+    double w = 1.0 / 479001600;
+    w = fma(w, f, 1.0 / 39916800);
+    w = fma(w, f, 1.0 / 3628800);
+    w = fma(w, f, 1.0 / 362880);
+    w = fma(w, f, 1.0 / 40320);
+    w = fma(w, f, 1.0 / 5040);
+    w = fma(w, f, 1.0 / 720);
+    w = fma(w, f, 1.0 / 120);
+    w = fma(w, f, 1.0 / 24);
+    w = fma(w, f, 1.0 / 6);
+    w = fma(w, f, 0.5);
+    w = fma(w, f, 1.0);
+    w = fma(w, f, 1.0);
+    w = t > -1000.0 ? ldexp(w, (int)n) : 0.0;  // NaN (an infinite logit and temperature): 0
+    return d == top ? 1.0 : w;
   }
 };
 
@@ -92,53 +107,22 @@ __device__ __forceinline__ uint32_t lane_u(uint32_t v, int lane) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
-// 64 * N entries of a wave in order (entry N * lane + i), each a count and a
-// weight, and their sums before the lane's first.
-template <int N>
-struct Entries {
-  uint32_t n[N], nb;
-  double w[N], wb;
-  __device__ __forceinline__ void scan() {
-    uint32_t ns = 0;
-    double ws = 0.0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) ns += n[i], ws += w[i];
-    nb = scan_sum(ns) - ns;
-    wb = __shfl_up(scan_sum(ws), 1, 64);
-    if ((threadIdx.x & 63) == 0) wb = 0.0;
-  }
-  // The first entry that is not empty and at whose end pred(count, weight)
-  // holds of the sums so far, which start at c and m; the last one that is not
-  // empty where none does (-1: all are empty).  c and m become the sums before
-  // it.
-  template <class Pred>
-  __device__ __forceinline__ int find(uint32_t& c, double& m, Pred&& pred) const {
-    uint32_t cb = c + nb;
-    double mb = m + wb;
-    int hit = -1, last = -1;  // in the lane
-    uint32_t hc = 0, lc = 0;
-    double hm = 0.0, lm = 0.0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (n[i] != 0) {
-        if (hit < 0 && pred(cb + n[i], mb + w[i])) hit = i, hc = cb, hm = mb;
-        last = i, lc = cb, lm = mb;
-      }
-      cb += n[i], mb += w[i];
-    }
-    uint64_t any = __ballot(hit >= 0);
-    if (any == 0) {
-      any = __ballot(last >= 0);
-      if (any == 0) return -1;
-      any = 1ull << (63 - __builtin_clzll(any));
-      hit = last, hc = lc, hm = lm;
-    }
-    const int src = __builtin_ctzll(any);
-    c = lane_u(hc, src);
-    m = lane_d(hm, src);
-    return N * src + (int)lane_u((uint32_t)hit, src);
-  }
-};
+// Sums over the lanes of each eight.
+template <class X>
+__device__ __forceinline__ X scan_sum8(X v) {
+  const int at = threadIdx.x & 7;
+  const X a = moved<0x111, 0xF>(v);  // row_shr: also from the eight before
+  v += at >= 1 ? a : X(0);
+  const X b = moved<0x112, 0xF>(v);
+  v += at >= 2 ? b : X(0);
+  const X c = moved<0x114, 0xF>(v);
+  return v + (at >= 4 ? c : X(0));
+}
+template <class X>
+__device__ __forceinline__ X before(X upto) {  // the lane before's; 0 in lane 0
+  const X v = __shfl_up(upto, 1, 64);
+  return (threadIdx.x & 63) == 0 ? X(0) : v;
+}
 
 // A place in the order: n tokens of bin d, after all of the bins before it;
 // c and m: their count and weight.
@@ -153,41 +137,97 @@ struct Filters {
   double p, m, u;
 };
 
-// The cuts and the draw, by one wave or by several alike.  hold(chunk, bins)
-// fills in a chunk's two bins per lane.  d: the drawn token's bin, nth: its
+// The last bin whose weight reaches m <= 1, 64 bins tried at a time.
+__device__ __forceinline__ int last_reaching(const Weights& wt, double m) {
+  const int lane = threadIdx.x & 63;
+  int lo = wt.top;
+#pragma unroll 1
+  for (int step = 1024; step > 0; step >>= step == 1024 ? 6 : 4) {  // 1024, 16, 1
+    const int mid = lo + step * (lane + 1);
+    const uint64_t in = __ballot(mid < kBins && wt.at(min(mid, kBins - 1)) >= m);
+    lo += step * (in == ~0ull ? 64 : __builtin_ctzll(~in));
+  }
+  return lo;
+}
+
+// The cuts and the draw, by one wave or by several alike.  hold_bins(chunk, n)
+// fills in a chunk's two bins per lane; lo: the last bin that reaches min-p
+// (where that is in (0, 1]).  d: the drawn token's bin, nth: its
 // place among the bin's tokens, S: the kept weight.
 template <class Hold>
-__device__ __forceinline__ void draw(const Weights& wt, const Filters& f, const uint32_t* cnt, const double* mass,
-                                     Hold&& hold_bins, int& d, uint32_t& nth, double& S) {
+__device__ __forceinline__ void draw(const Weights& wt, const Filters& f, int lo, const uint32_t* cnt,
+                                     const double* mass, Hold&& hold_bins, int& d, uint32_t& nth, double& S) {
   const int lane = threadIdx.x & 63;
-  Entries<CPL> ch;
+  // sums up to the end of the lane's CPL chunks
+  uint32_t lane_n = 0;
+  double lane_w = 0.0;
 #pragma unroll
-  for (int i = 0; i < CPL; ++i) ch.n[i] = cnt[CPL * lane + i], ch.w[i] = ch.n[i] != 0 ? mass[CPL * lane + i] : 0.0;
-  ch.scan();
-  Entries<2> bn;
+  for (int i = 0; i < CPL; ++i) {
+    const uint32_t n = cnt[CPL * lane + i];
+    lane_n += n;
+    lane_w += n != 0 ? mass[CPL * lane + i] : 0.0;
+  }
+  lane_n = scan_sum(lane_n);
+  lane_w = scan_sum(lane_w);
+  const uint32_t lane_nb = before(lane_n);
+  const double lane_wb = before(lane_w);
+  uint32_t n[2], upto_n = 0;  // of the chunk held: the lane's two bins, sums up to their end
+  double w[2], upto_w = 0.0;
   int held = -1;
   auto hold = [&](int chunk) {
     if (chunk == held) return;
     held = chunk;
-    hold_bins(chunk, bn.n);
+    hold_bins(chunk, n);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) bn.w[i] = bn.n[i] != 0 ? bn.n[i] * wt.at(chunk * kChunk + 2 * lane + i) : 0.0;
-    bn.scan();
+    for (int i = 0; i < 2; ++i) w[i] = n[i] != 0 ? n[i] * wt.at(chunk * kChunk + 2 * lane + i) : 0.0;
+    upto_n = scan_sum(n[0] + n[1]);
+    upto_w = scan_sum(w[0] + w[1]);
   };
-  // the first bin at whose end pred holds of the count and weight so far
+  // The first lane whose sums are not 0 and satisfy pred; the last that adds to
+  // them where none does.
+  auto first_lane = [&](bool some, bool hit) -> int {
+    const uint64_t any = __ballot(hit);
+    return any != 0 ? __builtin_ctzll(any) : 63 - __builtin_clzll(__ballot(some) | 1);
+  };
+  // the first bin that is not empty and at whose end pred(count, weight) holds
+  // of the sums so far; the last one that is not empty where none does
   auto find = [&](auto&& pred) -> Place {
+    const bool some = lane_n != lane_nb;  // the scan's sums of a lane without tokens may differ from the one before's
+    const int src = first_lane(some, some && pred(lane_n, lane_w));
+    const uint32_t cb = lane_u(lane_nb, src);
+    const double mb = lane_d(lane_wb, src);
+    const int at8 = lane & (CPL - 1);
+    const uint32_t cn = cnt[CPL * src + at8];
+    const uint32_t c_upto = cb + scan_sum8(cn);
+    const double m_upto = mb + scan_sum8(cn != 0 ? mass[CPL * src + at8] : 0.0);
+    const int c8 = first_lane(lane < CPL && cn != 0, lane < CPL && cn != 0 && pred(c_upto, m_upto));
     Place at{0, 0, 0, 0.0};
-    const int chunk = ch.find(at.c, at.m, pred);
+    at.c = c8 == 0 ? cb : lane_u(c_upto, c8 - 1);
+    at.m = c8 == 0 ? mb : lane_d(m_upto, c8 - 1);
+    const int chunk = CPL * src + c8;
     hold(chunk);
-    const int e = bn.find(at.c, at.m, pred);
-    at.d = chunk * kChunk + e;
-    at.n = lane_u((e & 1) ? bn.n[1] : bn.n[0], e >> 1);
+    // the first of the lane's bins, then the second
+    const uint32_t n1 = at.c + upto_n, n0 = n1 - n[1];
+    const double w1 = at.m + upto_w, w0 = at.m + (upto_w - w[1]);
+    const bool hit0 = n[0] != 0 && pred(n0, w0), hit1 = n[1] != 0 && pred(n1, w1);
+    const int l = first_lane((n[0] | n[1]) != 0, hit0 || hit1);
+    const bool second = lane_u(hit0 || (!hit1 && n[1] == 0) ? 0 : 1, l) != 0;
+    at.d = chunk * kChunk + 2 * l + second;
+    at.n = lane_u(second ? n[1] : n[0], l);
+    const double wb = before(upto_w);
+    at.c = lane_u(second ? n0 : n0 - n[0], l);
+    at.m += second ? lane_d(wb + w[0], l) : lane_d(wb, l);
     return at;
   };
   // top-k: the first k tokens
-  Place end = find([&](uint32_t c, double) { return f.k > 0 && c >= (uint64_t)f.k; });
-  if (f.k > 0 && end.c + (uint64_t)end.n > (uint64_t)f.k) end.n = (uint32_t)(f.k - end.c);
-  S = end.m + end.n * wt.at(end.d);
+  const uint32_t all = lane_u(lane_n, 63);
+  Place end{kBins, 0, all, lane_d(lane_w, 63)};  // all tokens
+  if (f.k > 0 && f.k < (int64_t)all) {
+    end = find([&](uint32_t c, double) { return c >= (uint32_t)f.k; });
+    end.n = min(end.n, (uint32_t)f.k - end.c);
+  }
+  auto weight = [&](const Place& at) { return at.m + (at.n != 0 ? at.n * wt.at(at.d) : 0.0); };
+  S = weight(end);
   // top-p: the tokens before which the weight is below the target
   if (f.p < 1.0) {
     const double target = f.p * S;
@@ -196,28 +236,21 @@ __device__ __forceinline__ void draw(const Weights& wt, const Filters& f, const 
     at.n = need >= 1.0 ? (need < (double)at.n ? (uint32_t)need : at.n) : 1u;
     if (at.d < end.d || (at.d == end.d && at.n < end.n)) end = at;
   }
-  // min-p: the last bin whose weight reaches it, 64 bins tried at a time
+  // min-p
   if (f.m > 1.0) {
     end = Place{wt.top, 1, 0, 0.0};
-  } else if (f.m > 0.0 && wt.at(end.d) < f.m) {
-    int lo = wt.top;  // at(lo) >= m
-#pragma unroll 1
-    for (int step = 1024; step > 0; step >>= step == 1024 ? 6 : 4) {  // 1024, 16, 1
-      const int mid = lo + step * (lane + 1);
-      const uint64_t in = __ballot(mid < kBins && wt.at(min(mid, kBins - 1)) >= f.m);
-      lo += step * (in == ~0ull ? 64 : __builtin_ctzll(~in));
-    }
+  } else if (f.m > 0.0 && lo < end.d) {  // the tokens up to bin lo
     const int chunk = lo / kChunk;
     hold(chunk);
-    uint32_t n = 0;
+    uint32_t to = 0;  // tokens up to bin lo
 #pragma unroll
-    for (int i = 0; i < CPL; ++i) n += CPL * lane + i < chunk ? ch.n[i] : 0;
+    for (int i = 0; i < CPL; ++i) to += CPL * lane + i < chunk ? cnt[CPL * lane + i] : 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) n += chunk * kChunk + 2 * lane + i <= lo ? bn.n[i] : 0;
-    n = lane_u(scan_sum(n), 63);
-    end = find([&](uint32_t c, double) { return c >= n; });
+    for (int i = 0; i < 2; ++i) to += chunk * kChunk + 2 * lane + i <= lo ? n[i] : 0;
+    to = lane_u(scan_sum(to), 63);
+    end = find([&](uint32_t c, double) { return c >= to; });
   }
-  S = end.m + end.n * wt.at(end.d);
+  S = weight(end);
   const double target = f.u * S;
   Place at = find([&](uint32_t, double m) { return m > target; });
   if (at.d > end.d) at = end;
@@ -239,8 +272,8 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   __shared__ uint32_t cnt[kChunks];
   __shared__ uint32_t bins[kChunk];
   __shared__ uint32_t places[(NR > 0 ? NR : 1) * FNW];
-  __shared__ uint32_t many_n, drawn_n;
-  __shared__ int drawn_d;
+  __shared__ uint32_t many_n, lost, drawn_n;
+  __shared__ int drawn_d, reaching;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t b = blockIdx.x;
   const uint16_t* row = logits + b * ld;
@@ -257,6 +290,11 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
+  for (int i = tid; i < kWindow / 4; i += FNT) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) many_n = lost = 0;
+  __syncthreads();  // before the row's loads, which a barrier would wait for
+  // a value that many of 64 samples have (the same samples for every wave)
+  const uint32_t sample = row[(int64_t)lane * V >> 6];
   uint4 held[NR > 0 ? NR : 1];
   if constexpr (NR > 0) {
 #pragma unroll
@@ -265,8 +303,6 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
       if (r * FNT + tid < pieces) held[r] = piece(r * FNT + tid);
     }
   }
-  // a value that many of 64 samples have (the same samples for every wave)
-  const uint32_t sample = row[(int64_t)lane * V >> 6];
   const float T = temps[b];
   Filters f;
   f.k = top_k != nullptr ? top_k[b] : 0;
@@ -274,8 +310,6 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   f.p = top_p != nullptr ? (double)top_p[b] : 1.0;
   f.m = min_p != nullptr ? (double)min_p[b] : 0.0;
   f.u = fmin(fmax((double)uniforms[b], 0.0), 1.0 - 0x1p-24);  // a NaN counts as 0
-  for (int i = tid; i < kWindow / 4; i += FNT) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) many_n = 0;
   uint32_t many = ~0u;
 #pragma unroll 1
   for (int e = 0; e < 64; e += 3) {  // one of its samples is met
@@ -285,7 +319,6 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
       break;
     }
   }
-  __syncthreads();
 
   // the counts: low half of word h & 0x7FFF for bits h < 0x8000, high half for the others
   auto add = [&](uint32_t h) { atomicAdd(&hist[h & 0x7FFFu], (h >> 15) * 0xFFFFu + 1u); };
@@ -330,18 +363,36 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     const uint32_t n = bits_count(bits_of(d));
     return d == 0x7FFF ? n + bits_count(0x8000u) : n;
   };
+  // The chunks' counts.  Eight lanes take the 128 words of a positive and of a
+  // negative chunk, a wave eight such pairs at a time; odd eights start 32 words
+  // further, so that a read touches every bank once.
   uint32_t sum = 0;  // of all counts, drawable or not
-  for (int i = tid; i < kWindow; i += FNT) sum += (hist[i] & 0xFFFFu) + (hist[i] >> 16);
-  for (int c = wave; c < kChunks; c += FNW) {
-    const uint32_t n = lane_u(scan_sum(bin_count(c * kChunk + 2 * lane) + bin_count(c * kChunk + 2 * lane + 1)), 63);
-    if (lane == 0) cnt[c] = n;
+  for (int g = wave * 8; g < kChunks / 2; g += FNW * 8) {
+    const int pair = g + lane / 8;
+    uint32_t lo = 0, hi = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = ((i * 32 + (lane & 8) * 4) & 127) + (lane & 7) * 4;
+      const uint4 x = *reinterpret_cast<const uint4*>(&hist[pair * kChunk + at]);
+      lo += (x.x & 0xFFFFu) + (x.y & 0xFFFFu) + (x.z & 0xFFFFu) + (x.w & 0xFFFFu);
+      hi += (x.x >> 16) + (x.y >> 16) + (x.z >> 16) + (x.w >> 16);
+    }
+    sum += lo + hi;
+    lo = scan_sum8(lo), hi = scan_sum8(hi);
+    if ((lane & 7) == 7) cnt[kChunks / 2 - 1 - pair] = lo, cnt[kChunks / 2 + pair] = hi;
   }
   sum = lane_u(scan_sum(sum), 63) + many_here - 512u * waves_pieces;
-  if (tid < 128) bins[tid] = 0;
+  if (lane == 0 && sum != 0) atomicAdd(&lost, sum);  // modulo 2^32: 0 over the waves where every count fits
   __syncthreads();
-  if (lane == 0 && sum != 0) atomicAdd(&bins[0], sum);  // modulo 2^32: 0 over the waves where nothing was lost
+  const bool counted = lost == 0;
+  if (tid == 0 && counted) {  // what the words do not say
+    if (many != ~0u && bin_of(many) < kBins) cnt[bin_of(many) / kChunk] += many_all;
+    const uint32_t minus = (hist[0] >> 16);  // -0, counted as +0
+    cnt[kChunks / 2] -= minus, cnt[kChunks / 2 - 1] += minus;
+    cnt[0] = bits_count(0x7F80u);  // NaN apart
+    cnt[kChunks - 1] = 0;          // -infinity, NaN
+  }
   __syncthreads();
-  const bool counted = bins[0] == 0;
 
   // the largest logit
   auto first_chunk = [&]() -> int {
@@ -357,7 +408,7 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     return chunk * kChunk + 2 * src + (lane_u(n0, src) != 0 ? 0 : 1);
   };
   Weights wt;
-  wt.T = (double)T;
+  wt.c = 1.4426950408889634 / (double)T;
   int d = 0;
   uint32_t nth = 0;
   double S = 0.0;
@@ -372,17 +423,22 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     }
     wt.top = first_bin(c0, bin_count(c0 * kChunk + 2 * lane), bin_count(c0 * kChunk + 2 * lane + 1));
     wt.xmax = bin_value(wt.top);
-    for (int c = wave; c < kChunks; c += FNW) {
-      if (cnt[c] == 0) continue;
-      const int e = c * kChunk + 2 * lane;
+    static_assert(kChunks <= 64 * FNW, "a lane for each of a wave's chunks");
+    uint64_t some = __ballot(lane < kChunks / FNW && cnt[min(wave + FNW * lane, kChunks - 1)] != 0);
+    for (; some != 0; some &= some - 1) {
+      const int c = wave + FNW * __builtin_ctzll(some), e = c * kChunk + 2 * lane;
       const uint32_t n0 = bin_count(e), n1 = bin_count(e + 1);
       const double m = (n0 != 0 ? n0 * wt.at(e) : 0.0) + (n1 != 0 ? n1 * wt.at(e + 1) : 0.0);
       const double all = lane_d(scan_sum(m), 63);
       if (lane == 0) mass[c] = all;
     }
+    if (wave == FNW - 1 && f.m > 0.0) {
+      const int lo = last_reaching(wt, f.m);
+      if (lane == 0) reaching = lo;
+    }
     __syncthreads();
     if (wave == 0) {
-      draw(wt, f, cnt, mass, [&](int chunk, uint32_t (&n)[2]) {
+      draw(wt, f, reaching, cnt, mass, [&](int chunk, uint32_t (&n)[2]) {
         n[0] = bin_count(chunk * kChunk + 2 * lane), n[1] = bin_count(chunk * kChunk + 2 * lane + 1);
       }, d, nth, S);
       if (lane == 0) drawn_d = d, drawn_n = nth, drawn_s = S;
@@ -437,7 +493,7 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
       }
       return;
     }
-    draw(wt, f, cnt, mass, [&](int chunk, uint32_t (&n)[2]) {  // the whole workgroup, the same chunk
+    draw(wt, f, last_reaching(wt, f.m), cnt, mass, [&](int chunk, uint32_t (&n)[2]) {  // the whole workgroup, the same chunk
       recount(chunk * kChunk, kChunk, bins);
       n[0] = bins[2 * lane], n[1] = bins[2 * lane + 1];
     }, d, nth, S);
@@ -446,16 +502,25 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   // the nth of the bin's tokens by index
   auto done = [&](int64_t token) {
     out[b] = token;
-    if (logprob != nullptr) logprob[b] = (float)((d == wt.top ? 0.0 : (bin_value(d) - wt.xmax) / wt.T) - log(S));
+    if (logprob != nullptr) logprob[b] = (float)((d == wt.top ? 0.0 : (bin_value(d) - wt.xmax) / (double)T) - log(S));
   };
-  const uint32_t bits = bits_of(d), alt = bits == 0 ? 0x8000u : bits;
+  // a half of a word matches where it is 0 here; +0 also meets -0
+  const uint32_t same = bits_of(d) * 0x10001u, mask = d == 0x7FFF ? 0x7FFF7FFFu : ~0u;
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  auto differ = [&](uint32_t w) -> u16x2 {  // 0 or 1 a half
+    return __builtin_elementwise_min(__builtin_bit_cast(u16x2, (w ^ same) & mask), u16x2{1, 1});
+  };
+  auto any_match = [&](const uint4& x) -> bool {
+    const u16x2 n = differ(x.x) + differ(x.y) + differ(x.z) + differ(x.w);
+    return __builtin_bit_cast(uint32_t, n) != 0x00040004u;
+  };
   auto matches = [&](const uint4& x) -> uint32_t {  // a bit for each of the eight
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     uint32_t m = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t h = (e & 1) ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu;
-      m |= h == bits || h == alt ? 1u << e : 0u;
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t n = __builtin_bit_cast(uint32_t, differ(w[e])) ^ 0x10001u;
+      m |= ((n & 1u) | (n >> 15)) << (2 * e);
     }
     return m;
   };
@@ -476,7 +541,8 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   if constexpr (NR > 0) {
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      const uint32_t n = lane_u(scan_sum((uint32_t)__popc(matches(held[r]))), 63);
+      uint32_t n = 0;
+      if (__any(any_match(held[r]))) n = lane_u(scan_sum((uint32_t)__popc(matches(held[r]))), 63);
       if (lane == 0) places[r * FNW + wave] = n;
     }
     __syncthreads();
@@ -540,9 +606,9 @@ extern "C" int lfs_sample_filtered(const void* logits, int64_t ld, const float* 
   hipLaunchKernelGGL(sample_filtered_kernel<NR>, dim3((unsigned)B), dim3(FNT), 0, (hipStream_t)stream,               \
                      (const uint16_t*)logits, ld, temperatures, uniforms, top_k, top_p, min_p, vocab, out, logprob)
   const int64_t pieces = ((int64_t)vocab + 7 + 7) / 8;  // at any alignment
-  if (pieces <= 5 * FNT) LFS_SF(5);
-  else if (pieces <= 10 * FNT) LFS_SF(10);
+  if (pieces <= 10 * FNT) LFS_SF(10);
   else if (pieces <= 20 * FNT) LFS_SF(20);
+  else if (pieces <= 40 * FNT) LFS_SF(40);
   else LFS_SF(0);
 #undef LFS_SF
   return check_launch("sample_filtered");
