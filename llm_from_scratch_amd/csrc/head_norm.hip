@@ -17,60 +17,134 @@
 namespace lfs {
 namespace {
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// The call's pointers and sizes.
+struct HeadNorm {
+  const uint16_t* qkv;
+  int64_t ld;
+  const float *qw, *kw, *cos_sin;
+  const int64_t *pos, *slots;
+  uint16_t *q_out, *kc, *vc, *k_out, *v_out;
+  int64_t num_slots, max_pos;
+  float eps;
+  int R, Hq, Hkv;
+  unsigned T;
+};
+
+// What a lane's chunk c of any head of a token needs besides the chunk.
 template <int D>
-__global__ __launch_bounds__(256) void qk_head_norm_rope_store_kernel(
-    const uint16_t* __restrict__ qkv, int64_t ld, const float* __restrict__ qw, const float* __restrict__ kw,
-    const float* __restrict__ cos_sin, int R, const int64_t* __restrict__ pos, const int64_t* __restrict__ slots,
-    uint16_t* __restrict__ q_out, uint16_t* __restrict__ kc, uint16_t* __restrict__ vc, uint16_t* __restrict__ k_out,
-    uint16_t* __restrict__ v_out, int64_t T, int Hq, int Hkv, int64_t num_slots, int64_t max_pos, float eps) {
-  constexpr int C = D / 8;  // lanes of a head
-  const int heads = Hq + 2 * Hkv, c = threadIdx.x % C, r2 = R / 16;  // r2: chunks of half the rotated dims
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / C;
-  if (unit >= T * heads) return;  // whole heads: the exchanges below stay among live lanes
-  const int64_t t = unit / heads;
-  const int h = (int)(unit - t * heads);
-  const uint4 x = *reinterpret_cast<const uint4*>(qkv + t * ld + h * D + 8 * c);
-  const int64_t slot = h >= Hq && slots != nullptr ? slots[t] : -1;
-  const bool store = slot >= 0 && slot < num_slots;
-  if (h >= Hq + Hkv) {
-    const int64_t e = (int64_t)(h - Hq - Hkv) * D + 8 * c;
-    if (store) *reinterpret_cast<uint4*>(vc + slot * Hkv * D + e) = x;
-    if (v_out != nullptr) *reinterpret_cast<uint4*>(v_out + t * Hkv * D + e) = x;
+struct Turn {
+  static constexpr int C = D / 8;  // lanes of a head
+  float w[2][8], cs[8], sn[8];     // of q and k; sn has the sign of its product
+  int src;                         // the lane with the other half's chunk
+  bool turned;
+
+  __device__ __forceinline__ static void load8(const float* p, float* f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = p[e];
+  }
+  __device__ __forceinline__ void load_weights(const HeadNorm& a, int c) {
+    load8(a.qw + 8 * c, w[0]);
+    load8(a.kw + 8 * c, w[1]);
+  }
+  __device__ __forceinline__ void load_row(const HeadNorm& a, int c, int64_t t) {
+    const int r2 = a.R / 16;  // chunks of half the rotated dims
+    const bool low = c < r2;
+    turned = c < 2 * r2;
+    src = (int)(threadIdx.x & 63) + (low ? r2 : turned ? -r2 : 0);
+    if (!turned) return;
+    int64_t p = a.pos[t];
+    p = p < 0 ? 0 : (p >= a.max_pos ? a.max_pos - 1 : p);
+    const float* row = a.cos_sin + p * a.R + 8 * (low ? c : c - r2);
+    load8(row, cs);
+    load8(row + a.R / 2, sn);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sn[e] = low ? -sn[e] : sn[e];
+  }
+  // the chunk of a head of q (k: isk): every lane of the head calls it
+  __device__ __forceinline__ u32x4 head(const u32x4& x, bool isk, float eps) const {
+    float f[8], y[8], other[8], ss = 0.f;
+    unpack8(make_uint4(x[0], x[1], x[2], x[3]), f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+    const float inv = rsqrtf(group_sum<C>(ss) * (1.0f / D) + eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = f[e] * inv * (isk ? w[1][e] : w[0][e]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) other[e] = __shfl(y[e], src, 64);
+    if (turned) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e], cs[e], other[e] * sn[e]);
+    }
+    return u32x4{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7])};
+  }
+};
+
+template <bool NT>
+__device__ __forceinline__ void put(uint16_t* p, const u32x4& x) {
+  if constexpr (NT) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(p));
+  else *reinterpret_cast<u32x4*>(p) = x;
+}
+// chunk c of head h (q, k, v heads in turn) of token t, as it leaves
+template <int D, bool NT>
+__device__ __forceinline__ void store_head(const HeadNorm& a, int64_t t, int h, int c, int64_t slot, const u32x4& x) {
+  if (h < a.Hq) {
+    put<NT>(a.q_out + (t * a.Hq + h) * D + 8 * c, x);
     return;
   }
-  float f[8], y[8], other[8];
-  unpack8(x, f);
-  float ss = 0.f;
+  const bool isv = h >= a.Hq + a.Hkv;
+  const int64_t e = (int64_t)(h - a.Hq - (isv ? a.Hkv : 0)) * D + 8 * c;
+  if (slot >= 0 && slot < a.num_slots) put<NT>((isv ? a.vc : a.kc) + slot * a.Hkv * D + e, x);
+  if (a.k_out != nullptr) put<NT>((isv ? a.v_out : a.k_out) + t * a.Hkv * D + e, x);
+}
+
+// Few tokens: D / 8 lanes per (token, head).
+template <int D>
+__global__ __launch_bounds__(256) void qk_head_norm_rope_store_kernel(HeadNorm a) {
+  constexpr int C = D / 8;
+  const unsigned heads = a.Hq + 2 * a.Hkv, unit = blockIdx.x * (256 / C) + threadIdx.x / C, t = unit / heads;
+  const int c = threadIdx.x % C, h = (int)(unit - t * heads);
+  if (t >= a.T) return;  // whole heads: the exchanges stay among live lanes
+  u32x4 x = *reinterpret_cast<const u32x4*>(a.qkv + t * a.ld + h * D + 8 * c);
+  const int64_t slot = h >= a.Hq && a.slots != nullptr ? a.slots[t] : -1;
+  if (h < a.Hq + a.Hkv) {
+    Turn<D> turn;
+    turn.load_weights(a, c);
+    turn.load_row(a, c, t);
+    x = turn.head(x, h >= a.Hq, a.eps);
+  }
+  store_head<D, false>(a, t, h, c, slot, x);
+}
+
+// Many tokens: a wave per token, 512 / D heads at a time, so that the weights
+// and the token's row of the table are read once for all of its heads.
+constexpr int HU = 4;  // heads of a lane whose loads are in flight together
+template <int D>
+__global__ __launch_bounds__(256) void qk_head_norm_rope_store_rows(HeadNorm a) {
+  constexpr int C = D / 8, HW = 64 / C;
+  const int lane = threadIdx.x & 63, c = lane % C, heads = a.Hq + 2 * a.Hkv;
+  Turn<D> turn;
+  turn.load_weights(a, c);
+  for (unsigned t = blockIdx.x * 4 + (threadIdx.x >> 6); t < a.T; t += gridDim.x * 4) {
+    const uint16_t* row = a.qkv + t * a.ld + 8 * c;
+    turn.load_row(a, c, t);
+    const int64_t slot = a.slots != nullptr ? a.slots[t] : -1;
+    for (int h0 = lane / C; h0 < heads; h0 += HU * HW) {
+      u32x4 x[HU];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
-  const float inv = rsqrtf(group_sum<C>(ss) * (1.0f / D) + eps);
-  const float* w = (h < Hq ? qw : kw) + 8 * c;
+      for (int i = 0; i < HU; ++i)
+        x[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + min(h0 + i * HW, heads - 1) * D));
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = f[e] * inv * w[e];
-  const bool low = c < r2, turned = c < 2 * r2;
-  const int src = (threadIdx.x & 63) + (low ? r2 : turned ? -r2 : 0);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) other[e] = __shfl(y[e], src, 64);
-  if (turned) {
-    int64_t p = pos[t];
-    p = p < 0 ? 0 : (p >= max_pos ? max_pos - 1 : p);
-    const float* cs = cos_sin + p * R + 8 * (low ? c : c - r2);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float s = cs[R / 2 + e];
-      y[e] = fmaf(y[e], cs[e], low ? -other[e] * s : other[e] * s);
+      for (int i = 0; i < HU; ++i) {
+        const int h = h0 + i * HW;
+        if (h < a.Hq + a.Hkv) x[i] = turn.head(x[i], h >= a.Hq, a.eps);
+        if (h < heads) store_head<D, true>(a, t, h, c, slot, x[i]);
+      }
     }
   }
-  const uint4 z = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]),
-                             pack_bf16x2(y[6], y[7]));
-  if (h < Hq) {
-    *reinterpret_cast<uint4*>(q_out + (t * Hq + h) * D + 8 * c) = z;
-  } else {
-    const int64_t e = (int64_t)(h - Hq) * D + 8 * c;
-    if (store) *reinterpret_cast<uint4*>(kc + slot * Hkv * D + e) = z;
-    if (k_out != nullptr) *reinterpret_cast<uint4*>(k_out + t * Hkv * D + e) = z;
-  }
 }
+constexpr int64_t kHeadRowsT = 2048;  // tokens from which a wave takes a whole token
 
 }  // namespace
 }  // namespace lfs
@@ -99,14 +173,18 @@ extern "C" int lfs_qk_head_norm_rope_store(const void* qkv, int64_t ld, const fl
               "qk_head_norm_rope_store: buffers must be 16-byte aligned");
   const int64_t heads = Hq + 2 * (int64_t)Hkv;
   LFS_REQUIRE(T < ((1ll << 32) - 256) / (D / 8) / heads, "qk_head_norm_rope_store: too many tokens");
-  const int64_t wgs = (T * heads * (D / 8) + 255) / 256;
-#define LFS_HN(DD)                                                                                                   \
-  hipLaunchKernelGGL(qk_head_norm_rope_store_kernel<DD>, dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,      \
-                     (const uint16_t*)qkv, ld, q_weight, k_weight, cos_sin, R, positions, slot_mapping,              \
-                     (uint16_t*)q_out, (uint16_t*)k_cache, (uint16_t*)v_cache, (uint16_t*)k_out, (uint16_t*)v_out, T, \
-                     Hq, Hkv, num_slots, max_positions, eps)
-  if (D == 64) LFS_HN(64);
-  else LFS_HN(128);
-#undef LFS_HN
+  const HeadNorm a{(const uint16_t*)qkv, ld, q_weight, k_weight, cos_sin, positions, slot_mapping, (uint16_t*)q_out,
+                   (uint16_t*)k_cache, (uint16_t*)v_cache, (uint16_t*)k_out, (uint16_t*)v_out, num_slots, max_positions,
+                   eps, R, Hq, Hkv, (unsigned)T};
+  hipStream_t st = (hipStream_t)stream;
+  if (T >= kHeadRowsT) {
+    const dim3 grid((unsigned)std::min<int64_t>((T + 3) / 4, 4096));
+    if (D == 64) hipLaunchKernelGGL(qk_head_norm_rope_store_rows<64>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(qk_head_norm_rope_store_rows<128>, grid, dim3(256), 0, st, a);
+  } else {
+    const dim3 grid((unsigned)((T * heads * (D / 8) + 255) / 256));
+    if (D == 64) hipLaunchKernelGGL(qk_head_norm_rope_store_kernel<64>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(qk_head_norm_rope_store_kernel<128>, grid, dim3(256), 0, st, a);
+  }
   return check_launch("qk_head_norm_rope_store");
 }
