@@ -1,7 +1,7 @@
 // One wave's walk over the tiles of one (sequence, kv head) of a paged KV pool,
-// and the log-sum-exp merge of such walks: the device code shared by the
-// paged decode (paged_kv.hip) and the decode over a sliding window
-// (paged_window.hip).
+// the balanced split of a batch into such walks, and their log-sum-exp merge:
+// shared by the paged decode (paged_kv.hip) and the decode over a sliding
+// window (paged_window.hip).
 #pragma once
 
 #include "common.h"
@@ -424,7 +424,224 @@ __device__ __forceinline__ void decode_walk(
   (void)lane;
 }
 
+// One wave: kv head kh of sequence b over context rows [t_begin, t_end)
+// (t_begin a multiple of `tile`, t_end <= Lc).  A range that is the whole
+// context (t_begin == 0, t_end >= Lc) writes the normalised bf16 output;
+// otherwise the unnormalised partial of query head kh*G + g goes to row
+// prow + g of the workspace (o: ws_o[row*D ..], (m, l): ws_ml[row*2 ..]).
+// pw: the wave's private LDS slice (T * GP floats).
+template <int D, int G>
+__device__ __forceinline__ void decode_chunk(
+    const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc,
+    const uint16_t* __restrict__ vc, const int32_t* __restrict__ btrow, float* __restrict__ ws_o,
+    float* __restrict__ ws_ml, uint16_t* __restrict__ out, int Hkv, int BS, int64_t NB, int tile,
+    float scale_log2, int b, int kh, int64_t t_begin, int64_t t_end, int64_t Lc, int64_t prow,
+    float* __restrict__ pw, int lane) {
+  using W = DecodeWave<D, G>;
+  W w(lane, Hkv);
+  const int Hq = Hkv * G;
+  typename W::QBuf qa;
+  w.load_q(qa, q, b, kh, Hq);
+  decode_walk<D, G>(w, qa, kc, vc, btrow, BS, NB, tile, scale_log2, kh, t_begin, t_end, 1,
+                    block_of(t_end - 1, BS) + 1, pw);
+  w.finish(t_begin == 0 && t_end >= Lc, out, ws_o, ws_ml, b, kh, Hq, prow);
+}
+
+// Balanced split: a fixed grid of nwg workgroups (wpg waves each, one kv
+// head per wave; one workgroup per CU) shares the work evenly, whatever the
+// context lengths.
+// Work units are (sequence b, kv-head group, tile) triples in that order,
+// n_b = ceil(L_b / tile) tiles per (sequence, group), where L_b is the
+// clamped context length; workgroup w takes the units [w*Ct, (w+1)*Ct),
+// Ct = ceil(total / nwg), and its waves walk the same tiles for the heads of
+// the group (so a workgroup reads wpg adjacent head slices of each row
+// together).  A (sequence, group) range that one workgroup covers entirely
+// is written out directly; otherwise workgroup w's partial of pair group
+// pg = b*ngroups + group is slot (w + pg)*wpg + wave -- unique, since along
+// the units both w and pg are non-decreasing and one of them grows at every
+// step from one (pg, w) overlap to the next.  Every workgroup scans the
+// per-sequence tile counts into LDS (B <= BAL_MAXB); workgroup 0 also
+// writes the scan (B+1 ints) to tp_out for the merge.
+constexpr int BAL_MAXB = 8192;
+
+__device__ __forceinline__ int decode_tiles(const int64_t* ctx_lens, int b, int64_t cap, int tile) {
+  const int64_t L = min(ctx_lens[b], cap);
+  return L > 0 ? (int)((L + tile - 1) >> __builtin_ctz(tile)) : 0;  // tile is 16, 32 or 64
+}
+
+// A window over the contexts: of L tokens the last `size` are visible and the
+// first `sinks`.  A sequence's visible rows are two ranges of tiles: of the
+// sinks before the window, [0, sinks) clipped, and of the window, whose first
+// tile may begin with hidden rows.
+struct Window {
+  int size, sinks;
+};
+struct WindowTiles {
+  int64_t first, end, sk;  // the window's rows first .. end - 1, the sinks' 0 .. sk - 1
+  int64_t w0;              // first row of the window's first tile
+  int ns, nw;              // tiles of the sinks and of the window
+  __device__ __forceinline__ WindowTiles(int64_t L, int64_t cap, int tile, const Window& w) {
+    const int sh = __builtin_ctz(tile);
+    L = max(L, (int64_t)0);
+    first = max((int64_t)0, L - w.size);
+    end = min(L, cap);
+    sk = min(min((int64_t)w.sinks, first), end);
+    w0 = first & -(int64_t)tile;
+    ns = (int)((sk + tile - 1) >> sh);
+    nw = end > first ? (int)((end - w0 + tile - 1) >> sh) : 0;
+  }
+};
+
+// One wave: kv head kh of sequence b over the visible tiles i0 .. i1 - 1 (the
+// sinks', then the window's), as decode_chunk.
+template <int D, int G>
+__device__ __forceinline__ void window_chunk(
+    const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
+    const int32_t* __restrict__ btrow, float* __restrict__ ws_o, float* __restrict__ ws_ml, uint16_t* __restrict__ out,
+    int Hkv, int BS, int64_t NB, int max_blocks, int tile, float scale_log2, int b, int kh, int i0, int i1,
+    const WindowTiles& wt, int64_t prow, float* __restrict__ pw, int lane) {
+  using W = DecodeWave<D, G>;
+  W w(lane, Hkv);
+  const int Hq = Hkv * G;
+  typename W::QBuf qa;
+  w.load_q(qa, q, b, kh, Hq);
+  if (i0 < wt.ns)
+    decode_walk<D, G>(w, qa, kc, vc, btrow, BS, NB, tile, scale_log2, kh, (int64_t)i0 * tile,
+                      min(wt.sk, (int64_t)i1 * tile), 1, max_blocks, pw);
+  const int64_t t0 = wt.w0 + (int64_t)max(0, i0 - wt.ns) * tile;
+  const int64_t t1 = min(wt.end, wt.w0 + (int64_t)(i1 - wt.ns) * tile);
+  if (t0 < t1)
+    decode_walk<D, G, true>(w, qa, kc, vc, btrow, BS, NB, tile, scale_log2, kh, t0, t1, 1, max_blocks, pw,
+                            NoPrologue(), wt.first);
+  w.finish(i0 == 0 && i1 == wt.ns + wt.nw, out, ws_o, ws_ml, b, kh, Hq, prow);
+}
+
+// WIN: over a window.
+template <int D, int G, bool WIN>
+__global__ __launch_bounds__(256) void paged_decode_balanced(
+    const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc,
+    const uint16_t* __restrict__ vc, const int64_t* __restrict__ ctx_lens,
+    const int32_t* __restrict__ bt, int64_t bt_stride, float* __restrict__ ws_o,
+    float* __restrict__ ws_ml, int* __restrict__ tp_out, uint16_t* __restrict__ out, int Hkv, int BS,
+    int64_t NB, int max_blocks, int B, int tile, float scale_log2, int ngroups, Window win) {
+  using Geo = DecodeGeom<D>;
+  constexpr int GP = G <= 4 ? 4 : 8;
+  __shared__ __attribute__((aligned(16))) float p_lds[4][Geo::T * GP];
+  __shared__ int tp[BAL_MAXB + 1];
+  __shared__ int wsum[4];
+  const int tid = threadIdx.x, nthr = blockDim.x;
+  const int wave = tid >> 6, lane = tid & 63, wpg = nthr >> 6;
+  const int64_t cap = (int64_t)max_blocks * BS;
+
+  // ---- tp[b] = sum of n_b' for b' < b (each thread a run of sequences)
+  const int per = (B + nthr - 1) / nthr;
+  const int lo = min(B, tid * per), hi = min(B, lo + per);
+  int run = 0;
+  for (int i = lo; i < hi; ++i) {
+    if constexpr (WIN) {
+      const WindowTiles wt(ctx_lens[i], cap, tile, win);
+      run += wt.ns + wt.nw;
+    } else {
+      run += decode_tiles(ctx_lens, i, cap, tile);
+    }
+    tp[i + 1] = run;
+  }
+  int incl = run;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 63) wsum[wave] = incl;
+  __syncthreads();
+  int excl = incl - run;
+  for (int w = 0; w < wave; ++w) excl += wsum[w];
+  for (int i = lo; i < hi; ++i) tp[i + 1] += excl;
+  if (tid == 0) tp[0] = 0;
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= B; i += nthr) tp_out[i] = tp[i];
+
+  // 32-bit throughout: the host refuses 2^31 work units, and a 64-bit divide
+  // is some 0.3 us of a chain that no other work hides
+  const unsigned total = (unsigned)ngroups * (unsigned)tp[B];
+  const unsigned nwg = gridDim.x;
+  const unsigned Ct = max(1u, (total + nwg - 1) / nwg);
+  unsigned u = blockIdx.x * Ct;
+  const unsigned u_end = min(total, u + Ct);
+  if (u >= u_end) return;
+  // first sequence: the largest b with ngroups * tp[b] <= u (it has n_b > 0)
+  int b_lo = 0, b_hi = B - 1;
+  while (b_lo < b_hi) {
+    const int mid = (b_lo + b_hi + 1) >> 1;
+    if ((unsigned)ngroups * (unsigned)tp[mid] <= u) b_lo = mid;
+    else b_hi = mid - 1;
+  }
+  int b = b_lo;
+  float* pw = p_lds[wave];
+  while (u < u_end) {
+    const unsigned nb = tp[b + 1] - tp[b];
+    const unsigned base = (unsigned)ngroups * (unsigned)tp[b];
+    const int grp = (int)((u - base) / nb);
+    const unsigned i0 = (u - base) - grp * nb;
+    const unsigned seg_end = min(u_end, base + (grp + 1) * nb);
+    const int kh = grp * wpg + wave;
+    if (kh < Hkv) {
+      const int64_t slot = ((int64_t)blockIdx.x + (int64_t)b * ngroups + grp) * wpg + wave;
+      if constexpr (WIN) {
+        const WindowTiles wt(ctx_lens[b], cap, tile, win);
+        const int i1 = (int)(i0 + (seg_end - u));
+        window_chunk<D, G>(q, kc, vc, bt + (int64_t)b * bt_stride, ws_o, ws_ml, out, Hkv, BS, NB, max_blocks, tile,
+                           scale_log2, b, kh, (int)i0, i1, wt, slot * G, pw, lane);
+      } else {
+        const int64_t Lc = min(ctx_lens[b], cap);
+        const int64_t t_begin = (int64_t)i0 * tile;
+        const int64_t t_end = min(Lc, (int64_t)(i0 + (seg_end - u)) * tile);
+        decode_chunk<D, G>(q, kc, vc, bt + (int64_t)b * bt_stride, ws_o, ws_ml, out, Hkv, BS, NB, tile,
+                           scale_log2, b, kh, t_begin, t_end, Lc, slot * G, pw, lane);
+      }
+    }
+    u = seg_end;
+    if (u >= base + ngroups * nb) {
+      ++b;
+      while (b < B && tp[b + 1] == tp[b]) ++b;  // sequences with no context
+    }
+  }
+}
+
 // ------------------------------------------------------------ decode merge --
+// Where the partials of (sequence b, query head h) live: ns of them, the
+// s-th at workspace row r0 + s * rstep (o at ws_o[row * D], (m, l) at
+// ws_ml[row * 2]).  ns == 1: the split kernel wrote the output itself;
+// ns == 0: no context.
+struct PartMap {
+  int bps, max_splits;  // fixed chunks of bps blocks (bps > 0)
+  const int* tp;        // balanced split (bps == 0): tile-count scan, B + 1 ints
+  int tile, ngroups, wpg, G, nwg, B;
+};
+
+__device__ __forceinline__ int part_span(const PartMap& pm, int b, int h, int Hq, int64_t Lc, int BS,
+                                         int64_t& r0, int64_t& rstep) {
+  if (pm.bps > 0) {
+    const int64_t chunk = (int64_t)pm.bps * BS;
+    r0 = (int64_t)b * pm.max_splits * Hq + h;
+    rstep = Hq;
+    return Lc > 0 ? (int)((Lc + chunk - 1) / chunk) : 0;
+  }
+  r0 = 0;
+  rstep = (int64_t)pm.wpg * pm.G;
+  const int nb = pm.tp[b + 1] - pm.tp[b];
+  if (nb == 0) return 0;
+  const int kh = h / pm.G, g = h - kh * pm.G;
+  const int grp = kh / pm.wpg, wv = kh - grp * pm.wpg;
+  const unsigned total = (unsigned)pm.ngroups * (unsigned)pm.tp[pm.B];  // < 2^31, as in the split
+  const unsigned Ct = max(1u, (total + pm.nwg - 1) / (unsigned)pm.nwg);
+  const unsigned start = (unsigned)pm.ngroups * (unsigned)pm.tp[b] + (unsigned)grp * (unsigned)nb;
+  const unsigned wf = start / Ct, wl = (start + nb - 1) / Ct;
+  r0 = (((int64_t)wf + (int64_t)b * pm.ngroups + grp) * pm.wpg + wv) * pm.G + g;
+  return (int)(wl - wf + 1);
+}
+
 // Log-sum-exp merge of one output element: partials s = 0 .. ns-1 of a
 // (sequence, head) at workspace rows r0 + s*rs, element d.  All lanes of a
 // wave share the (sequence, head) (D is a multiple of 64).  Up to MERGE_NS
@@ -489,6 +706,137 @@ __device__ __forceinline__ float merge_element(const float* __restrict__ ws_o, c
     res = den > 0.f ? num / den : 0.f;
   }
   return res;
+}
+
+// One thread per output element: workgroup (x, b) merges elements
+// x*256 .. x*256+255 of sequence b's Hq*D outputs (whole heads for D = 64 /
+// 128).  256-thread workgroups, one per CU at the cfg3 shapes: the same
+// arithmetic as one 64 / 128-thread workgroup per (head, sequence), bit for
+// bit, and 0.1-0.2 us (cfg3) to 2 us (cfg4) less kernel time -- fewer
+// workgroups to dispatch; the two dependent round trips (lengths and scan,
+// then the partials) remain.
+constexpr int MERGE_THREADS = 256;
+__global__ __launch_bounds__(MERGE_THREADS) void paged_decode_merge(
+    const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
+    const int64_t* __restrict__ ctx_lens, uint16_t* __restrict__ out, int Hq, int D, int BS,
+    int max_blocks, PartMap pm) {
+  const int b = blockIdx.y;
+  const int e = blockIdx.x * MERGE_THREADS + threadIdx.x;
+  if (e >= Hq * D) return;
+  const int h = e / D, d = e - h * D;
+  const int64_t Lc = min(ctx_lens[b], (int64_t)max_blocks * BS);
+  int64_t r0, rs;
+  const int ns = part_span(pm, b, h, Hq, Lc, BS, r0, rs);
+  if (ns == 1) return;
+  out[(int64_t)b * Hq * D + e] = (uint16_t)f32_to_bf16(merge_element(ws_o, ws_ml, r0, rs, ns, D, d));
+}
+
+// The merge fused with the act_quant of its output row (the output
+// projection's FP8 input): one 128-thread workgroup per (128-value act_quant
+// group, sequence), every group independent.  Each thread merges one element
+// of the group (the arithmetic of paged_decode_merge; ns == 1: the split
+// kernel wrote the value), then 16 lanes quantise the group's 128 bf16
+// values 8 each, as act_quant does: codes and scale bit-identical to
+// act_quant(out row, 128).  Needs Hq * D % 128 == 0.
+__global__ __launch_bounds__(128) void paged_decode_merge_quant_group(
+    const float* __restrict__ ws_o, const float* __restrict__ ws_ml, const int64_t* __restrict__ ctx_lens,
+    uint16_t* __restrict__ out, uint8_t* __restrict__ qo, float* __restrict__ qs, int Hq, int D, int BS,
+    int max_blocks, PartMap pm) {
+  __shared__ __attribute__((aligned(16))) uint16_t vals[128];
+  const int g = blockIdx.x, b = blockIdx.y, t = threadIdx.x;
+  const int E = Hq * D;
+  const int e = g * 128 + t;
+  const int h = e / D, d = e - h * D;
+  const int64_t Lc = min(ctx_lens[b], (int64_t)max_blocks * BS);
+  int64_t r0, rs;
+  const int ns = part_span(pm, b, h, Hq, Lc, BS, r0, rs);
+  uint16_t* orow = out + (int64_t)b * E;
+  uint16_t v;
+  if (ns == 1) {
+    v = orow[e];  // written by the split kernel
+  } else {
+    v = (uint16_t)f32_to_bf16(merge_element(ws_o, ws_ml, r0, rs, ns, D, d));
+    orow[e] = v;
+  }
+  vals[t] = v;
+  __syncthreads();
+  if (t < 16) {
+    float f[8];
+    unpack8(*reinterpret_cast<const uint4*>(&vals[t * 8]), f);
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
+    amax = group_max<16>(amax);
+    const float sc = scale_from_amax(amax, false);
+    *reinterpret_cast<uint2*>(qo + (int64_t)b * E + g * 128 + t * 8) = quant8(f, sc);
+    if (t == 0) qs[(int64_t)b * (E / 128) + g] = sc;
+  }
+}
+
+template <int D, int G, bool WIN>
+void launch_balanced(unsigned nwg, dim3 block, hipStream_t st, const uint16_t* q, const uint16_t* kc,
+                     const uint16_t* vc, const int64_t* cl, const int32_t* bt, int64_t bts, float* wo,
+                     float* wml, int* tp, uint16_t* out, int Hkv, int BS, int64_t NB, int max_blocks, int B,
+                     int tile, float sl2, int ngroups, Window win) {
+  hipLaunchKernelGGL((paged_decode_balanced<D, G, WIN>), dim3(nwg), block, 0, st, q, kc, vc, cl, bt, bts, wo, wml,
+                     tp, out, Hkv, BS, NB, max_blocks, B, tile, sl2, ngroups, win);
+}
+
+template <int D, bool WIN = false>
+bool dispatch_balanced(int G, unsigned nwg, dim3 block, hipStream_t st, const uint16_t* q,
+                       const uint16_t* kc, const uint16_t* vc, const int64_t* cl, const int32_t* bt,
+                       int64_t bts, float* wo, float* wml, int* tp, uint16_t* out, int Hkv, int BS,
+                       int64_t NB, int max_blocks, int B, int tile, float sl2, int ngroups, Window win = Window{}) {
+#define LFS_G(GG) \
+  case GG: launch_balanced<D, GG, WIN>(nwg, block, st, q, kc, vc, cl, bt, bts, wo, wml, tp, out, Hkv, BS, NB, max_blocks, B, tile, sl2, ngroups, win); return true;
+  switch (G) {
+    LFS_G(1) LFS_G(2) LFS_G(3) LFS_G(4) LFS_G(5) LFS_G(6) LFS_G(7) LFS_G(8)
+    default: return false;
+  }
+#undef LFS_G
+}
+
+// compute units of the current device (the balanced split's grid)
+int decode_cu_count() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (cached[dev] == 0) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cached[dev] = n;
+  }
+  return cached[dev];
+}
+
+// balanced split geometry: wpg waves (kv heads) per workgroup, ngroups
+// groups, nwg workgroups -- one 4-wave workgroup per CU, one round.  Fewer,
+// longer streams beat filling the kernel's occupancy (two waves per SIMD):
+// measured at 1 / 2 / 3 / 4 / 8 workgroups per CU, cfg3 44.3 / 49.4 / 56.6 /
+// 56.0 / 66.2 us, cfg4 1169 / 1190 / 1202 / 1212 / 1257 us (fewer tile
+// pipelines to ramp up, fewer partials, fewer concurrent DRAM streams).
+struct BalancedGeom {
+  int wpg, ngroups, nwg;
+};
+BalancedGeom balanced_geom(int Hkv) {
+  BalancedGeom g;
+  g.wpg = Hkv < 4 ? Hkv : 4;
+  g.ngroups = (Hkv + g.wpg - 1) / g.wpg;
+  g.nwg = decode_cu_count() * (4 / g.wpg);
+  return g;
+}
+
+int paged_decode_merge_launch(float* ws_o, float* ws_ml, const int64_t* context_lens, void* out, void* q_out,
+                              float* q_scale, int64_t B, int Hq, int D, int BS, int max_blocks, const PartMap& pm,
+                              hipStream_t st) {
+  if (q_out != nullptr) {
+    hipLaunchKernelGGL(paged_decode_merge_quant_group, dim3((unsigned)(Hq * D / 128), (unsigned)B), dim3(128), 0, st,
+                       ws_o, ws_ml, context_lens, (uint16_t*)out, (uint8_t*)q_out, q_scale, Hq, D, BS, max_blocks, pm);
+    return check_launch("paged_decode(merge + quant)");
+  }
+  hipLaunchKernelGGL(paged_decode_merge, dim3((unsigned)((Hq * D + MERGE_THREADS - 1) / MERGE_THREADS), (unsigned)B),
+                     dim3(MERGE_THREADS), 0, st, ws_o, ws_ml, context_lens, (uint16_t*)out, Hq, D, BS, max_blocks, pm);
+  return check_launch("paged_decode(merge)");
 }
 
 }  // namespace

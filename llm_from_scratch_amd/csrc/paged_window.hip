@@ -11,9 +11,15 @@
 // both for one (sequence, kv head), its waves every fourth tile of the split;
 // the waves' partials (o, m, l) meet in LDS.  With one split that is the
 // output, in one launch; else the splits' partials go to the workspace and a
-// second launch merges them.  Unlike contexts, windows are of one length, so
-// equal splits balance: as many as give every CU a workgroup.
-// Bound: HBM, the visible keys and values read once.
+// second launch merges them.  Windows are of one length, so equal splits
+// balance, unless they are long: then contexts inside the window and a last
+// round of workgroups cost more than the paged decode's balanced split does
+// (decode_wave.h, the same walk with one wave per kv head, an equal share of
+// all visible tiles per workgroup).
+// Bound: HBM, the visible keys and values read once.  256 sequences past a
+// window of 4096 (32 / 8 heads of 128, 4.1 GB) take 670 us, 6.1 TB/s; 64 past one
+// of 1024 (16 / 4 of 64, 67 MB) 20 us: 6 us for the launch, the table, the
+// first tile and the merge in LDS, then 4.8 TB/s.
 #include "common.h"
 #include "decode_wave.h"
 
@@ -29,7 +35,7 @@ __global__ __launch_bounds__(64 * WNW, 2) void paged_window_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ kc, const uint16_t* __restrict__ vc,
     const int64_t* __restrict__ ctx_lens, const int32_t* __restrict__ bt, int64_t bt_stride, float* __restrict__ ws_o,
     float* __restrict__ ws_ml, uint16_t* __restrict__ out, int Hkv, int BS, int64_t NB, int max_blocks, int tile,
-    int window, int sinks, float scale_log2, int splits, int per) {
+    Window win, float scale_log2, int splits, int per) {
   using W = DecodeWave<D, G>;
   __shared__ __attribute__((aligned(16))) float p_lds[WNW][DecodeGeom<D>::T * W::GP];
   __shared__ __attribute__((aligned(16))) float part_o[WNW][G * D];
@@ -39,28 +45,24 @@ __global__ __launch_bounds__(64 * WNW, 2) void paged_window_kernel(
   const int kh = blockIdx.x % Hkv, split = blockIdx.x / Hkv % splits;
   const int64_t b = blockIdx.x / Hkv / splits;
   const int Hq = Hkv * G;
-  const int64_t L = max(ctx_lens[b], (int64_t)0), end = min(L, (int64_t)max_blocks * BS);
-  // hidden: tokens sk .. first - 1
-  const int64_t first = max((int64_t)0, L - window), sk = min(min((int64_t)sinks, first), end);
+  const WindowTiles wt(ctx_lens[b], (int64_t)max_blocks * BS, tile, win);
 
   W w(lane, Hkv);
   typename W::QBuf qa;
   w.load_q(qa, q, b, kh, Hq);
   const int32_t* btrow = bt + b * bt_stride;
-  if (sk > 0) {  // the sinks' tiles, from the last split and wave on, which have the fewest of the window's
-    const unsigned n = ((unsigned)sk + tile - 1) >> __builtin_ctz(tile);  // tiles: sk <= sinks < 2^31
-    const int64_t each = splits == 1 ? n : (n + splits - 1) / (unsigned)splits;
-    const int64_t t0 = (splits - 1 - split) * each * tile, t1 = min(sk, t0 + each * tile);
+  if (wt.ns > 0) {  // the sinks' tiles, from the last split and wave on, which have the fewest of the window's
+    const int each = splits == 1 ? wt.ns : (wt.ns + splits - 1) / splits;
+    const int64_t t0 = (int64_t)(splits - 1 - split) * each * tile, t1 = min(wt.sk, t0 + (int64_t)each * tile);
     const int64_t t = t0 + (WNW - 1 - wave) * tile;
     if (t < t1)
       decode_walk<D, G>(w, qa, kc, vc, btrow, BS, NB, tile, scale_log2, kh, t, t1, WNW, max_blocks, p_lds[wave]);
   }
-  const int64_t w0 = first & -(int64_t)tile;  // 16, 32 or 64
-  const int64_t t0 = w0 + (int64_t)split * per * tile, t1 = min(end, t0 + (int64_t)per * tile);
+  const int64_t t0 = wt.w0 + (int64_t)split * per * tile, t1 = min(wt.end, t0 + (int64_t)per * tile);
   const int64_t t = t0 + wave * tile;
   if (t < t1)
     decode_walk<D, G, true>(w, qa, kc, vc, btrow, BS, NB, tile, scale_log2, kh, t, t1, WNW, max_blocks, p_lds[wave],
-                            NoPrologue(), first);
+                            NoPrologue(), wt.first);
   w.reduce_lanes();
   if (w.ts == 0) {
 #pragma unroll
@@ -125,16 +127,24 @@ __global__ __launch_bounds__(128) void paged_window_merge(const float* __restric
   if (t == 0) qs[blockIdx.x] = sc;
 }
 
-int window_cu_count() {
-  static int cached[64] = {0};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (cached[dev] == 0) {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cached[dev] = n;
-  }
-  return cached[dev];
+// Whether a call takes the balanced split: long windows (from 48 tiles, with one
+// query head per kv head from 32) and at least 32 tiles of work per CU.  us,
+// equal splits / balanced, contexts past the window (evenly spaced from 10
+// tokens to past it): 12 / 4 heads of 64, window 4096, 32 sequences 35.2 / 35.3
+// (32.4 / 28.5), 64 55 / 57 (51 / 43), 80 96 / 67 (62 / 53), 256 203 / 180; 32 / 8
+// of 128, 4096, 4 22 / 27, 16 58 / 56 (54 / 41), 256 740 / 680; window 1024 (33
+// tiles), 64 55 / 58 (52 / 57), 256 196 / 192 (173 / 197); 8 / 8 of 64, window
+// 2048 (33 tiles), 64 61 / 55 (56 / 47), 128 120 / 98.
+bool window_balanced(int64_t B, int64_t units, int64_t cus, int64_t tiles, int G) {
+  return B <= BAL_MAXB && tiles >= (G == 1 ? 32 : 48) && units * tiles >= 32 * cus;
+}
+// Equal splits of a window otherwise: one while a wave then has at most two
+// tiles (the merge costs what they do: 5 tiles 8.5 us in two splits, 8.2 in
+// one), else as many as CUs allow.  us, one split / those: one sequence, 12 / 4
+// heads of 64, window 512 10.0 / 8.6, 1024 13.5 / 9.2; 16 sequences 17.3 / 12.1.
+int window_splits(int64_t units, int64_t cus, int64_t tiles) {
+  if (tiles <= 2 * WNW) return 1;
+  return (int)std::max<int64_t>(1, std::min(cus / units, (tiles + WNW - 1) / WNW));
 }
 
 }  // namespace
@@ -144,9 +154,12 @@ using namespace lfs;
 
 extern "C" int64_t lfs_paged_decode_window_workspace_bytes(int64_t B, int32_t num_q_heads, int32_t head_dim) {
   if (B < 0 || num_q_heads <= 0 || head_dim <= 0) return -1;
-  // units * splits <= CUs workgroups of at most 8 query rows, D + 2 floats a row
-  const int64_t cus = window_cu_count();
-  return B > cus ? 0 : 4 * cus * std::min(8, num_q_heads) * ((int64_t)head_dim + 2);
+  const int64_t cus = decode_cu_count();
+  // equal splits: at most a workgroup per CU, of at most 8 query rows; the
+  // balanced split: as lfs_paged_decode; D + 2 floats a row
+  int64_t need = B > cus ? 0 : 4 * cus * std::min(8, num_q_heads) * ((int64_t)head_dim + 2);
+  if (B <= BAL_MAXB) need = std::max(need, 4 * (8 * cus + 2 * B) * num_q_heads * ((int64_t)head_dim + 2) + 4 * (B + 1));
+  return need;
 }
 
 extern "C" int lfs_paged_decode_window(const void* q, const void* k_cache, const void* v_cache,
@@ -173,7 +186,7 @@ extern "C" int lfs_paged_decode_window(const void* q, const void* k_cache, const
               "paged_decode_window: q, caches and out must be 16-byte aligned");
   LFS_REQUIRE((q_out == nullptr) == (q_scale == nullptr), "paged_decode_window: q_out and q_scale go together");
   LFS_REQUIRE(q_out == nullptr || Hq * D % 128 == 0, "paged_decode_window: the quantised output needs Hq*D %% 128 == 0");
-  const int64_t units = B * Hkv, cus = window_cu_count();
+  const int64_t units = B * Hkv, cus = decode_cu_count();
   LFS_REQUIRE(B < (1ll << 24) / Hkv, "paged_decode_window: too many (sequence, kv head) workgroups");
   const int64_t need = lfs_paged_decode_window_workspace_bytes(B, Hq, D);
   LFS_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
@@ -181,21 +194,45 @@ extern "C" int lfs_paged_decode_window(const void* q, const void* k_cache, const
   int tile = 16;
   for (int t = D == 64 ? 64 : 32; t >= 16; t >>= 1)
     if (BS % t == 0) { tile = t; break; }
+  const int G = Hq / Hkv;
+  const float sl2 = scale * 1.4426950408889634f;
+  const Window win{window, sinks};
+  hipStream_t st = (hipStream_t)stream;
   // a window's tiles, whatever its place in them
   const int64_t seen = std::min<int64_t>(window, (int64_t)max_blocks * BS), tiles = (seen + tile - 1) / tile + 1;
-  const int splits = (int)std::max<int64_t>(1, std::min(cus / units, (tiles + WNW - 1) / WNW));
+  if (window_balanced(B, units, cus, tiles, G)) {
+    const BalancedGeom bg = balanced_geom(Hkv);
+    const int64_t rows = ((int64_t)bg.nwg + B * bg.ngroups) * bg.wpg * G;
+    LFS_REQUIRE((int64_t)bg.ngroups * B * (((int64_t)max_blocks * BS + tile - 1) / tile + 2) < (1ll << 31),
+                "paged_decode_window: too many context tiles for the balanced split");
+    float* ws_o = (float*)workspace;
+    float* ws_ml = ws_o + rows * D;
+    int* tp = (int*)(ws_ml + rows * 2);
+    const PartMap pm{0, 0, tp, tile, bg.ngroups, bg.wpg, G, bg.nwg, (int)B};
+    const bool ok = D == 64
+        ? dispatch_balanced<64, true>(G, (unsigned)bg.nwg, dim3(64 * bg.wpg), st, (const uint16_t*)q,
+                                      (const uint16_t*)k_cache, (const uint16_t*)v_cache, context_lens, block_tables,
+                                      bt_stride, ws_o, ws_ml, tp, (uint16_t*)out, Hkv, BS, num_blocks, max_blocks,
+                                      (int)B, tile, sl2, bg.ngroups, win)
+        : dispatch_balanced<128, true>(G, (unsigned)bg.nwg, dim3(64 * bg.wpg), st, (const uint16_t*)q,
+                                       (const uint16_t*)k_cache, (const uint16_t*)v_cache, context_lens, block_tables,
+                                       bt_stride, ws_o, ws_ml, tp, (uint16_t*)out, Hkv, BS, num_blocks, max_blocks,
+                                       (int)B, tile, sl2, bg.ngroups, win);
+    LFS_REQUIRE(ok, "paged_decode_window: unsupported group size %d", G);
+    const int rc = check_launch("paged_decode_window(balanced split)");
+    if (rc) return rc;
+    return paged_decode_merge_launch(ws_o, ws_ml, context_lens, out, q_out, q_scale, B, Hq, D, BS, max_blocks, pm, st);
+  }
+  const int splits = window_splits(units, cus, tiles);
   const int per = (int)((tiles + splits - 1) / splits);
-  const int G = Hq / Hkv;
   float* ws_o = (float*)workspace;
   float* ws_ml = ws_o + (int64_t)B * Hq * splits * D;
-  const float sl2 = scale * 1.4426950408889634f;
-  hipStream_t st = (hipStream_t)stream;
 #define LFS_G(DD, GG)                                                                                                 \
   case GG:                                                                                                            \
     hipLaunchKernelGGL((paged_window_kernel<DD, GG>), dim3((unsigned)(units * splits)), dim3(64 * WNW), 0, st,        \
                        (const uint16_t*)q, (const uint16_t*)k_cache, (const uint16_t*)v_cache, context_lens,          \
                        block_tables, bt_stride, ws_o, ws_ml, (uint16_t*)out, Hkv, BS, num_blocks, max_blocks, tile,   \
-                       window, sinks, sl2, splits, per);                                                              \
+                       win, sl2, splits, per);                                                                        \
     break;
   if (D == 64) {
     switch (G) {
