@@ -213,12 +213,20 @@ __device__ __forceinline__ bool ranked_item(const int32_t* cu_q, const int32_t* 
 }
 
 // WIN: a query at position p sees the keys t <= p with t > p - window or t <
-// sinks.  The workgroup walks the tiles of the sinks and those from its first
-// row's window on; keys in between, and within those tiles, that none of its
-// rows sees are never read (their blocks may be freed): their places hold a
-// visible key's row, masked.
+// sinks.  The workgroup's keys are those of the sinks and those from its first
+// row's window on, in 16-key halves that follow each other without a gap: place
+// v of the walk is key v in the sinks' halves (v < vs), key v + shift in the
+// window's.  So a tile may hold both, and a window costs less than two halves
+// beyond its keys.  Keys that none of the workgroup's rows sees are never read
+// (their blocks may be freed): of the halves' own, their places hold a visible
+// key's row, masked.  In whole tiles, the sinks in one of their own, 16 x 2048
+// tokens (12 / 4 heads of 64, window 512) took 94 us, four chunks of 2048 to 16384
+// tokens (32 / 8 of 128, window 4096) 651; in halves 89 and 620: 510 and 888
+// TFLOP/s of visible pairs.  Bound as without a window, and by the tiles at a
+// window's two ends, which are computed whole.  At D = 64 in 128 registers, some
+// spilled: in 137, three waves a SIMD, the first took 99 us.
 template <int D, bool PAGED, bool WIN>
-__global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
+__global__ __launch_bounds__(64 * NW, WIN && D == 64 ? 4 : 2) void prefill_attention_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, const int32_t* __restrict__ bt,
     int64_t bt_stride, int64_t num_slots, uint16_t* __restrict__ out, Div dB, Div dHkv, Div G, Div dBS,
@@ -276,19 +284,20 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
                         ? -1 : __builtin_amdgcn_readfirstlane(off + (int)(min(r0 + RW * wave + RW - 1, rows - 1) / G));
   const int wlast = off + (int)(min(r0 + RW * NW - 1, rows - 1) / G);
   const int nkt = min(lk, wlast + 1) <= 0 ? 0 : (min(lk, wlast + 1) + KT - 1) / KT;
-  // WIN: the workgroup's hidden keys hlo .. hhi - 1, its tiles of sinks (0 ..
-  // ns - 1) and its window's first; a wave's rows all miss the keys to pmiss
-  int hlo = 0, hhi = 0, ns = 0, tw = 0, pmiss = 0;
+  // WIN: places v0 .. v1 - 1 hold keys that no row of the workgroup sees; a
+  // wave's rows all miss the keys from the sinks to pmiss
+  int vs = 0, shift = 0, v0 = 0, v1 = 0, pmiss = 0;
   if constexpr (WIN) {
-    hhi = max(0, off + (int)(r0 / G) - window + 1);
-    hlo = min(sinks, hhi);
-    if (hlo == hhi) hlo = hhi = 0;
-    tw = hhi / KT;
-    ns = min((hlo + KT - 1) / KT, tw);
+    // of the window of the workgroup's first row
+    const int first = __builtin_amdgcn_readfirstlane(max(0, off + (int)(r0 / G) - window + 1));
+    v0 = min(sinks, first);
+    vs = min((v0 + 15) & ~15, first & ~15);
+    shift = (first & ~15) - vs;
+    v1 = vs + (first & 15);
     pmiss = pfirst - window;
   }
-  const int nt = WIN ? ns + max(0, nkt - tw) : nkt;
-  auto tile_key = [&](int j) { return (!WIN || j < ns ? j : j - ns + tw) * KT; };
+  auto key_at = [&](int v) { return WIN && v >= vs ? v + shift : v; };
+  const int nt = WIN ? __builtin_amdgcn_readfirstlane((max(0, min(lk, wlast + 1) - shift) + KT - 1) / KT) : nkt;
   const int64_t rowb = (int64_t)Hkv * RB;  // bytes per token of k / v
   const uint8_t* kb = reinterpret_cast<const uint8_t*>(k) + (int64_t)kh * RB;
   const uint8_t* vb = reinterpret_cast<const uint8_t*>(v) + (int64_t)kh * RB;
@@ -299,7 +308,8 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
   // fetches the chunk that belongs there.
   const int crow = RPW * wave + lane / (D / 8);  // row of instruction 0
   unsigned krow[NC], vrow[NC];  // byte offsets from local row 0
-  const int crow0 = PAGED ? crow & 15 : crow;
+  constexpr bool HALF = PAGED || WIN;  // local row 0 is the wave's first (else the tile's)
+  const int crow0 = HALF ? crow & 15 : crow;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int r = crow + RPC * c;
@@ -313,17 +323,14 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
   // an invalid table entry reads slot 0.  The entry is loaded one tile ahead.
   const int hoff = (RPW * wave) & ~15;  // the wave's half within a tile
   int blk = 0, boff = 0, lblk = 0, loff = 0;  // block and offset of the half's first key, and of key lk - 1
-  // WIN: the key in the place of the first of the half at key t: key hhi for a
-  // half that nobody sees
-  auto half_key = [&](int t) { return t >= lk ? max(lk - 1, 0) : t >= hlo && t + 16 <= hhi ? hhi : t; };
   if constexpr (PAGED && !WIN) {
     boff = hoff;
     while (boff >= BS) boff -= BS, ++blk;
     lblk = (int)((unsigned)max(lk - 1, 0) / dBS), loff = max(lk - 1, 0) - lblk * BS;
   }
-  auto entry = [&](int t) -> int {  // table entry of the half that starts at key t
+  auto entry = [&](int t) -> int {  // table entry of the half that starts at key (WIN: place) t
     if constexpr (WIN) {
-      const int key = half_key(t);
+      const int key = min(key_at(t), max(lk - 1, 0));
       blk = (int)((unsigned)key / dBS);
       boff = key - blk * BS;
     }
@@ -332,31 +339,26 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
     return bt[e];
   };
   int next = 0;
-  if constexpr (PAGED) next = entry(tile_key(0) + hoff);
-  // copies of the K or V rows of the tile at key t0 into buffer buf (0 / 1;
+  if constexpr (PAGED) next = entry(hoff);
+  // copies of the K or V rows of the tile at key (WIN: place) t0 into buffer buf (0 / 1;
   // V tiles are buffers 2 / 3); first: token or slot of its local row 0
   auto fetch = [&](const uint8_t* base, int64_t first, int t0, int buf, const unsigned (&rows16)[NC]) {
-    const int valid = PAGED ? max(0, lk - 1 - (t0 + hoff)) : lk - 1 - t0;  // last local row that may be read
+    // last local row that may be read
+    const int valid = HALF ? max(0, lk - 1 - key_at(t0 + hoff)) : lk - 1 - t0;
     const uint8_t* p = base + first * rowb;
     const unsigned dst = lbase + buf * TB + RPW * wave * RB;
-    const int th = t0 + hoff;  // the wave's first key
-    if (WIN && th < hhi && th + 16 > hlo) {
-      // hidden keys among the wave's 16, whose places take a visible row of
-      // theirs: the last sink's, else the window's first (a half that nobody
-      // sees has that as its row 0)
-      const int key0 = PAGED ? th : t0;  // of local row 0
-      const bool none = PAGED && th >= hlo && th + 16 <= hhi;
+    const int th = t0 + hoff;  // the wave's first place
+    if (WIN && th < v1 && th + 16 > v0) {
+      // hidden keys among the wave's 16: the last sink's row, else the window's first
       unsigned at[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int r = crow0 + RPC * c, key = key0 + r;
-        int to = min(r, valid);
-        if (none) to = 0;
-        else if (key >= hlo && key < hhi) to = (key0 < hlo ? hlo - 1 : hhi) - key0;
+        const int r = crow0 + RPC * c, v = th + r;
+        const int to = min(v >= v0 && v < v1 ? (th < v0 ? v0 - 1 : v1) - th : r, valid);
         at[c] = rows16[c] + (unsigned)(to - r) * (unsigned)rowb;
       }
       copy_rows<NC>(p, at, dst);
-    } else if (valid >= (PAGED ? 15 : KT - 1)) {
+    } else if (valid >= (HALF ? 15 : KT - 1)) {
       copy_rows<NC>(p, rows16, dst);
     } else {
       unsigned at[NC];
@@ -367,7 +369,7 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
     }
   };
   int64_t kfirst = 0;  // local row 0 of the K tile last fetched
-  auto fetch_k = [&](int t0, int t1, int buf) {  // t1: key of the tile after it
+  auto fetch_k = [&](int t0, int buf) {
     if constexpr (PAGED) {
       const int b = __builtin_amdgcn_readfirstlane(next);
       kfirst = b < 0 || (int64_t)b * BS >= num_slots ? 0 : (int64_t)b * BS + (WIN || t0 + hoff < lk ? boff : loff);
@@ -376,10 +378,10 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
         while (boff >= BS) boff -= BS, ++blk;
       }
     } else {
-      kfirst = (int64_t)k0 + t0;
+      kfirst = (int64_t)k0 + (WIN ? min(key_at(t0 + hoff), max(lk - 1, 0)) : t0);
     }
     fetch(kb, kfirst, t0, buf, krow);
-    if constexpr (PAGED) next = entry(t1 + hoff);
+    if constexpr (PAGED) next = entry(t0 + KT + hoff);
   };
 
   // Q^T (B operand): lane l supplies row l % 32, dims 16c + 8h .. +7
@@ -418,14 +420,37 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
   auto mask_max = [&](v16f (&s)[NB], int t0) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) s[b] *= scale_log2;
-    if (t0 + KT - 1 > pfirst || (WIN && t0 <= plast - window && t0 + KT > sinks)) {
+    if constexpr (!WIN) {
+      if (t0 + KT - 1 > pfirst) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = t0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4;
-          if (key > qp || (WIN && key <= qp - window && key >= sinks)) s[b][r] = -INFINITY;
-        }
+          for (int r = 0; r < 16; ++r)
+            if (t0 + 32 * b + 8 * (r / 4) + 4 * h + r % 4 > qp) s[b][r] = -INFINITY;
+      }
+    } else {
+      // of element r of block b: its half's first key, and how far past it
+      auto half = [&](int b, int r) { return key_at(t0 + 32 * b + 16 * (r / 8)); };
+      auto in_half = [&](int r) { return 8 * (r / 4 % 2) + 4 * h + r % 4; };
+      const int last = key_at(t0 + KT - 1), past = t0 + KT > vs ? key_at(max(t0, vs)) : t0;
+      if (last > pfirst) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (half(b, r) > qp - in_half(r)) s[b][r] = -INFINITY;
+      }
+      // where the tile holds places of hidden keys, or past the sinks one that
+      // the wave's last row misses
+      if ((t0 < v1 && t0 + KT > v0 && v0 < v1) || (past <= plast - window && last >= sinks)) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = half(b, r) + in_half(r);
+            if (key <= qp - window && key >= sinks) s[b][r] = -INFINITY;
+          }
+      }
     }
     float mx = s[0][0];
 #pragma unroll
@@ -472,11 +497,11 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
   constexpr int NS = NB * NDC, NP = KT / 16 * NDB;  // MFMAs of S^T and of O^T per tile
   constexpr int AH = 4;                             // operand reads ahead of them
   if (nt > 0) {
-    fetch_k(tile_key(0), tile_key(1), 0);
-    fetch(vb, kfirst, tile_key(0), 2, vrow);
+    fetch_k(0, 0);
+    fetch(vb, kfirst, 0, 2, vrow);
   }
   for (int j = 0; j < nt; ++j) {
-    const int t0 = tile_key(j), buf = j & 1;
+    const int t0 = j * KT, buf = j & 1;
     // tile j is in LDS for every wave; every wave is done with tile j - 1,
     // whose buffers the next copies fill
     __builtin_amdgcn_s_waitcnt(0);
@@ -486,11 +511,11 @@ __global__ __launch_bounds__(64 * NW, 2) void prefill_attention_kernel(
     for (int n = 0; n < AH; ++n) kf[n] = k_frag(n, buf);
     __builtin_amdgcn_sched_barrier(0);
     if (j + 1 < nt) {
-      fetch_k(tile_key(j + 1), tile_key(j + 2), buf ^ 1);
-      fetch(vb, kfirst, tile_key(j + 1), 2 + (buf ^ 1), vrow);
+      fetch_k(t0 + KT, buf ^ 1);
+      fetch(vb, kfirst, t0 + KT, 2 + (buf ^ 1), vrow);
     }
-    if (WIN && t0 + KT - 1 <= pmiss && t0 >= sinks) continue;  // none of the wave's rows sees a key
-    if (t0 > plast) continue;  // the wave's rows end before this tile (it still copies)
+    if (WIN && t0 >= vs && key_at(t0) >= sinks && key_at(t0 + KT - 1) <= pmiss) continue;  // no row sees a key
+    if (key_at(t0) > plast) continue;  // the wave's rows end before this tile (it still copies)
     v16f s[NB];
     uint32_t pw[NB][8];
 #pragma unroll

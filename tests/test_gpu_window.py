@@ -79,7 +79,7 @@ def test_prefill_whole_prompts(Hq, Hkv, D, window, sinks):
 
 @pytest.mark.parametrize("Hq,Hkv,D", HEADS[:4])
 @pytest.mark.parametrize("BS", [16, 48, 256])
-@pytest.mark.parametrize("window,sinks", [(1, 0), (33, 5), (200, 0), (257, 64), (100, 300)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (33, 5), (21, 5), (200, 0), (257, 64), (100, 300), (645, 250)])
 def test_prefill_chunks_over_the_pool(Hq, Hkv, D, BS, window, sinks):
     """New tokens behind cached ones; blocks behind the first query's window
     are freed and everything nobody sees is NaN."""
