@@ -20,6 +20,9 @@ Interface (nano-vLLM style, as the runner expects):
     hidden = model(input_ids [T], positions [T])      # bf16 [T, d_model]
     logits = model.compute_logits(hidden)             # bf16 [T, vocab]
 
+DecodeModelConfig also gives the attention a sliding window with sinks and
+norms per head (qk_head_norm_rope_store), which the reference has not.
+
 Kernels per layer: add_rmsnorm (+act_quant) -> qkv FP8 GEMM ->
 qk_norm_rope_store -> paged decode (split + merge with the act_quant of its
 output; where a single launch is the default split, one launch does the
@@ -67,6 +70,18 @@ class DecodeModelConfig:
     rope_theta: float = 10000.0
     max_model_length: int = 4096
     rms_eps: float = 1e-5
+    # attention over the last sliding_window tokens and the first
+    # num_sink_tokens ones (None: over the whole context)
+    sliding_window: Optional[int] = None
+    num_sink_tokens: int = 0
+    # "full": q_norm over d_model and k_norm over Hkv*D, as the reference;
+    # "head": over each head's D values, with weights shared by the heads
+    qk_norm: str = "full"
+
+    def __post_init__(self):
+        if self.qk_norm not in ("full", "head"):
+            raise ValueError(f'qk_norm must be "full" or "head", got {self.qk_norm!r}')
+        kernels._window_args(self.sliding_window, self.num_sink_tokens)
 
     @property
     def head_dim(self) -> int:
@@ -74,7 +89,8 @@ class DecodeModelConfig:
 
     def runner_config(self, **kw) -> dict:
         d = dict(num_layers=self.num_layers, num_heads=self.num_heads, num_kv_heads=self.num_kv_heads,
-                 hidden_size=self.d_model, head_dim=self.head_dim, max_model_length=self.max_model_length)
+                 hidden_size=self.d_model, head_dim=self.head_dim, max_model_length=self.max_model_length,
+                 sliding_window=self.sliding_window, num_sink_tokens=self.num_sink_tokens)
         d.update(kw)
         return d
 
@@ -94,7 +110,9 @@ class DecodeModelConfig:
             p = f"layers.{i}."
             for name, n_out in (("q_proj", d), ("k_proj", kv), ("v_proj", kv), ("output_proj", d)):
                 lin(p + "att." + name, n_out, d)
-            keys[p + "att.q_norm.weight"], keys[p + "att.k_norm.weight"] = (d,), (kv,)
+            per_head = self.qk_norm == "head"
+            keys[p + "att.q_norm.weight"] = (self.head_dim if per_head else d,)
+            keys[p + "att.k_norm.weight"] = (self.head_dim if per_head else kv,)
             keys[p + "att_norm.weight"], keys[p + "ffn_norm.weight"] = (d,), (d,)
             keys[p + "ffn.gate.weight"] = (self.n_routed_experts, d)
             keys[p + "ffn.gate.expert_bias"] = (self.n_routed_experts,)
@@ -159,9 +177,12 @@ class PagedGQAAttention(nn.Module):
         self.q_dim, self.kv_dim = d, cfg.num_kv_heads * D
         self.qkv_proj = FP8Linear(d, d + 2 * self.kv_dim, device=device)
         self.output_proj = FP8Linear(d, d, device=device)
+        self.head_norm = cfg.qk_norm == "head"
+        self.window, self.sinks = cfg.sliding_window, cfg.num_sink_tokens
         # torch.nn.RMSNorm default eps (machine epsilon of the fp32 compute)
-        self.q_norm = RMSNorm(d, eps=torch.finfo(torch.float32).eps, device=device)
-        self.k_norm = RMSNorm(cfg.num_kv_heads * D, eps=torch.finfo(torch.float32).eps, device=device)
+        self.q_norm = RMSNorm(D if self.head_norm else d, eps=torch.finfo(torch.float32).eps, device=device)
+        self.k_norm = RMSNorm(D if self.head_norm else cfg.num_kv_heads * D, eps=torch.finfo(torch.float32).eps,
+                              device=device)
         self.rope = rope
         self.k_cache = torch.empty(0)  # pool views attached by the model runner
         self.v_cache = torch.empty(0)
@@ -175,7 +196,7 @@ class PagedGQAAttention(nn.Module):
         assert self.k_cache.numel(), "PagedGQAAttention needs the KV pool (ModelRunner.allocate_kv_cache)"
         qkv = self.qkv_proj.gemm(xq, xs)
         shape = (T, self.num_heads, self.num_kv_heads, self.head_dim, ctx.block_tables.size(1),
-                 self.k_cache.size(1)) if not ctx.is_prefill else None
+                 self.k_cache.size(1)) if not ctx.is_prefill and self.window is None and not self.head_norm else None
         # the paired order (one workgroup per (sequence, kv head), a long and
         # a short one per CU) when the output projection can quantise its
         # input itself; else one workgroup per pair of kv heads with the
@@ -201,24 +222,26 @@ class PagedGQAAttention(nn.Module):
                 trace.update(qkv=qkv, q=q, att_o=o, att_out=out)
             return out
         whole = ctx.is_prefill and ctx.block_tables is None  # whole prompts: the keys of this very call
-        q = kernels.qk_norm_rope_store(qkv, self.q_norm.weight, self.k_norm.weight, self.rope.cos_sin_cached,
-                                       positions, self.num_heads, self.num_kv_heads, self.q_norm.eps,
-                                       self.k_cache, self.v_cache, ctx.slot_mapping, return_kv=whole)
+        norm_rope_store = kernels.qk_head_norm_rope_store if self.head_norm else kernels.qk_norm_rope_store
+        q = norm_rope_store(qkv, self.q_norm.weight, self.k_norm.weight, self.rope.cos_sin_cached,
+                            positions, self.num_heads, self.num_kv_heads, self.q_norm.eps,
+                            self.k_cache, self.v_cache, ctx.slot_mapping, return_kv=whole)
+        seen = dict(window=self.window, sinks=self.sinks)
         if ctx.is_prefill:
             if ctx.block_tables is not None:  # prefix-cache hit: keys from the pool
                 o = kernels.flash_attn_varlen_func(q, self.k_cache, self.v_cache, ctx.cu_seqlens_q,
                                                    ctx.cu_seqlens_k, ctx.max_seqlen_q, ctx.max_seqlen_k,
-                                                   self.scale, block_table=ctx.block_tables)
+                                                   self.scale, block_table=ctx.block_tables, **seen)
             else:
                 q, k, v = q
                 o = kernels.flash_attn_varlen_func(q, k, v, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
-                                                   ctx.max_seqlen_q, ctx.max_seqlen_k, self.scale)
+                                                   ctx.max_seqlen_q, ctx.max_seqlen_k, self.scale, **seen)
             o = o.reshape(T, -1)
             out = self.output_proj(o)
         else:
             # the merge also writes the output projection's FP8 input (act_quant fused)
             o, oq, os_ = kernels.paged_attention_decode(q, self.k_cache, self.v_cache, ctx.context_lens,
-                                                        ctx.block_tables, self.scale, quant=True)
+                                                        ctx.block_tables, self.scale, quant=True, **seen)
             o = o.reshape(T, -1)
             out = self.output_proj.gemm(oq, os_)
         if trace is not None:

@@ -14,10 +14,17 @@ Behavioural fixes (the reference's bugs are not copied):
     would cache every block of a block-aligned prompt that matches another
     sequence's, leaving the prefill no query token to sample from): it is
     recomputed into a fresh block, so num_cached_tokens < num_tokens.
+
+Beyond the reference: blocks behind a sliding window go back to the pool while
+their sequence runs (``release_behind``), a running sequence's blocks are shared
+with a fork of it (``fork``), and the blocks in use move to the pool's start
+(``pack``).  The last two return the block copies that go with them
+(kernels.copy_kv_blocks).
 """
 from __future__ import annotations
 
 from collections import deque
+from typing import Optional
 
 import numpy as np
 import xxhash
@@ -43,8 +50,9 @@ class Block:
 
 
 class BlockManager:
-    def __init__(self, num_blocks: int, block_size: int):
+    def __init__(self, num_blocks: int, block_size: int, window: Optional[int] = None, sinks: int = 0):
         self.block_size = block_size
+        self.window, self.sinks = window, sinks
         self.blocks = [Block(i) for i in range(num_blocks)]
         self.hash_to_block_id: dict[int, int] = {}
         self.free_block_ids: deque[int] = deque(range(num_blocks))
@@ -104,12 +112,77 @@ class BlockManager:
 
     def deallocate(self, seq: Sequence) -> None:
         for block_id in seq.block_table:
-            block = self.blocks[block_id]
-            block.ref_count -= 1
-            if block.ref_count == 0:
-                self._deallocate_block(block_id)
+            if block_id >= 0:
+                self._drop(block_id)
         seq.block_table = []
         seq.num_cached_tokens = 0
+        seq.num_released_blocks = 0
+
+    def _drop(self, block_id: int) -> None:
+        block = self.blocks[block_id]
+        block.ref_count -= 1
+        if block.ref_count == 0:
+            self._deallocate_block(block_id)
+
+    def release_behind(self, seq: Sequence) -> None:
+        """Free the sequence's blocks that no token from its newest on sees: all
+        of their positions behind the newest token's window and none among the
+        sinks.  Their table entries become -1.  The last two blocks stay (the
+        hash of a block that fills takes the one before it)."""
+        if self.window is None:
+            return
+        BS, table = self.block_size, seq.block_table
+        first = -(-self.sinks // BS)  # blocks of the sinks
+        behind = max(0, seq.num_tokens - self.window) // BS  # blocks wholly before the newest token's window
+        end = min(behind, len(table) - 2)
+        for i in range(first + seq.num_released_blocks, end):
+            self._drop(table[i])
+            table[i] = -1
+        seq.num_released_blocks = max(seq.num_released_blocks, end - first)
+
+    def _last_is_partial(self, seq: Sequence) -> bool:
+        """Whether the sequence's last block has room: the newest token's keys
+        are not stored yet, so num_tokens - 1 are."""
+        return (seq.num_tokens - 1) % self.block_size != 0
+
+    def can_fork(self, seq: Sequence, n: int = 1) -> bool:
+        return not self._last_is_partial(seq) or len(self.free_block_ids) >= n
+
+    def fork(self, parent: Sequence, child: Sequence) -> list[tuple[int, int]]:
+        """Give a fork of a running sequence its blocks: the parent's, shared,
+        but for a last block that both would go on filling, of which it gets a
+        copy.  Returns the (source, destination) block copies to make."""
+        assert child.block_table == parent.block_table and parent.block_table
+        copies = []
+        if self._last_is_partial(parent):
+            source = self.blocks[parent.block_table[-1]]
+            block = self._allocate_block(self.free_block_ids[0])
+            block.update(source.hash, list(source.token_ids))
+            child.block_table[-1] = block.block_id
+            copies.append((source.block_id, block.block_id))
+        shared = child.block_table[:-1] if copies else child.block_table
+        for block_id in shared:
+            if block_id >= 0:
+                self.blocks[block_id].ref_count += 1
+        return copies
+
+    def pack(self) -> list[tuple[int, int]]:
+        """Move the blocks in use to the ids 0 .. n - 1, n their number: those at
+        or past n, in order, to the free ones below.  Returns the (source,
+        destination) block copies to make; the caller renames table entries
+        alike."""
+        n = len(self.used_block_ids)
+        sources = sorted(b for b in self.used_block_ids if b >= n)
+        holes = [b for b in range(n) if b not in self.used_block_ids]
+        for src, dst in zip(sources, holes):
+            a, b = self.blocks[src], self.blocks[dst]
+            b.hash, b.ref_count, b.token_ids = a.hash, a.ref_count, a.token_ids
+            if self.hash_to_block_id.get(a.hash) == src:
+                self.hash_to_block_id[a.hash] = dst
+            a.reset()
+        self.used_block_ids = set(range(n))
+        self.free_block_ids = deque(range(n, len(self.blocks)))
+        return list(zip(sources, holes))
 
     def can_append(self, seq: Sequence) -> bool:
         if seq.num_tokens % self.block_size == 1:

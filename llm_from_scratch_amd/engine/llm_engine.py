@@ -32,7 +32,9 @@ class LLMEngine:
             max_cached_blocks=min(config.get("max_cached_blocks", self.model_runner.num_available_kv_blocks),
                                   self.model_runner.num_available_kv_blocks),
             block_size=block_size,
-            eos=config.get("eos", 50256))
+            eos=config.get("eos", 50256),
+            sliding_window=config.get("sliding_window"),
+            num_sink_tokens=config.get("num_sink_tokens", 0))
         self.tokenizer = tokenizer
         self.generator = generator
         self.verbose = verbose
@@ -52,6 +54,24 @@ class LLMEngine:
             assert self.tokenizer is not None, "string prompts need a tokenizer"
             prompt = self.tokenizer.encode(prompt)
         self.scheduler.add_sequence(Sequence(list(prompt), sampling_params))
+
+    def fork(self, seq_id: int, n: int = 1) -> list[int]:
+        """n branches of a running sequence, between steps: each goes on from its
+        tokens with draws of its own.  They share its blocks; only a partly
+        filled last one is copied.  Returns their ids."""
+        parent = next((s for s in self.scheduler.running if s.seq_id == seq_id), None)
+        if parent is None:
+            raise ValueError(f"no running sequence {seq_id}")
+        children, copies = self.scheduler.fork(parent, n)
+        self.model_runner.copy_blocks(copies)
+        return [c.seq_id for c in children]
+
+    def pack_kv_cache(self) -> int:
+        """Move the blocks in use to the start of the pool, between steps;
+        returns their number n: kv_cache[:, :, :n] then holds every running
+        sequence's keys and values."""
+        self.model_runner.copy_blocks(self.scheduler.pack())
+        return len(self.scheduler.block_manager.used_block_ids)
 
     def generate(self, prompts: Seq[Union[str, list[int]]], sampling_params: SamplingParams) -> dict:
         for p in prompts:

@@ -78,20 +78,33 @@ class Sampler:
     The noise comes from a counter-based generator keyed by a seed and a
     per-call offset: the seed is the given generator's initial seed, or one
     drawn from torch's default generator on first use (so torch.manual_seed
-    makes runs repeatable); the offset advances every call."""
+    makes runs repeatable); the offset advances every call.
+
+    With any of ``top_k`` (int32 [B]), ``top_p`` and ``min_p`` (fp32 [B]) the
+    tokens come from kernels.sample_filtered instead, on uniform numbers of a
+    generator with the same seed."""
 
     def __init__(self):
         self._seed: Optional[int] = None
         self._offset = 0
+        self._uniforms: dict = {}  # (device, seed): generator
 
     def __call__(self, logits: torch.Tensor, temperatures: torch.Tensor,
-                 generator: Optional[torch.Generator] = None) -> torch.Tensor:
+                 generator: Optional[torch.Generator] = None, top_k: Optional[torch.Tensor] = None,
+                 top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None) -> torch.Tensor:
         if generator is not None:
             seed = generator.initial_seed()
         else:
             if self._seed is None:
                 self._seed = int(torch.randint(0, 2 ** 62, (1,)).item())
             seed = self._seed
+        if top_k is not None or top_p is not None or min_p is not None:
+            key = (logits.device, seed)
+            if key not in self._uniforms:
+                self._uniforms[key] = torch.Generator(device=logits.device).manual_seed(seed)
+            u = torch.rand(logits.size(0), generator=self._uniforms[key], device=logits.device)
+            return kernels.sample_filtered(logits.to(torch.bfloat16), temperatures.to(torch.float32), u, top_k=top_k,
+                                           top_p=top_p, min_p=min_p)
         offset = self._offset
         self._offset += (logits.size(-1) + 3) // 4
         return kernels.sample_gumbel(logits.to(torch.bfloat16), temperatures.to(torch.float32), seed, offset)
@@ -220,6 +233,20 @@ class ModelRunner:
         return torch.tensor([s.temperature for s in seqs], dtype=torch.float32,
                             pin_memory=True).to(self.device, non_blocking=True)
 
+    def prepare_filters(self, seqs: list[Sequence]) -> dict:
+        """The sampling filters of the batch that any of its sequences has."""
+        filters = {}
+        for name, dtype, off in (("top_k", torch.int32, 0), ("top_p", torch.float32, 1.0), ("min_p", torch.float32, 0.0)):
+            values = [getattr(s, name) for s in seqs]
+            if any(v != off for v in values):
+                filters[name] = torch.tensor(values, dtype=dtype, pin_memory=True).to(self.device, non_blocking=True)
+        return filters
+
+    def copy_blocks(self, copies: list[tuple[int, int]]) -> None:
+        """Copy whole blocks of every layer's K and V: (source, destination)."""
+        if copies:
+            kernels.copy_kv_blocks(self.kv_cache, *zip(*copies))
+
     # --------------------------------------------------------------- run ---
     @torch.inference_mode()
     def run_model(self, input_ids: torch.Tensor, positions: torch.Tensor, is_prefill: bool) -> torch.Tensor:
@@ -260,7 +287,7 @@ class ModelRunner:
             # one logit row per sequence: the last prompt token
             last = get_context().cu_seqlens_q[1:] - 1
             logits = logits[last]
-        token_ids = self.sampler(logits, self.prepare_sample(seqs), generator).tolist()
+        token_ids = self.sampler(logits, self.prepare_sample(seqs), generator, **self.prepare_filters(seqs)).tolist()
         reset_context()
         return token_ids
 

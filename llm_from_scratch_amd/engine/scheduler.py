@@ -14,6 +14,7 @@ Behavioural fixes (the reference's bugs are not copied):
 from __future__ import annotations
 
 from collections import deque
+from typing import Optional
 
 from .block_manager import BlockManager
 from .sequence import Sequence, SequenceStatus
@@ -21,8 +22,8 @@ from .sequence import Sequence, SequenceStatus
 
 class Scheduler:
     def __init__(self, max_num_sequences: int, max_num_batched_tokens: int, max_cached_blocks: int,
-                 block_size: int, eos: int):
-        self.block_manager = BlockManager(max_cached_blocks, block_size)
+                 block_size: int, eos: int, sliding_window: Optional[int] = None, num_sink_tokens: int = 0):
+        self.block_manager = BlockManager(max_cached_blocks, block_size, sliding_window, num_sink_tokens)
         self.max_num_batched_tokens = max_num_batched_tokens
         self.max_num_sequences = max_num_sequences
         self.waiting: deque[Sequence] = deque()
@@ -58,11 +59,15 @@ class Scheduler:
 
         while self.running:
             seq = self.running.popleft()
+            self.block_manager.release_behind(seq)
             if not self.block_manager.can_append(seq):
                 if self.running:
-                    self.preempt(self.running.pop())
-                    self.running.appendleft(seq)  # retry it with the freed blocks
-                    continue
+                    self.running.appendleft(seq)
+                    victim = self._victim()
+                    self.running.remove(victim)
+                    self.preempt(victim)
+                    continue  # the first running sequence is tried with the freed blocks
+                self._victim([seq])
                 self.preempt(seq)
                 break
             if num_tokens >= self.max_num_batched_tokens or len(scheduled) >= self.max_num_sequences:
@@ -74,6 +79,40 @@ class Scheduler:
         if scheduled:
             self.running.extendleft(reversed(scheduled))
         return scheduled, False
+
+    def _victim(self, among=None) -> Sequence:
+        """The newest running sequence whose context the pool can hold at once,
+        as its prefill will ask: behind a sliding window one may outgrow the
+        pool, and could never be resumed."""
+        total = len(self.block_manager.blocks)
+        for seq in reversed(self.running if among is None else among):
+            if seq.num_blocks <= total:
+                return seq
+        raise RuntimeError("the KV pool is full, and no running sequence fits it to be resumed later")
+
+    def fork(self, seq: Sequence, n: int = 1) -> tuple[list[Sequence], list[tuple[int, int]]]:
+        """n sequences that go on from a running one's tokens, on its blocks:
+        (children, the block copies to make before the next step)."""
+        if seq not in self.running:
+            raise ValueError(f"sequence {seq.seq_id} is not running: only a running one has keys to share")
+        if not self.block_manager.can_fork(seq, n):
+            raise RuntimeError(f"no free blocks for {n} forks of sequence {seq.seq_id}")
+        children, copies = [], []
+        for _ in range(n):
+            child = seq.fork()
+            copies += self.block_manager.fork(seq, child)
+            self.running.append(child)
+            children.append(child)
+        return children, copies
+
+    def pack(self) -> list[tuple[int, int]]:
+        """Move the blocks in use to the pool's start: the block copies to make
+        before the next step."""
+        copies = self.block_manager.pack()
+        moved = dict(copies)
+        for seq in self.running:
+            seq.block_table = [moved.get(b, b) for b in seq.block_table]
+        return copies
 
     def preempt(self, seq: Sequence) -> None:
         self.block_manager.deallocate(seq)

@@ -19,14 +19,20 @@ from typing import Optional
 @dataclass
 class SamplingParams:
     """utils/sampler.py:7-23 of the reference, plus the ``max_model_length``
-    field engine/sequence.py:34 reads from it."""
+    field engine/sequence.py:34 reads from it and the filters of
+    kernels.sample_filtered (top_k 0, top_p 1 and min_p 0: none)."""
     temperature: float = 1.0
     max_tokens: int = 256
     ignore_eos: bool = False
     max_model_length: Optional[int] = None
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
 
     def __post_init__(self):
         assert self.temperature > 1e-10, "greedy sampling is not permitted"
+        assert self.top_k >= 0 and 0 < self.top_p <= 1 and 0 <= self.min_p <= 1, \
+            "top_k must be >= 0, top_p in (0, 1], min_p in [0, 1]"
 
 
 class SequenceStatus(Enum):
@@ -48,11 +54,22 @@ class Sequence:
         self.num_tokens = len(self.token_ids)
         self.num_prompt_tokens = len(self.token_ids)
         self.num_cached_tokens = 0
-        self.block_table: list[int] = []
+        self.block_table: list[int] = []  # -1: a block freed behind the sliding window
+        self.num_released_blocks = 0  # from the first block without sinks on
+        self.top_k, self.top_p, self.min_p = sp.top_k, sp.top_p, sp.min_p
         self.temperature = sp.temperature
         self.max_tokens = sp.max_tokens
         self.ignore_eos = sp.ignore_eos
         self.max_model_length = sp.max_model_length
+
+    def fork(self) -> "Sequence":
+        """A sequence of its own id that continues from the same tokens (its
+        blocks still the parent's: BlockManager.fork)."""
+        child = copy(self)
+        child.seq_id = next(Sequence.counter)
+        child.token_ids = copy(self.token_ids)
+        child.block_table = copy(self.block_table)
+        return child
 
     def __len__(self):
         return self.num_tokens
