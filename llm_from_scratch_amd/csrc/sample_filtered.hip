@@ -31,14 +31,15 @@
 namespace lfs {
 namespace {
 
-constexpr int FNT = 512;             // threads: 256 registers each, room for the row and the cuts
+constexpr int FNT = 1024;            // threads
 constexpr int FNW = FNT / 64;
 constexpr int kBins = 65536;
 constexpr int kChunk = 128;          // bins of a chunk: two per lane
 constexpr int kChunks = kBins / kChunk;
 constexpr int CPL = kChunks / 64;    // chunks per lane
 constexpr int kWindow = 32768;       // 32-bit bins counted at once
-constexpr uint32_t kNever = 0xFFFFu; // a NaN, in the place of tokens past the row
+constexpr int FU = 8;                // 16-byte pieces of the row that a thread has in flight
+constexpr int kList = FNT;           // equal tokens ranked as a list, one a thread
 
 // Bin of a logit, 0 the largest value; kBins for one that is never drawn
 // (-infinity, NaN).  -0 and +0 are equal.
@@ -260,8 +261,6 @@ __device__ __forceinline__ void draw(const Weights& wt, const Filters& f, int lo
   nth = skip > 0.0 ? (skip < (double)(at.n - 1) ? (uint32_t)skip : at.n - 1) : 0u;
 }
 
-// NR: 16-byte pieces of the row that a thread holds; 0: rows of any length.
-template <int NR>
 __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     const uint16_t* __restrict__ logits, int64_t ld, const float* __restrict__ temps,
     const float* __restrict__ uniforms, const int32_t* __restrict__ top_k, const float* __restrict__ top_p,
@@ -271,38 +270,31 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   __shared__ double drawn_s;
   __shared__ uint32_t cnt[kChunks];
   __shared__ uint32_t bins[kChunk];
-  __shared__ uint32_t places[(NR > 0 ? NR : 1) * FNW];
-  __shared__ uint32_t many_n, lost, drawn_n;
+  __shared__ uint32_t places[FNW + 1];
+  __shared__ uint32_t many_n, lost, drawn_n, list_n;
+  __shared__ __attribute__((aligned(16))) uint32_t list[kList];
   __shared__ int drawn_d, reaching;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t b = blockIdx.x;
   const uint16_t* row = logits + b * ld;
-  // 16-byte pieces: piece i holds tokens 8i - skew .. + 7
-  const int skew = (int)(((uintptr_t)row >> 1) & 7), pieces = (int)(((int64_t)V + skew + 7) / 8);
-  auto piece = [&](int i) -> uint4 {
-    const int64_t t = 8ll * i - skew;
-    if (t >= 0 && t + 8 <= V) return *reinterpret_cast<const uint4*>(row + t);
-    uint32_t w[4];
+  // The row: `head` tokens up to a 16-byte boundary, `pieces` of 8, and the rest.
+  const int head = min(V, (int)(-(uintptr_t)row >> 1 & 7)), pieces = (V - head) / 8;
+  const uint4* body = reinterpret_cast<const uint4*>(row + head);
+  // of the first 16 threads: a token outside the pieces, or -1
+  const int edge = tid < 8 ? (tid < head ? tid : -1) : tid < 16 && head + 8 * pieces + tid - 8 < V ? head + 8 * pieces + tid - 8 : -1;
+  // fn(piece, its number, whether it is one) over the pieces, FU of a thread's loaded together
+  auto walk = [&](auto&& fn) {
+    for (int first = 0; first < pieces; first += FU * FNT) {
+      uint4 x[FU];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t a = t + 2 * e;
-      w[e] = (a >= 0 && a < V ? row[a] : kNever) | (a + 1 >= 0 && a + 1 < V ? row[a + 1] : kNever) << 16;
+      for (int u = 0; u < FU; ++u) x[u] = body[min(first + u * FNT + tid, pieces - 1)];
+#pragma unroll
+      for (int u = 0; u < FU; ++u)
+        if (first + u * FNT + wave * 64 < pieces) fn(x[u], first + u * FNT + tid, first + u * FNT + tid < pieces);
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
   };
-  for (int i = tid; i < kWindow / 4; i += FNT) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) many_n = lost = 0;
-  __syncthreads();  // before the row's loads, which a barrier would wait for
   // a value that many of 64 samples have (the same samples for every wave)
   const uint32_t sample = row[(int64_t)lane * V >> 6];
-  uint4 held[NR > 0 ? NR : 1];
-  if constexpr (NR > 0) {
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      held[r] = make_uint4(~0u, ~0u, ~0u, ~0u);
-      if (r * FNT + tid < pieces) held[r] = piece(r * FNT + tid);
-    }
-  }
   const float T = temps[b];
   Filters f;
   f.k = top_k != nullptr ? top_k[b] : 0;
@@ -310,6 +302,9 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   f.p = top_p != nullptr ? (double)top_p[b] : 1.0;
   f.m = min_p != nullptr ? (double)min_p[b] : 0.0;
   f.u = fmin(fmax((double)uniforms[b], 0.0), 1.0 - 0x1p-24);  // a NaN counts as 0
+  for (int i = tid; i < kWindow / 4; i += FNT) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
+  if (tid == 0) many_n = lost = list_n = 0;
+  __syncthreads();
   uint32_t many = ~0u;
 #pragma unroll 1
   for (int e = 0; e < 64; e += 3) {  // one of its samples is met
@@ -323,32 +318,28 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   // the counts: low half of word h & 0x7FFF for bits h < 0x8000, high half for the others
   auto add = [&](uint32_t h) { atomicAdd(&hist[h & 0x7FFFu], (h >> 15) * 0xFFFFu + 1u); };
   uint32_t many_here = 0;  // of the wave
-  auto count = [&](const uint4& x) {
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    if (many == ~0u) {
+  if (many == ~0u) {
+    walk([&](const uint4& x, int, bool in) {
+      if (!in) return;
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) add(w[e] & 0xFFFFu), add(w[e] >> 16);
-    } else {
+    });
+  } else {
+    walk([&](const uint4& x, int, bool in) {
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t h = (e & 1) ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu;
-        many_here += __popcll(__ballot(h == many));
-        if (h != many) add(h);
+        many_here += __popcll(__ballot(in && h == many));
+        if (in && h != many) add(h);
       }
-    }
-  };
-  int waves_pieces = 0;  // of the wave
-  if constexpr (NR > 0) {
-#pragma unroll
-    for (int r = 0; r < NR; ++r)
-      if (r * FNT + wave * 64 < pieces) count(held[r]), ++waves_pieces;
-  } else {
-    for (int i = wave * 64; i < pieces; i += FNT) {
-      uint4 x = make_uint4(~0u, ~0u, ~0u, ~0u);
-      if (i + lane < pieces) x = piece(i + lane);
-      count(x);
-      ++waves_pieces;
-    }
+    });
+  }
+  if (wave == 0) {
+    const uint32_t h = edge >= 0 ? row[edge] : 0;
+    many_here += __popcll(__ballot(edge >= 0 && h == many));
+    if (edge >= 0 && h != many) add(h);
   }
   if (lane == 0 && many_here != 0) atomicAdd(&many_n, many_here);
   __syncthreads();
@@ -381,7 +372,7 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     lo = scan_sum8(lo), hi = scan_sum8(hi);
     if ((lane & 7) == 7) cnt[kChunks / 2 - 1 - pair] = lo, cnt[kChunks / 2 + pair] = hi;
   }
-  sum = lane_u(scan_sum(sum), 63) + many_here - 512u * waves_pieces;
+  sum = lane_u(scan_sum(sum), 63) + many_here - (wave == 0 ? (uint32_t)V : 0u);
   if (lane == 0 && sum != 0) atomicAdd(&lost, sum);  // modulo 2^32: 0 over the waves where every count fits
   __syncthreads();
   const bool counted = lost == 0;
@@ -425,12 +416,20 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     wt.xmax = bin_value(wt.top);
     static_assert(kChunks <= 64 * FNW, "a lane for each of a wave's chunks");
     uint64_t some = __ballot(lane < kChunks / FNW && cnt[min(wave + FNW * lane, kChunks - 1)] != 0);
-    for (; some != 0; some &= some - 1) {
-      const int c = wave + FNW * __builtin_ctzll(some), e = c * kChunk + 2 * lane;
-      const uint32_t n0 = bin_count(e), n1 = bin_count(e + 1);
-      const double m = (n0 != 0 ? n0 * wt.at(e) : 0.0) + (n1 != 0 ? n1 * wt.at(e + 1) : 0.0);
-      const double all = lane_d(scan_sum(m), 63);
-      if (lane == 0) mass[c] = all;
+    while (some != 0) {  // two chunks at a time, for the latency of their exponentials and sums
+      const int c0 = wave + FNW * __builtin_ctzll(some);
+      some &= some - 1;
+      const int c1 = some != 0 ? wave + FNW * __builtin_ctzll(some) : c0;
+      some &= some - 1;
+      const int e0 = c0 * kChunk + 2 * lane, e1 = c1 * kChunk + 2 * lane;
+      auto weight = [&](int e) {  // bins before the first have no tokens and no finite weight
+        const uint32_t n = bin_count(e);
+        const double w = wt.at(e);
+        return n != 0 ? n * w : 0.0;
+      };
+      const double m0 = weight(e0) + weight(e0 + 1), m1 = weight(e1) + weight(e1 + 1);
+      const double all0 = lane_d(scan_sum(m0), 63), all1 = lane_d(scan_sum(m1), 63);
+      if (lane == 0) mass[c0] = all0, mass[c1] = all1;
     }
     if (wave == FNW - 1 && f.m > 0.0) {
       const int lo = last_reaching(wt, f.m);
@@ -506,85 +505,89 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   };
   // a half of a word matches where it is 0 here; +0 also meets -0
   const uint32_t same = bits_of(d) * 0x10001u, mask = d == 0x7FFF ? 0x7FFF7FFFu : ~0u;
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-  auto differ = [&](uint32_t w) -> u16x2 {  // 0 or 1 a half
-    return __builtin_elementwise_min(__builtin_bit_cast(u16x2, (w ^ same) & mask), u16x2{1, 1});
-  };
-  auto any_match = [&](const uint4& x) -> bool {
-    const u16x2 n = differ(x.x) + differ(x.y) + differ(x.z) + differ(x.w);
-    return __builtin_bit_cast(uint32_t, n) != 0x00040004u;
+  // Top bits of the halves that are 0, and perhaps of a half above one (the
+  // borrow): exact on whether there is one
+  auto zeros = [&](uint32_t w) { return (w - 0x10001u) & ~w & 0x80008000u; };
+  auto any_match = [&](const uint4& x) {
+    return (zeros((x.x ^ same) & mask) | zeros((x.y ^ same) & mask) | zeros((x.z ^ same) & mask) |
+            zeros((x.w ^ same) & mask)) != 0;
   };
   auto matches = [&](const uint4& x) -> uint32_t {  // a bit for each of the eight
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t n = __builtin_bit_cast(uint32_t, differ(w[e])) ^ 0x10001u;
-      m |= ((n & 1u) | (n >> 15)) << (2 * e);
+      const uint32_t n = (w[e] ^ same) & mask;
+      m |= ((n & 0xFFFFu) == 0 ? 1u << (2 * e) : 0u) | ((n >> 16) == 0 ? 2u << (2 * e) : 0u);
     }
     return m;
   };
-  // in the 64 pieces of a wave from piece i on, of which a lane's holds m: the
-  // token if the nth is there, else nth less those there
-  auto pick = [&](uint32_t m, int i) -> bool {
-    const uint32_t mine = __popc(m), upto = scan_sum(mine), all = lane_u(upto, 63);
-    if (nth >= all) {
-      nth -= all;
-      return false;
-    }
-    if (nth < upto && nth >= upto - mine) {
-      for (uint32_t skip = nth - (upto - mine); skip > 0; --skip) m &= m - 1;
-      done(8ll * (i + lane) - skew + __builtin_ctz(m));
-    }
-    return true;
+  auto note = [&](uint32_t token) {
+    const uint32_t at = atomicAdd(&list_n, 1u);
+    if (at < kList) list[at] = token;
   };
-  if constexpr (NR > 0) {
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      uint32_t n = 0;
-      if (__any(any_match(held[r]))) n = lane_u(scan_sum((uint32_t)__popc(matches(held[r]))), 63);
-      if (lane == 0) places[r * FNW + wave] = n;
+  walk([&](const uint4& x, int i, bool in) {
+    if (!in || !any_match(x)) return;
+    for (uint32_t m = matches(x); m != 0; m &= m - 1) note(head + 8 * i + __builtin_ctz(m));
+  });
+  auto equal_bits = [&](uint32_t h) { return ((h ^ same) & mask & 0xFFFFu) == 0; };
+  if (edge >= 0 && equal_bits(row[edge])) note(edge);
+  __syncthreads();
+  const uint32_t equal = list_n;
+  if (equal <= kList) {  // the nth smallest: a thread counts those before its own
+    if (tid >= (int)equal) return;
+    const uint32_t mine = list[tid];
+    uint32_t less = 0, i = 0;
+    for (; i + 4 <= equal; i += 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(&list[i]);
+      less += (x.x < mine) + (x.y < mine) + (x.z < mine) + (x.w < mine);
     }
-    __syncthreads();
-    uint32_t at = 0;  // tokens of the bin before the wave's r-th pieces
-    int mine = -1;
-    constexpr int PPL = (NR * FNW + 63) / 64;
-    uint32_t n[PPL], before = 0;
-#pragma unroll
-    for (int i = 0; i < PPL; ++i) {
-      n[i] = PPL * lane + i < NR * FNW ? places[PPL * lane + i] : 0;
-      before += n[i];
+    for (; i < equal; ++i) less += list[i] < mine;
+    if (less == nth) done(mine);
+    return;
+  }
+  // many equals: a wave counts those of a consecutive part of the pieces, and
+  // one looks through its part; the tokens before and after the pieces are in
+  // the first wave
+  const int per = ((pieces + FNW - 1) / FNW + 63) & ~63, i0 = min(pieces, wave * per), i1 = min(pieces, i0 + per);
+  auto in_piece = [&](int i) { return i + lane < i1 ? matches(body[i + lane]) : 0u; };
+  uint32_t here = 0;
+  for (int i = i0; i < i1; i += 64) here += __popc(in_piece(i));
+  here = lane_u(scan_sum(here), 63);
+  const uint64_t edges = wave == 0 ? __ballot(edge >= 0 && equal_bits(row[max(edge, 0)])) : 0;
+  if (lane == 0) places[wave] = here;
+  if (tid == 0) places[FNW] = __popcll(edges & 0xFF);
+  __syncthreads();
+  if (nth < places[FNW]) {  // before the pieces
+    if (wave == 0 && lane < 8 && (edges >> lane & 1) && __popcll(edges & ((1ull << lane) - 1)) == (int)nth) done(edge);
+    return;
+  }
+  nth -= places[FNW];
+  uint32_t sum_n = 0, before_n = 0;
+  for (int w = 0; w < FNW; ++w) {
+    if (w == wave) before_n = sum_n;
+    sum_n += places[w];
+  }
+  if (nth >= sum_n) {  // after them
+    nth -= sum_n;
+    if (wave == 0 && lane >= 8 && (edges >> lane & 1) &&
+        __popcll(edges & ((1ull << lane) - 1) & ~0xFFull) == (int)nth)
+      done(edge);
+    return;
+  }
+  if (nth < before_n || nth >= before_n + here) return;
+  nth -= before_n;
+  for (int i = i0; i < i1; i += 64) {
+    uint32_t m = in_piece(i);
+    const uint32_t mine = __popc(m), upto = scan_sum(mine), all = lane_u(upto, 63);
+    if (nth < all) {
+      if (nth < upto && nth >= upto - mine) {
+        for (uint32_t skip = nth - (upto - mine); skip > 0; --skip) m &= m - 1;
+        done(head + 8ll * (i + lane) + __builtin_ctz(m));
+      }
+      return;
     }
-    before = scan_sum(before) - before;
-#pragma unroll
-    for (int i = 0; i < PPL; ++i) {
-      if (nth >= before && nth < before + n[i]) mine = PPL * lane + i, at = before;
-      before += n[i];
-    }
-    const uint64_t any = __ballot(mine >= 0);
-    if (any == 0) return;  // not reached: the bin holds more than nth tokens
-    const int src = __builtin_ctzll(any), place = (int)lane_u((uint32_t)mine, src);
-    if (place % FNW != wave) return;
-    nth -= lane_u(at, src);
-#pragma unroll
-    for (int r = 0; r < NR; ++r)
-      if (r == place / FNW) pick(matches(held[r]), r * FNT + wave * 64);
-  } else {
-    const int per = ((pieces + FNW - 1) / FNW + 63) & ~63;  // pieces of a wave
-    const int i0 = min(pieces, wave * per), i1 = min(pieces, i0 + per);
-    auto at = [&](int i) { return i + lane < i1 ? matches(piece(i + lane)) : 0u; };
-    uint32_t here = 0;
-    for (int i = i0; i < i1; i += 64) here += __popc(at(i));
-    here = lane_u(scan_sum(here), 63);
-    if (lane == 0) places[wave] = here;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-      if (nth < places[w]) return;
-      nth -= places[w];
-    }
-    if (nth >= here) return;
-    for (int i = i0; i < i1; i += 64)
-      if (pick(at(i), i)) return;
+    nth -= all;
   }
 }
 
@@ -602,14 +605,7 @@ extern "C" int lfs_sample_filtered(const void* logits, int64_t ld, const float* 
   LFS_REQUIRE(logits && temperatures && uniforms && out, "sample_filtered: null pointer");
   LFS_REQUIRE(B < (1ll << 22), "sample_filtered: too many rows");
   LFS_REQUIRE(vocab <= (1 << 30), "sample_filtered: vocabulary too large");
-#define LFS_SF(NR)                                                                                                  \
-  hipLaunchKernelGGL(sample_filtered_kernel<NR>, dim3((unsigned)B), dim3(FNT), 0, (hipStream_t)stream,               \
-                     (const uint16_t*)logits, ld, temperatures, uniforms, top_k, top_p, min_p, vocab, out, logprob)
-  const int64_t pieces = ((int64_t)vocab + 7 + 7) / 8;  // at any alignment
-  if (pieces <= 10 * FNT) LFS_SF(10);
-  else if (pieces <= 20 * FNT) LFS_SF(20);
-  else if (pieces <= 40 * FNT) LFS_SF(40);
-  else LFS_SF(0);
-#undef LFS_SF
+  hipLaunchKernelGGL(sample_filtered_kernel, dim3((unsigned)B), dim3(FNT), 0, (hipStream_t)stream,
+                     (const uint16_t*)logits, ld, temperatures, uniforms, top_k, top_p, min_p, vocab, out, logprob);
   return check_launch("sample_filtered");
 }
