@@ -35,6 +35,7 @@ stream; outputs are allocated here, as the reference wrappers do
 """
 from __future__ import annotations
 
+import functools
 import math
 import numbers
 from array import array
@@ -57,6 +58,9 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 # handle alone 0.1 us; four tensors' device objects compared 1.1 us, their
 # indices 0.3 us; shapes as tuples built from slices 0.5 us each.
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -85,7 +89,7 @@ def _launch(what: str, fn, on: torch.Tensor, *args) -> None:
     """fn(*args, stream) on the device and current stream of ``on``, also
     where that is not the current device."""
     dev = on.get_device()
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         rc = fn(*args, _stream(on))
     else:
         with torch.cuda.device(dev):
@@ -505,6 +509,13 @@ def paged_decode_window_workspace_bytes(batch: int, num_q_heads: int, head_dim: 
     return int(_lib.load().lfs_paged_decode_window_workspace_bytes(batch, num_q_heads, head_dim))
 
 
+@functools.lru_cache(maxsize=256)
+def _window_workspace(device: int, batch: int, num_q_heads: int, head_dim: int) -> int:
+    """paged_decode_window_workspace_bytes on a device (by its number of CUs)."""
+    with torch.cuda.device(device):
+        return paged_decode_window_workspace_bytes(batch, num_q_heads, head_dim)
+
+
 MAX_WINDOW = 1 << 30  # a longer window, or more sinks, hide nothing of any context
 
 
@@ -555,10 +566,12 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     assert block_tables.dim() == 2 and block_tables.stride(1) == 1, "block_tables must be [B, max_blocks]"
     assert context_lens.is_contiguous() and context_lens.numel() == q.size(0)
     _on_gpu(q, k_cache, v_cache, context_lens, block_tables)
-    for t, n in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
-        _dtype(t, torch.bfloat16, n)
-    _dtype(context_lens, torch.int64, "context_lens")
-    _dtype(block_tables, torch.int32, "block_tables")
+    if not (q.dtype is k_cache.dtype is v_cache.dtype is torch.bfloat16 and context_lens.dtype is torch.int64
+            and block_tables.dtype is torch.int32):
+        for t, n in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache")):
+            _dtype(t, torch.bfloat16, n)
+        _dtype(context_lens, torch.int64, "context_lens")
+        _dtype(block_tables, torch.int32, "block_tables")
     B, Hq, D = q.shape
     NB, BS, Hkv, Dk = k_cache.shape
     assert Dk == D, "head_dim mismatch between q and the caches"
@@ -568,18 +581,22 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         scale = 1.0 / math.sqrt(D)
     if windowed:
         assert blocks_per_split is None, "blocks_per_split does not go with a window"
-        need = paged_decode_window_workspace_bytes(B, Hq, D)
-        if workspace is None:
-            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+        need = _window_workspace(q.get_device(), B, Hq, D)
+        if workspace is not None:
+            _on_gpu(q, workspace)
+            assert workspace.is_contiguous(), "workspace must be contiguous"
+        elif need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         o = torch.empty_like(q)
         oq = os_ = None
         if quant:
             oq = torch.empty(B, Hq * D, dtype=FP8, device=q.device)
             os_ = torch.empty(B, Hq * D // 128, dtype=torch.float32, device=q.device)
         _launch("paged_attention_decode", _lib.load().lfs_paged_decode_window, q,
-                _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(context_lens), _ptr(block_tables), block_tables.stride(0),
-                _ptr(o), _ptr(workspace), workspace.numel() * workspace.element_size(), B, Hq, Hkv, D, BS, NB, max_blocks,
-                min(window, MAX_WINDOW), min(sinks, MAX_WINDOW), float(scale), _ptr(oq), _ptr(os_))
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(),
+                block_tables.stride(0), o.data_ptr(), _ptr(workspace),
+                0 if workspace is None else workspace.nbytes, B, Hq, Hkv, D, BS, NB, max_blocks,
+                min(window, MAX_WINDOW), min(sinks, MAX_WINDOW), scale, _ptr(oq), _ptr(os_))
         return (o, oq, os_) if quant else o
     if blocks_per_split is None:
         bps = default_blocks_per_split(B, Hkv, max_blocks, BS, quant_values=(Hq // Hkv) * D if quant else 0)
@@ -763,7 +780,7 @@ def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _, Hq, D = q.shape
     if block_table is not None:
         assert k.dim() == 4, "with block_table, k and v are the paged caches [NB, BS, Hkv, D]"
-        _on_gpu(block_table)
+        _on_gpu(q, block_table)
         _dtype(block_table, torch.int32, "block_table")
         assert block_table.dim() == 2 and block_table.stride(1) == 1 and block_table.size(0) == B
         NB, BS, Hkv, Dk = k.shape
@@ -876,27 +893,31 @@ def sample_filtered(logits: torch.Tensor, temperatures: torch.Tensor, uniforms: 
     Returns int64 [B], with ``return_logprob`` also the fp32 [B] logarithms of
     the drawn tokens' shares of the kept weight."""
     assert logits.dim() == 2 and logits.stride(1) == 1, "logits must be [B, V] with unit column stride"
-    _on_gpu(logits, temperatures, uniforms)
+    _on_gpu(logits)
     _dtype(logits, torch.bfloat16, "logits")
     B, V = logits.shape
     if logits.stride(0) < V:  # broadcast rows (an expanded view): give each row its own copy
         logits = logits.contiguous()
-    rows = [temperatures, uniforms, top_k, top_p, min_p]
-    for i, (t, dt, n) in enumerate(zip(rows, _SAMPLE_TYPES, ("temperatures", "uniforms", "top_k", "top_p", "min_p"))):
-        if t is not None:
-            if t.get_device() != logits.get_device():
-                _on_gpu(logits, t)
-            _dtype(t, dt, n)
-            assert t.shape == (B,), f"{n} must be [B]"
+    dev, rows = logits.get_device(), [temperatures, uniforms, top_k, top_p, min_p]
+    for i, t in enumerate(rows):
+        if t is None:
+            continue
+        if t.get_device() != dev:
+            _on_gpu(logits, t)
+        if t.dtype is not _SAMPLE_TYPES[i]:
+            _dtype(t, _SAMPLE_TYPES[i], _SAMPLE_NAMES[i])
+        assert t.shape == (B,), f"{_SAMPLE_NAMES[i]} must be [B]"
+        if not t.is_contiguous():
             rows[i] = t.contiguous()
     out = torch.empty(B, dtype=torch.int64, device=logits.device)
     logprob = torch.empty(B, dtype=torch.float32, device=logits.device) if return_logprob else None
     _launch("sample_filtered", _lib.load().lfs_sample_filtered, logits,
-            _ptr(logits), logits.stride(0), *map(_ptr, rows), B, V, _ptr(out), _ptr(logprob))
+            logits.data_ptr(), logits.stride(0) if B > 1 else V, *map(_ptr, rows), B, V, out.data_ptr(), _ptr(logprob))
     return (out, logprob) if return_logprob else out
 
 
 _SAMPLE_TYPES = (torch.float32, torch.float32, torch.int32, torch.float32, torch.float32)
+_SAMPLE_NAMES = ("temperatures", "uniforms", "top_k", "top_p", "min_p")
 
 
 # ------------------------------------------------- fused decode-step rows --
@@ -1066,32 +1087,36 @@ def qk_head_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight:
     D = width // heads
     assert width == heads * D, "qkv width mismatch"
     _on_gpu(qkv, q_weight, k_weight, cos_sin, positions)
-    _dtype(qkv, torch.bfloat16, "qkv")
-    for t, n in ((q_weight, "q_weight"), (k_weight, "k_weight"), (cos_sin, "cos_sin")):
-        _dtype(t, torch.float32, n)
-        assert t.is_contiguous(), f"{n} must be contiguous"
-    assert q_weight.shape == (D,) and k_weight.shape == (D,), "q_weight and k_weight must be [D]"
-    assert cos_sin.dim() == 2, "cos_sin must be [max_pos, R]"
-    _dtype(positions, torch.int64, "positions")
+    if not (qkv.dtype is torch.bfloat16 and q_weight.dtype is k_weight.dtype is cos_sin.dtype is torch.float32
+            and positions.dtype is torch.int64):
+        _dtype(qkv, torch.bfloat16, "qkv")
+        for t, n in ((q_weight, "q_weight"), (k_weight, "k_weight"), (cos_sin, "cos_sin")):
+            _dtype(t, torch.float32, n)
+        _dtype(positions, torch.int64, "positions")
+    assert q_weight.is_contiguous() and k_weight.is_contiguous(), "q_weight and k_weight must be contiguous"
+    assert q_weight.shape == k_weight.shape == (D,), "q_weight and k_weight must be [D]"
+    assert cos_sin.dim() == 2 and cos_sin.is_contiguous(), "cos_sin must be contiguous [max_pos, R]"
     assert positions.numel() == T and positions.is_contiguous(), "positions must be [T]"
     num_slots = 0
     if slot_mapping is not None:
         _on_gpu(qkv, k_cache, v_cache, slot_mapping)
-        _dtype(slot_mapping, torch.int64, "slot_mapping")
-        for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-            _dtype(t, torch.bfloat16, n)
-            assert t.is_contiguous() and t.dim() == 4 and t.shape[2:] == (num_kv_heads, D), \
-                f"{n} must be [NB, BS, Hkv, D]"
-        assert v_cache.shape == k_cache.shape
+        if not (k_cache.dtype is v_cache.dtype is torch.bfloat16 and slot_mapping.dtype is torch.int64):
+            _dtype(slot_mapping, torch.int64, "slot_mapping")
+            _dtype(k_cache, torch.bfloat16, "k_cache")
+            _dtype(v_cache, torch.bfloat16, "v_cache")
+        shape = k_cache.shape
+        assert len(shape) == 4 and shape[2:] == (num_kv_heads, D) and v_cache.shape == shape, \
+            "k_cache and v_cache must be [NB, BS, Hkv, D]"
+        assert k_cache.is_contiguous() and v_cache.is_contiguous(), "k_cache and v_cache must be contiguous"
         assert slot_mapping.numel() == T and slot_mapping.is_contiguous()
-        num_slots = k_cache.shape[0] * k_cache.shape[1]
+        num_slots = shape[0] * shape[1]
     q = torch.empty(T, num_q_heads, D, dtype=torch.bfloat16, device=qkv.device)
     k = torch.empty(T, num_kv_heads, D, dtype=torch.bfloat16, device=qkv.device) if return_kv else None
     v = torch.empty_like(k) if return_kv else None
     _launch("qk_head_norm_rope_store", _lib.load().lfs_qk_head_norm_rope_store, qkv,
-            _ptr(qkv), qkv.stride(0) if T > 1 else width, _ptr(q_weight), _ptr(k_weight), _ptr(cos_sin), cos_sin.size(1),
-            _ptr(positions), _ptr(slot_mapping), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k), _ptr(v), T, num_q_heads,
-            num_kv_heads, D, num_slots, cos_sin.size(0), float(eps))
+            qkv.data_ptr(), qkv.stride(0) if T > 1 else width, q_weight.data_ptr(), k_weight.data_ptr(),
+            cos_sin.data_ptr(), cos_sin.size(1), positions.data_ptr(), _ptr(slot_mapping), q.data_ptr(), _ptr(k_cache),
+            _ptr(v_cache), _ptr(k), _ptr(v), T, num_q_heads, num_kv_heads, D, num_slots, cos_sin.size(0), eps)
     return (q, k, v) if return_kv else q
 
 

@@ -115,6 +115,15 @@ def test_strides_and_broadcast_rows():
         run(view, rng.uniform(0.5, 1, view.shape[0]), rng.random(view.shape[0], np.float32), p=0.95)
 
 
+def test_settings_of_any_stride():
+    x, B = logits_of(6, 900, 2.0, 9), 6
+    g = torch.Generator(device=DEV).manual_seed(2)
+    u = torch.rand(2 * B, generator=g, device=DEV)[::2]
+    t, p = torch.full((1,), 0.7, device=DEV).expand(B), torch.full((1,), 0.9, device=DEV).expand(B)
+    assert torch.equal(K.sample_filtered(x, t, u, top_p=p),
+                       K.sample_filtered(x, t.contiguous(), u.contiguous(), top_p=p.contiguous()))
+
+
 def test_frequencies():
     logits = torch.tensor([[0.0, 1.0, 2.0, -1.0, 0.5]], device=DEV).to(torch.bfloat16)
     n = 40000
