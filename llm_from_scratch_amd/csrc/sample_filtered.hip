@@ -16,16 +16,22 @@
 // Weights and their sums are held in 64 bits: with 32 the borders of tokens
 // in the tail of a wide vocabulary move by more than the tokens weigh.
 //
-// One workgroup per row, which it reads once, into registers (longer rows are
-// read again).  Counts of all 65536 bit patterns stand in 128 KiB of LDS, two
-// 16-bit ones a word, under the tokens' own bits: a token costs a few
+// One workgroup per row.  Counts of all 65536 bit patterns stand in 128 KiB of
+// LDS, two 16-bit ones a word, under the tokens' own bits: a token costs a few
 // instructions and one LDS addition.  A count past 65535 carries or is lost,
 // so that the counts no longer add up to the tokens; such a row is counted
 // again in 32-bit bins, a window of them at a time.  A value that holds many
 // of the row (a mask's, say) is counted by ballots and not in LDS, where its
 // additions would queue up: one that 8 of 64 samples have.  One wave then
 // walks the counts (512 chunks of 128 bins, a chunk an exponent and a sign)
-// for the cuts, and the workgroup looks up the token among equals.
+// for the cuts; meanwhile the others read the row again, from the caches,
+// into registers, and find the token among equals there.
+//
+// Measured: 256 rows of 150001 with all filters 40 us, one row of 32000
+// 15 us.  The bound is not memory (the logits of the 256 take 16 us): it is
+// the LDS additions (9 us of 30 in a long row), the second read (6) and the
+// chain of the cuts, 4 us of one wave's dependent steps.  The cuts as a loop
+// over one search took a row of 32000 to 16.7 us.
 #include "common.h"
 
 namespace lfs {
@@ -39,6 +45,8 @@ constexpr int kChunks = kBins / kChunk;
 constexpr int CPL = kChunks / 64;    // chunks per lane
 constexpr int kWindow = 32768;       // 32-bit bins counted at once
 constexpr int FU = 8;                // 16-byte pieces of the row that a thread has in flight
+constexpr int FH = 20;               // and that a thread of all waves but one holds
+constexpr int FNH = FNT - 64;
 constexpr int kList = FNT;           // equal tokens ranked as a list, one a thread
 
 // Bin of a logit, 0 the largest value; kBins for one that is never drawn
@@ -271,7 +279,7 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   __shared__ uint32_t cnt[kChunks];
   __shared__ uint32_t bins[kChunk];
   __shared__ uint32_t places[FNW + 1];
-  __shared__ uint32_t many_n, lost, drawn_n, list_n;
+  __shared__ uint32_t many_value, many_n, lost, drawn_n, list_n;
   __shared__ __attribute__((aligned(16))) uint32_t list[kList];
   __shared__ int drawn_d, reaching;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -282,9 +290,9 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   const uint4* body = reinterpret_cast<const uint4*>(row + head);
   // of the first 16 threads: a token outside the pieces, or -1
   const int edge = tid < 8 ? (tid < head ? tid : -1) : tid < 16 && head + 8 * pieces + tid - 8 < V ? head + 8 * pieces + tid - 8 : -1;
-  // fn(piece, its number, whether it is one) over the pieces, FU of a thread's loaded together
-  auto walk = [&](auto&& fn) {
-    for (int first = 0; first < pieces; first += FU * FNT) {
+  // fn(piece, its number, whether it is one) over the pieces past `from`, FU of a thread's loaded together
+  auto walk = [&](int from, auto&& fn) {
+    for (int first = from; first < pieces; first += FU * FNT) {
       uint4 x[FU];
 #pragma unroll
       for (int u = 0; u < FU; ++u) x[u] = body[min(first + u * FNT + tid, pieces - 1)];
@@ -293,8 +301,6 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
         if (first + u * FNT + wave * 64 < pieces) fn(x[u], first + u * FNT + tid, first + u * FNT + tid < pieces);
     }
   };
-  // a value that many of 64 samples have (the same samples for every wave)
-  const uint32_t sample = row[(int64_t)lane * V >> 6];
   const float T = temps[b];
   Filters f;
   f.k = top_k != nullptr ? top_k[b] : 0;
@@ -304,29 +310,33 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   f.u = fmin(fmax((double)uniforms[b], 0.0), 1.0 - 0x1p-24);  // a NaN counts as 0
   for (int i = tid; i < kWindow / 4; i += FNT) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
   if (tid == 0) many_n = lost = list_n = 0;
-  __syncthreads();
-  uint32_t many = ~0u;
-#pragma unroll 1
-  for (int e = 0; e < 64; e += 3) {  // one of its samples is met
-    const uint32_t v = lane_u(sample, e);
-    if (__popcll(__ballot(sample == v)) >= 8) {
-      many = v;
-      break;
+  if (wave == FNW - 1) {  // a value that 8 of 64 samples have
+    const uint32_t v = row[(int64_t)lane * V >> 6];
+    uint64_t alike = ~0ull;  // lanes with the same bits
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint64_t ones = __ballot(v >> e & 1);
+      alike &= (v >> e & 1) ? ones : ~ones;
     }
+    const uint64_t often = __ballot(__popcll(alike) >= 8);
+    if (lane == 0) many_value = often != 0 ? 0u : ~0u;
+    if (often != 0 && lane == __builtin_ctzll(often)) many_value = v;
   }
+  __syncthreads();
+  const uint32_t many = many_value;
 
   // the counts: low half of word h & 0x7FFF for bits h < 0x8000, high half for the others
   auto add = [&](uint32_t h) { atomicAdd(&hist[h & 0x7FFFu], (h >> 15) * 0xFFFFu + 1u); };
   uint32_t many_here = 0;  // of the wave
   if (many == ~0u) {
-    walk([&](const uint4& x, int, bool in) {
+    walk(0, [&](const uint4& x, int, bool in) {
       if (!in) return;
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) add(w[e] & 0xFFFFu), add(w[e] >> 16);
     });
   } else {
-    walk([&](const uint4& x, int, bool in) {
+    walk(0, [&](const uint4& x, int, bool in) {
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -403,6 +413,7 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   int d = 0;
   uint32_t nth = 0;
   double S = 0.0;
+  uint4 held[FH];
   if (counted) {
     const int c0 = first_chunk();
     if (c0 < 0) {  // nothing can be drawn
@@ -414,12 +425,15 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     }
     wt.top = first_bin(c0, bin_count(c0 * kChunk + 2 * lane), bin_count(c0 * kChunk + 2 * lane + 1));
     wt.xmax = bin_value(wt.top);
-    static_assert(kChunks <= 64 * FNW, "a lane for each of a wave's chunks");
-    uint64_t some = __ballot(lane < kChunks / FNW && cnt[min(wave + FNW * lane, kChunks - 1)] != 0);
+    // the last wave looks for min-p's last bin meanwhile
+    const int waves = f.m > 0.0 ? FNW - 1 : FNW;
+    static_assert(kChunks <= 64 * (FNW - 1), "a lane for each of a wave's chunks");
+    const int mine = wave + waves * lane;
+    uint64_t some = __ballot(wave < waves && mine < kChunks && cnt[min(mine, kChunks - 1)] != 0);
     while (some != 0) {  // two chunks at a time, for the latency of their exponentials and sums
-      const int c0 = wave + FNW * __builtin_ctzll(some);
+      const int c0 = wave + waves * __builtin_ctzll(some);
       some &= some - 1;
-      const int c1 = some != 0 ? wave + FNW * __builtin_ctzll(some) : c0;
+      const int c1 = some != 0 ? wave + waves * __builtin_ctzll(some) : c0;
       some &= some - 1;
       const int e0 = c0 * kChunk + 2 * lane, e1 = c1 * kChunk + 2 * lane;
       auto weight = [&](int e) {  // bins before the first have no tokens and no finite weight
@@ -431,12 +445,16 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
       const double all0 = lane_d(scan_sum(m0), 63), all1 = lane_d(scan_sum(m1), 63);
       if (lane == 0) mass[c0] = all0, mass[c1] = all1;
     }
-    if (wave == FNW - 1 && f.m > 0.0) {
+    if (wave >= waves) {
       const int lo = last_reaching(wt, f.m);
       if (lane == 0) reaching = lo;
     }
     __syncthreads();
-    if (wave == 0) {
+    if (wave > 0) {  // the row again, for the search after the draw
+#pragma unroll
+      for (int r = 0; r < FH; ++r)
+        if (r * FNH + wave * 64 - 64 < pieces) held[r] = body[min(r * FNH + tid - 64, pieces - 1)];
+    } else {
       draw(wt, f, reaching, cnt, mass, [&](int chunk, uint32_t (&n)[2]) {
         n[0] = bin_count(chunk * kChunk + 2 * lane), n[1] = bin_count(chunk * kChunk + 2 * lane + 1);
       }, d, nth, S);
@@ -526,10 +544,16 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     const uint32_t at = atomicAdd(&list_n, 1u);
     if (at < kList) list[at] = token;
   };
-  walk([&](const uint4& x, int i, bool in) {
+  auto search = [&](const uint4& x, int i, bool in) {
     if (!in || !any_match(x)) return;
     for (uint32_t m = matches(x); m != 0; m &= m - 1) note(head + 8 * i + __builtin_ctz(m));
-  });
+  };
+  if (counted && wave > 0) {
+#pragma unroll
+    for (int r = 0; r < FH; ++r)
+      if (r * FNH + wave * 64 - 64 < pieces) search(held[r], r * FNH + tid - 64, r * FNH + tid - 64 < pieces);
+  }
+  walk(counted ? FH * FNH : 0, search);
   auto equal_bits = [&](uint32_t h) { return ((h ^ same) & mask & 0xFFFFu) == 0; };
   if (edge >= 0 && equal_bits(row[edge])) note(edge);
   __syncthreads();
