@@ -9,8 +9,8 @@
 // Bound: HBM, each byte read and written once.  A workgroup copies 4 KiB, one
 // nontemporal 16-byte load and store a thread, pieces of a block in order,
 // then pairs, then planes: 257 blocks of 128 KiB in 24 planes (1.6 GB both
-// ways) take 259 us, 6.2 TB/s; without the nontemporal hint 275 us, with 2, 4
-// and 8 chunks a thread 266, 271 and 350 us.  4 blocks (25 MB): 5 us.
+// ways) take 259 us, 6.2 TB/s.  Without the nontemporal hint 275 us, and then with
+// 2, 4 and 8 chunks a thread 299, 306 and 413 us.  4 blocks (25 MB): 6 us.
 #include "common.h"
 
 #include <algorithm>

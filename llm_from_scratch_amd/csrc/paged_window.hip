@@ -17,7 +17,7 @@
 // (decode_wave.h, the same walk with one wave per kv head, an equal share of
 // all visible tiles per workgroup).
 // Bound: HBM, the visible keys and values read once.  256 sequences past a
-// window of 4096 (32 / 8 heads of 128, 4.1 GB) take 670 us, 6.1 TB/s; 64 past one
+// window of 4096 (32 / 8 heads of 128, 4.1 GB) take 630 us, 6.5 TB/s; 64 past one
 // of 1024 (16 / 4 of 64, 67 MB) 20 us: 6 us for the launch, the table, the
 // first tile and the merge in LDS, then 4.8 TB/s.
 #include "common.h"

@@ -28,10 +28,12 @@
 // into registers, and find the token among equals there.
 //
 // Measured: 256 rows of 150001 with all filters 40 us, one row of 32000
-// 15 us.  The bound is not memory (the logits of the 256 take 16 us): it is
-// the LDS additions (9 us of 30 in a long row), the second read (6) and the
-// chain of the cuts, 4 us of one wave's dependent steps.  The cuts as a loop
-// over one search took a row of 32000 to 16.7 us.
+// 15 us.  The bound is not memory (the logits of the 256 take 16 us): of a
+// long row's 69000 cycles the counting, with one LDS addition a token, takes
+// 25000, the cuts, a chain of one wave's dependent steps, 9000 to 11000, and
+// the second read and its search 13000; a row of 32000 has 6000, 7000 to
+// 10000 and 4000 of 34000.  The cuts as a loop over one search took such a row
+// to 16.7 us: fewer instructions, but more steps in the chain.
 #include "common.h"
 
 namespace lfs {
