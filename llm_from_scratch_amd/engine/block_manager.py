@@ -13,7 +13,9 @@ Behavioural fixes (the reference's bugs are not copied):
   * a prompt's last block is never taken from the prefix cache (:85-114
     would cache every block of a block-aligned prompt that matches another
     sequence's, leaving the prefill no query token to sample from): it is
-    recomputed into a fresh block, so num_cached_tokens < num_tokens.
+    recomputed into a fresh block, so num_cached_tokens < num_tokens;
+  * a cached block must have the whole prefix's hash, not only the tokens: one
+    that was freed and then took the same tokens behind another prefix is no hit.
 
 Beyond the reference: blocks behind a sliding window go back to the pool while
 their sequence runs (``release_behind``), a running sequence's blocks are shared
@@ -92,7 +94,7 @@ class BlockManager:
             token_ids = seq.block(i)
             h = self.compute_hash(token_ids, h) if len(token_ids) == self.block_size else -1
             block_id = self.hash_to_block_id.get(h, -1)
-            if block_id == -1 or self.blocks[block_id].token_ids != token_ids:
+            if block_id == -1 or self.blocks[block_id].hash != h or self.blocks[block_id].token_ids != token_ids:
                 cache_miss = True
             if i == seq.num_blocks - 1:
                 cache_miss = True  # the last prompt token is always computed
