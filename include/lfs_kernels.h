@@ -399,7 +399,7 @@ int lfs_prefill_attention_window(const void* q, const void* k, const void* v, co
  * window or t < sinks.  Hidden tokens are never read: the table entries of
  * blocks that hold only such tokens may be -1.  workspace: at least
  * lfs_paged_decode_window_workspace_bytes(...) bytes, sized on the device that
- * runs the call.  q_out / q_scale as for lfs_paged_decode.  window >= 1,
+ * runs the call, 16-byte aligned.  q_out / q_scale as for lfs_paged_decode.  window >= 1,
  * sinks >= 0.  The grid depends only on the shapes and the window.
  */
 int64_t lfs_paged_decode_window_workspace_bytes(int64_t B, int32_t num_q_heads, int32_t head_dim);

@@ -184,6 +184,7 @@ extern "C" int lfs_paged_decode_window(const void* q, const void* k_cache, const
   LFS_REQUIRE(max_blocks == 0 || block_tables, "paged_decode_window: null block table");
   LFS_REQUIRE(((((uintptr_t)q) | ((uintptr_t)k_cache) | ((uintptr_t)v_cache) | ((uintptr_t)out)) & 15u) == 0,
               "paged_decode_window: q, caches and out must be 16-byte aligned");
+  LFS_REQUIRE(((uintptr_t)workspace & 15u) == 0, "paged_decode_window: the workspace must be 16-byte aligned");
   LFS_REQUIRE((q_out == nullptr) == (q_scale == nullptr), "paged_decode_window: q_out and q_scale go together");
   LFS_REQUIRE(q_out == nullptr || Hq * D % 128 == 0, "paged_decode_window: the quantised output needs Hq*D %% 128 == 0");
   const int64_t units = B * Hkv, cus = decode_cu_count();

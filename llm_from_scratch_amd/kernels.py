@@ -1099,6 +1099,7 @@ def qk_head_norm_rope_store(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight:
     assert positions.numel() == T and positions.is_contiguous(), "positions must be [T]"
     num_slots = 0
     if slot_mapping is not None:
+        assert k_cache is not None and v_cache is not None, "slot_mapping needs k_cache and v_cache"
         _on_gpu(qkv, k_cache, v_cache, slot_mapping)
         if not (k_cache.dtype is v_cache.dtype is torch.bfloat16 and slot_mapping.dtype is torch.int64):
             _dtype(slot_mapping, torch.int64, "slot_mapping")

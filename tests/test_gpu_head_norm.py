@@ -65,6 +65,13 @@ def test_values_and_slots(Hq, Hkv, D, R, T):
     assert torch.equal(q3, q) and torch.equal(k3, k) and torch.equal(v3, v)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,R,T", [(12, 4, 64, 64, 2048), (32, 8, 128, 64, 2053), (15, 3, 64, 32, 3001),
+                                          (1, 1, 128, 128, 2500), (5, 2, 64, 16, 20001)])
+def test_many_tokens(Hq, Hkv, D, R, T):
+    """A wave per token, also more tokens than the grid has waves."""
+    test_values_and_slots(Hq, Hkv, D, R, T)
+
+
 def test_extremes():
     """Zero heads stay 0 (eps), large ones keep their direction, positions
     outside the table read its ends, no token is no launch."""
@@ -114,6 +121,7 @@ def test_refusals():
                         (dict(cos_sin=a["cos_sin"][:0]), ValueError),
                         (dict(qkv=a["qkv"].float()), TypeError),
                         (dict(num_q_heads=5), AssertionError),
+                        (dict(slot_mapping=a["positions"]), AssertionError),
                         (dict(positions=a["positions"][:3]), AssertionError),
                         (dict(positions=a["positions"].int()), TypeError),
                         (dict(qkv=a["qkv"].cpu()), ValueError),

@@ -180,6 +180,47 @@ def test_decode_batches(B, Hq, Hkv, D, window, sinks):
     assert torch.equal(oq.view(torch.uint8), wq.view(torch.uint8)) and torch.equal(os_, ws)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,D,BS,window,sinks", [(45, 12, 4, 64, 16, 810, 4), (47, 32, 8, 128, 16, 790, 33),
+                                                       (70, 8, 8, 64, 16, 520, 0), (33, 8, 4, 64, 64, 4100, 70),
+                                                       (300, 8, 1, 128, 32, 1601, 1)])
+def test_decode_long_windows_of_many_sequences(B, Hq, Hkv, D, BS, window, sinks):
+    """An equal share of all visible tiles per workgroup: contexts of none, one,
+    a window's length and far past it; also captured, with other lengths and
+    tables at each replay, and with the quantised output."""
+    rng = np.random.default_rng(B)
+    NB, width = 300, 2 * window // BS + 3
+    kc, vc, q = bf16(rng, NB, BS, Hkv, D), bf16(rng, NB, BS, Hkv, D), bf16(rng, B, Hq, D)
+    fk, fv = f64(kc), f64(vc)
+
+    def contexts():
+        lens = rng.integers(0, width * BS + 1, B)
+        lens[:6] = 0, 1, window, window + 1, window + sinks, width * BS
+        return torch.from_numpy(lens).to(DEV), torch.from_numpy(rng.integers(0, NB, (B, width)).astype(np.int32)).to(DEV)
+
+    cl, bt = contexts()
+    call = lambda: K.paged_attention_decode(q, kc, vc, cl, bt, 0.1, quant=True, window=window, sinks=sinks)
+    o, oq, os_ = call()
+    wq, ws = K.act_quant(o.view(B, -1))
+    assert torch.equal(oq.view(torch.uint8), wq.view(torch.uint8)) and torch.equal(os_, ws)
+    for b in list(range(8)) + list(range(8, B, 1 + B // 8)) + [B - 1]:
+        n, table = int(cl[b]), bt[b].cpu().numpy()
+        keep = np.flatnonzero(P.window_mask([n - 1], n, window, sinks)[0]) if n else np.zeros(0, int)
+        slots = table[keep // BS], keep % BS
+        want = P.window_attention(f64(q[b:b + 1]), fk[slots], fv[slots], [10 ** 9], 0.1, 2 * 10 ** 9, 0)
+        close(o[b:b + 1], want if n else (np.zeros(1), np.zeros(1)), f"row {b}, context {n}")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    for step in range(4):
+        g.replay()
+        got = [x.clone() for x in out]
+        torch.cuda.synchronize()
+        for x, y in zip(got, call()):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), step
+        for old, new in zip((cl, bt), contexts()):
+            old.copy_(new)
+
+
 def test_decode_more_sequences_than_a_split_holds():
     rng = np.random.default_rng(5)
     B, window = 8200, 20

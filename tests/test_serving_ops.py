@@ -93,6 +93,7 @@ def test_window_refusals(lib):
     refused(lib, decode(NB=0), b"empty KV pool")
     refused(lib, decode(q=None), b"null pointer")
     refused(lib, decode(qo=16), b"go together")
+    refused(lib, decode(ws=8), b"workspace must be 16-byte aligned")
     assert decode(B=0) == 0
     assert lib.lfs_paged_decode_window_workspace_bytes(-1, 8, 64) == -1
 
