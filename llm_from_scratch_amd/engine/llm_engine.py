@@ -20,9 +20,23 @@ from .scheduler import Scheduler
 from .sequence import SamplingParams, Sequence
 
 
+def check_window(model: torch.nn.Module, window: Optional[int], sinks: int) -> None:
+    """The engine frees the blocks behind ``window`` but the first ``sinks``
+    tokens': none of the model's attention layers may still see them."""
+    if window is None:
+        return
+    for name, m in model.named_modules():
+        if hasattr(m, "k_cache") and hasattr(m, "window"):
+            if m.window is None or m.window > window or m.sinks > sinks:
+                raise ValueError(f"{name} sees a window of {m.window} and {m.sinks} first tokens, but the engine keeps "
+                                 f"{window} and {sinks}")
+
+
 class LLMEngine:
     def __init__(self, model: torch.nn.Module, config: dict, tokenizer=None, device="cuda",
                  generator: Optional[torch.Generator] = None, verbose: bool = False):
+        window, sinks = config.get("sliding_window"), config.get("num_sink_tokens", 0)
+        check_window(model, window, sinks)
         self.model_runner = ModelRunner(model, config, device)
         block_size = config.get("block_size", 256)
         Sequence.block_size = block_size
@@ -33,8 +47,8 @@ class LLMEngine:
                                   self.model_runner.num_available_kv_blocks),
             block_size=block_size,
             eos=config.get("eos", 50256),
-            sliding_window=config.get("sliding_window"),
-            num_sink_tokens=config.get("num_sink_tokens", 0))
+            sliding_window=window,
+            num_sink_tokens=sinks)
         self.tokenizer = tokenizer
         self.generator = generator
         self.verbose = verbose

@@ -81,13 +81,14 @@ class Sampler:
     makes runs repeatable); the offset advances every call.
 
     With any of ``top_k`` (int32 [B]), ``top_p`` and ``min_p`` (fp32 [B]) the
-    tokens come from kernels.sample_filtered instead, on uniform numbers of a
-    generator with the same seed."""
+    tokens come from kernels.sample_filtered instead, on uniform numbers of
+    torch's generator with the same seed and an offset that advances alike."""
 
     def __init__(self):
         self._seed: Optional[int] = None
         self._offset = 0
-        self._uniforms: dict = {}  # (device, seed): generator
+        self._uniforms: Optional[torch.Generator] = None
+        self._uniform_offset = 0
 
     def __call__(self, logits: torch.Tensor, temperatures: torch.Tensor,
                  generator: Optional[torch.Generator] = None, top_k: Optional[torch.Tensor] = None,
@@ -99,10 +100,13 @@ class Sampler:
                 self._seed = int(torch.randint(0, 2 ** 62, (1,)).item())
             seed = self._seed
         if top_k is not None or top_p is not None or min_p is not None:
-            key = (logits.device, seed)
-            if key not in self._uniforms:
-                self._uniforms[key] = torch.Generator(device=logits.device).manual_seed(seed)
-            u = torch.rand(logits.size(0), generator=self._uniforms[key], device=logits.device)
+            gen = self._uniforms
+            if gen is None or gen.device != logits.device:
+                gen = self._uniforms = torch.Generator(device=logits.device)
+            gen.manual_seed(seed)
+            gen.set_offset(self._uniform_offset)
+            u = torch.rand(logits.size(0), generator=gen, device=logits.device)
+            self._uniform_offset = gen.get_offset()
             return kernels.sample_filtered(logits.to(torch.bfloat16), temperatures.to(torch.float32), u, top_k=top_k,
                                            top_p=top_p, min_p=min_p)
         offset = self._offset

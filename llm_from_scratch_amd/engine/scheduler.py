@@ -93,6 +93,8 @@ class Scheduler:
     def fork(self, seq: Sequence, n: int = 1) -> tuple[list[Sequence], list[tuple[int, int]]]:
         """n sequences that go on from a running one's tokens, on its blocks:
         (children, the block copies to make before the next step)."""
+        if n < 1:
+            raise ValueError(f"n must be >= 1, got {n}")
         if seq not in self.running:
             raise ValueError(f"sequence {seq.seq_id} is not running: only a running one has keys to share")
         if not self.block_manager.can_fork(seq, n):

@@ -31,8 +31,8 @@ class SamplingParams:
 
     def __post_init__(self):
         assert self.temperature > 1e-10, "greedy sampling is not permitted"
-        assert self.top_k >= 0 and 0 < self.top_p <= 1 and 0 <= self.min_p <= 1, \
-            "top_k must be >= 0, top_p in (0, 1], min_p in [0, 1]"
+        assert 0 <= self.top_k < 2 ** 31 and 0 < self.top_p <= 1 and 0 <= self.min_p <= 1, \
+            "top_k must be in [0, 2**31), top_p in (0, 1], min_p in [0, 1]"
 
 
 class SequenceStatus(Enum):

@@ -3,9 +3,12 @@ behind a sliding window, forks, packing the pool, sampling filters."""
 import random
 
 import pytest
+import torch
 
 from llm_from_scratch_amd.decode_model import DecodeModelConfig
 from llm_from_scratch_amd.engine import BlockManager, SamplingParams, Scheduler, Sequence
+from llm_from_scratch_amd.engine.block_manager import Block
+from llm_from_scratch_amd.engine.llm_engine import check_window
 from llm_from_scratch_amd.engine.model_runner import ModelRunner
 
 BS = 16
@@ -117,6 +120,9 @@ def test_fork_refusals():
     sched.postprocess([s], [1])
     with pytest.raises(RuntimeError, match="no free blocks"):
         sched.fork(s, 2)
+    for n in (0, -1):
+        with pytest.raises(ValueError, match="n must be"):
+            sched.fork(s, n)
     assert len(sched.running) == 1
     consistent(sched.block_manager, [s])
     sched.fork(s, 1)
@@ -203,8 +209,69 @@ def test_preemption_spares_what_could_not_come_back():
             alone.postprocess(ran, [i % 5])
 
 
+def test_the_same_tokens_behind_another_prefix_are_no_hit():
+    """A block freed with its hash still known, then filled with the same tokens
+    behind other ones: the first prompt must not find it."""
+    p1, p2, x = list(range(BS)), list(range(100, 100 + BS)), list(range(50, 50 + BS))
+    bm = BlockManager(5, BS)
+    keep, a = Sequence(p1 + [7]), Sequence(p1 + x + [7])
+    bm.allocate(keep)
+    bm.allocate(a)
+    block = a.block_table[1]
+    bm.deallocate(a)
+    spare = Sequence([1])  # frees leave the queue's front: block is next but one
+    bm.allocate(spare)
+    while bm.free_block_ids[1] != block:
+        bm.free_block_ids.rotate(1)
+    b = Sequence(p2 + x)  # its last block takes x after p2
+    bm.allocate(b)
+    assert b.block_table[1] == block
+    bm.deallocate(spare)
+    bm.free_block_ids.append(len(bm.blocks))
+    bm.blocks.append(Block(len(bm.blocks)))
+    c = Sequence(p1 + x + [7])
+    bm.allocate(c)
+    assert c.block_table[0] == keep.block_table[0] and c.block_table[1] != block and c.num_cached_tokens == BS
+
+
+def test_packing_leaves_no_false_prefix():
+    """The same where packing moves a block onto a freed one's place."""
+    p1, p2, x = list(range(BS)), list(range(100, 100 + BS)), list(range(50, 50 + BS))
+    bm = BlockManager(12, BS)
+    keep, a, b = Sequence(p1 + [7]), Sequence(p1 + x + [7]), Sequence(p2 + x + [7])
+    for s in (keep, a, b):
+        bm.allocate(s)
+    hole = a.block_table[1]
+    bm.deallocate(a)
+    moved = dict(bm.pack())
+    b.block_table = [moved.get(i, i) for i in b.block_table]
+    c = Sequence(p1 + x + [7])
+    bm.allocate(c)
+    assert hole in moved.values()
+    assert c.block_table[0] == keep.block_table[0] and c.block_table[1] not in b.block_table
+    assert c.num_cached_tokens == BS
+
+
+def test_engine_and_model_windows_agree():
+    class Layer(torch.nn.Module):
+        def __init__(self, window, sinks):
+            super().__init__()
+            self.k_cache = self.v_cache = torch.empty(0)
+            self.window, self.sinks = window, sinks
+
+    model = torch.nn.Sequential(Layer(64, 4), Layer(32, 0))
+    check_window(model, None, 0)
+    check_window(model, 64, 4)
+    check_window(model, 100, 16)
+    for window, sinks in ((63, 4), (64, 3)):
+        with pytest.raises(ValueError, match="the engine keeps"):
+            check_window(model, window, sinks)
+    with pytest.raises(ValueError, match="window of None"):
+        check_window(torch.nn.Sequential(Layer(None, 0)), 64, 4)
+
+
 def test_sampling_params_and_filters():
-    for bad in (dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.1), dict(min_p=-0.1), dict(min_p=2.0)):
+    for bad in (dict(top_k=-1), dict(top_k=2 ** 31), dict(top_p=0.0), dict(top_p=1.1), dict(min_p=-0.1), dict(min_p=2.0)):
         with pytest.raises(AssertionError):
             SamplingParams(**bad)
     runner = ModelRunner.__new__(ModelRunner)

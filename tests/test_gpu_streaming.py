@@ -14,7 +14,7 @@ import torch
 
 from llm_from_scratch_amd.context import reset_context
 from llm_from_scratch_amd.decode_model import DecodeModel, DecodeModelConfig
-from llm_from_scratch_amd.engine import BlockManager, LLMEngine, ModelRunner, SamplingParams, Sequence
+from llm_from_scratch_amd.engine import BlockManager, LLMEngine, ModelRunner, Sampler, SamplingParams, Sequence
 from oracle import paged_kv as P
 
 pytestmark = pytest.mark.gpu
@@ -209,6 +209,19 @@ def test_filters_mix_in_a_batch_and_seeds_repeat():
     while not eng.scheduler.is_finished():
         done.update(eng.step()[0])
     assert done[sorted(done)[1]][:25] == a[1]
+
+
+def test_filter_draws_advance_whatever_the_generator():
+    """Calls with generators of two seeds in turn: no draw repeats, a second
+    sampler draws the same."""
+    logits = torch.zeros(8, 4096, dtype=torch.bfloat16, device="cuda")
+    T, p = torch.ones(8, device="cuda"), torch.full((8,), 0.99, device="cuda")
+    g = [torch.Generator(device="cuda").manual_seed(s) for s in (5, 6)]
+    runs = []
+    for _ in range(2):
+        s = Sampler()
+        runs.append([tuple(s(logits, T, g[i % 2], top_p=p).tolist()) for i in range(6)])
+    assert runs[0] == runs[1] and len(set(runs[0])) == 6
 
 
 def test_a_stream_outgrows_its_pool():
