@@ -24,16 +24,20 @@
 // of the row (a mask's, say) is counted by ballots and not in LDS, where its
 // additions would queue up: one that 8 of 64 samples have.  One wave then
 // walks the counts (512 chunks of 128 bins, a chunk an exponent and a sign)
-// for the cuts; meanwhile the others read the row again, from the caches,
-// into registers, and find the token among equals there.
+// for top-k, top-p and the draw, another for min-p's cut; meanwhile the others
+// read the row again, from the caches, into registers, and find the token
+// among equals there.
 //
-// Measured: 256 rows of 150001 with all filters 40 us, one row of 32000
-// 15 us.  The bound is not memory (the logits of the 256 take 16 us): of a
-// long row's 69000 cycles the counting, with one LDS addition a token, takes
-// 25000, the cuts, a chain of one wave's dependent steps, 9000 to 11000, and
-// the second read and its search 13000; a row of 32000 has 6000, 7000 to
-// 10000 and 4000 of 34000.  The cuts as a loop over one search took such a row
-// to 16.7 us: fewer instructions, but more steps in the chain.
+// Measured: 256 rows of 150001 with top-p and min-p 39 us, one row of 32000
+// with all filters 14.5 us.  The bound is not memory (the logits of the 256 take
+// 16 us), but a chain of phases: of a long row's 74000 cycles (one of 256) the
+// counting takes 30000, by HBM and one LDS addition a token at nine cycles a
+// wave's, the sums of counts and of weights 11000, by instructions (16 cycles
+// each over the workgroup, 32 in 64 bits), the cuts 8000, by one wave's
+// latencies, and the second read and its search 19000; a row of 32000 has 6200,
+// 11000, 7000 and 3000 of 32000.  Loads begun while LDS is cleared and beside
+// the counting took the 256 rows to 41.6 us, the cuts as a loop over one
+// search one row to 16.7.
 #include "common.h"
 
 namespace lfs {
@@ -47,8 +51,9 @@ constexpr int kChunks = kBins / kChunk;
 constexpr int CPL = kChunks / 64;    // chunks per lane
 constexpr int kWindow = 32768;       // 32-bit bins counted at once
 constexpr int FU = 8;                // 16-byte pieces of the row that a thread has in flight
-constexpr int FH = 20;               // and that a thread of all waves but one holds
-constexpr int FNH = FNT - 64;
+constexpr int FH = 22;               // and that a thread of all waves but two holds
+constexpr int FNH = FNT - 128;
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 constexpr int kList = FNT;           // equal tokens ranked as a list, one a thread
 
 // Bin of a logit, 0 the largest value; kBins for one that is never drawn
@@ -67,8 +72,9 @@ __device__ __forceinline__ double bin_value(int d) { return (double)bf16_to_f32(
 struct Weights {
   int top;  // the largest logit's bin
   double xmax, c;
-  __device__ __forceinline__ double at(int d) const {
-    const double t = (bin_value(d) - xmax) * c, n = rint(t), f = (t - n) * 0.6931471805599453;
+  __device__ __forceinline__ double at(int d) const { return d == top ? 1.0 : of(bin_value(d) - xmax); }
+  __device__ __forceinline__ double of(double x) const {
+    const double t = x * c, n = rint(t), f = (t - n) * 0.6931471805599453;
     double w = 1.0 / 479001600;
     w = fma(w, f, 1.0 / 39916800);
     w = fma(w, f, 1.0 / 3628800);
@@ -82,8 +88,7 @@ struct Weights {
     w = fma(w, f, 0.5);
     w = fma(w, f, 1.0);
     w = fma(w, f, 1.0);
-    w = t > -1000.0 ? ldexp(w, (int)n) : 0.0;  // NaN (an infinite logit and temperature): 0
-    return d == top ? 1.0 : w;
+    return t > -1000.0 ? ldexp(w, (int)n) : 0.0;  // NaN (an infinite logit and temperature): 0
   }
 };
 
@@ -135,12 +140,12 @@ __device__ __forceinline__ X before(X upto) {  // the lane before's; 0 in lane 0
   return (threadIdx.x & 63) == 0 ? X(0) : v;
 }
 
-// A place in the order: n tokens of bin d, after all of the bins before it;
-// c and m: their count and weight.
+// A place in the order: n tokens of bin d, w each, after all of the bins
+// before it; c and m: their count and weight.
 struct Place {
   int d;
   uint32_t n, c;
-  double m;
+  double m, w;
 };
 
 struct Filters {
@@ -148,9 +153,16 @@ struct Filters {
   double p, m, u;
 };
 
-// The last bin whose weight reaches m <= 1, 64 bins tried at a time.
-__device__ __forceinline__ int last_reaching(const Weights& wt, double m) {
+// The last bin whose weight reaches m in (0, 1]: among the 64 around the one
+// that the inverse formula names in 32 bits, or, where it lies outside (values
+// next to 0, whose bins are narrower than that is exact), 64 bins tried at a
+// time.
+__device__ __forceinline__ int last_reaching(const Weights& wt, float T, double m) {
   const int lane = threadIdx.x & 63;
+  const float x = (float)wt.xmax + __builtin_amdgcn_logf((float)m) * 0.6931472f * T;
+  const int near = max(wt.top, min(bin_of(__float_as_uint(x) >> 16) - 32, kBins - 64));
+  const uint64_t reach = __ballot(near + lane < kBins && wt.at(min(near + lane, kBins - 1)) >= m);
+  if ((reach & 1) != 0 && reach != ~0ull) return near + __builtin_ctzll(~reach) - 1;
   int lo = wt.top;
 #pragma unroll 1
   for (int step = 1024; step > 0; step >>= step == 1024 ? 6 : 4) {  // 1024, 16, 1
@@ -161,48 +173,56 @@ __device__ __forceinline__ int last_reaching(const Weights& wt, double m) {
   return lo;
 }
 
-// The cuts and the draw, by one wave or by several alike.  hold_bins(chunk, n)
-// fills in a chunk's two bins per lane; lo: the last bin that reaches min-p
-// (where that is in (0, 1]).  d: the drawn token's bin, nth: its
-// place among the bin's tokens, S: the kept weight.
+// A row's order by its counts, for the cuts and the draw: of one wave, or of several alike.  hold_bins(chunk, n)
+// fills in a chunk's two bins per lane.
 template <class Hold>
-__device__ __forceinline__ void draw(const Weights& wt, const Filters& f, int lo, const uint32_t* cnt,
-                                     const double* mass, Hold&& hold_bins, int& d, uint32_t& nth, double& S) {
-  const int lane = threadIdx.x & 63;
-  // sums up to the end of the lane's CPL chunks
-  uint32_t lane_n = 0;
-  double lane_w = 0.0;
-#pragma unroll
-  for (int i = 0; i < CPL; ++i) {
-    const uint32_t n = cnt[CPL * lane + i];
-    lane_n += n;
-    lane_w += n != 0 ? mass[CPL * lane + i] : 0.0;
-  }
-  lane_n = scan_sum(lane_n);
-  lane_w = scan_sum(lane_w);
-  const uint32_t lane_nb = before(lane_n);
-  const double lane_wb = before(lane_w);
+struct Order {
+  const Weights& wt;
+  const uint32_t* cnt;
+  const double* mass;
+  Hold hold_bins;
+  int lane, held = -1;
+  // sums up to the end of the lane's CPL chunks, and before them
+  uint32_t lane_n = 0, lane_nb;
+  double lane_w = 0.0, lane_wb;
   uint32_t n[2], upto_n = 0;  // of the chunk held: the lane's two bins, sums up to their end
-  double w[2], upto_w = 0.0;
-  int held = -1;
-  auto hold = [&](int chunk) {
+  double one[2], w[2], upto_w = 0.0;  // of a token, of the bin
+
+  __device__ __forceinline__ Order(const Weights& wt, const uint32_t* cnt, const double* mass, Hold hold_bins)
+      : wt(wt), cnt(cnt), mass(mass), hold_bins(hold_bins), lane(threadIdx.x & 63) {
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) {
+      const uint32_t c = cnt[CPL * lane + i];
+      lane_n += c;
+      lane_w += c != 0 ? mass[CPL * lane + i] : 0.0;
+    }
+    lane_n = scan_sum(lane_n);
+    lane_w = scan_sum(lane_w);
+    lane_nb = before(lane_n);
+    lane_wb = before(lane_w);
+  }
+  __device__ __forceinline__ void hold(int chunk) {
     if (chunk == held) return;
     held = chunk;
     hold_bins(chunk, n);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w[i] = n[i] != 0 ? n[i] * wt.at(chunk * kChunk + 2 * lane + i) : 0.0;
+    for (int i = 0; i < 2; ++i) {
+      one[i] = wt.at(chunk * kChunk + 2 * lane + i);
+      w[i] = n[i] != 0 ? n[i] * one[i] : 0.0;
+    }
     upto_n = scan_sum(n[0] + n[1]);
     upto_w = scan_sum(w[0] + w[1]);
-  };
+  }
   // The first lane whose sums are not 0 and satisfy pred; the last that adds to
   // them where none does.
-  auto first_lane = [&](bool some, bool hit) -> int {
+  __device__ __forceinline__ static int first_lane(bool some, bool hit) {
     const uint64_t any = __ballot(hit);
     return any != 0 ? __builtin_ctzll(any) : 63 - __builtin_clzll(__ballot(some) | 1);
-  };
+  }
   // the first bin that is not empty and at whose end pred(count, weight) holds
   // of the sums so far; the last one that is not empty where none does
-  auto find = [&](auto&& pred) -> Place {
+  template <class Pred>
+  __device__ __forceinline__ Place find(Pred&& pred) {
     const bool some = lane_n != lane_nb;  // the scan's sums of a lane without tokens may differ from the one before's
     const int src = first_lane(some, some && pred(lane_n, lane_w));
     const uint32_t cb = lane_u(lane_nb, src);
@@ -212,7 +232,7 @@ __device__ __forceinline__ void draw(const Weights& wt, const Filters& f, int lo
     const uint32_t c_upto = cb + scan_sum8(cn);
     const double m_upto = mb + scan_sum8(cn != 0 ? mass[CPL * src + at8] : 0.0);
     const int c8 = first_lane(lane < CPL && cn != 0, lane < CPL && cn != 0 && pred(c_upto, m_upto));
-    Place at{0, 0, 0, 0.0};
+    Place at{0, 0, 0, 0.0, 0.0};
     at.c = c8 == 0 ? cb : lane_u(c_upto, c8 - 1);
     at.m = c8 == 0 ? mb : lane_d(m_upto, c8 - 1);
     const int chunk = CPL * src + c8;
@@ -228,29 +248,30 @@ __device__ __forceinline__ void draw(const Weights& wt, const Filters& f, int lo
     const double wb = before(upto_w);
     at.c = lane_u(second ? n0 : n0 - n[0], l);
     at.m += second ? lane_d(wb + w[0], l) : lane_d(wb, l);
+    at.w = lane_d(second ? one[1] : one[0], l);
     return at;
-  };
-  // top-k: the first k tokens
-  const uint32_t all = lane_u(lane_n, 63);
-  Place end{kBins, 0, all, lane_d(lane_w, 63)};  // all tokens
-  if (f.k > 0 && f.k < (int64_t)all) {
-    end = find([&](uint32_t c, double) { return c >= (uint32_t)f.k; });
-    end.n = min(end.n, (uint32_t)f.k - end.c);
   }
-  auto weight = [&](const Place& at) { return at.m + (at.n != 0 ? at.n * wt.at(at.d) : 0.0); };
-  S = weight(end);
-  // top-p: the tokens before which the weight is below the target
-  if (f.p < 1.0) {
-    const double target = f.p * S;
-    Place at = find([&](uint32_t, double m) { return m >= target; });
-    const double need = ceil((target - at.m) / wt.at(at.d));
-    at.n = need >= 1.0 ? (need < (double)at.n ? (uint32_t)need : at.n) : 1u;
-    if (at.d < end.d || (at.d == end.d && at.n < end.n)) end = at;
+  __device__ __forceinline__ static double weight(Place at) { return at.m + at.n * at.w; }
+  // the last token that top-k and top-p keep
+  __device__ __forceinline__ Place first_cuts(const Filters& f) {
+    const uint32_t all = lane_u(lane_n, 63);
+    Place end{kBins, 0, all, lane_d(lane_w, 63), 0.0};  // all tokens
+    if (f.k > 0 && f.k < (int64_t)all) {
+      end = find([&](uint32_t c, double) { return c >= (uint32_t)f.k; });
+      end.n = min(end.n, (uint32_t)f.k - end.c);
+    }
+    if (f.p < 1.0) {  // the tokens before which the weight is below the target
+      const double target = f.p * weight(end);
+      Place at = find([&](uint32_t, double m) { return m >= target; });
+      const double need = ceil((target - at.m) / at.w);
+      at.n = need >= 1.0 ? (need < (double)at.n ? (uint32_t)need : at.n) : 1u;
+      end = earlier(end, at);
+    }
+    return end;
   }
-  // min-p
-  if (f.m > 1.0) {
-    end = Place{wt.top, 1, 0, 0.0};
-  } else if (f.m > 0.0 && lo < end.d) {  // the tokens up to bin lo
+  // that min-p keeps; lo: the last bin that reaches it, where it is in (0, 1]
+  __device__ __forceinline__ Place min_cut(const Filters& f, int lo) {
+    if (f.m > 1.0) return Place{wt.top, 1, 0, 0.0, 1.0};
     const int chunk = lo / kChunk;
     hold(chunk);
     uint32_t to = 0;  // tokens up to bin lo
@@ -259,39 +280,48 @@ __device__ __forceinline__ void draw(const Weights& wt, const Filters& f, int lo
 #pragma unroll
     for (int i = 0; i < 2; ++i) to += chunk * kChunk + 2 * lane + i <= lo ? n[i] : 0;
     to = lane_u(scan_sum(to), 63);
-    end = find([&](uint32_t c, double) { return c >= to; });
+    return find([&](uint32_t c, double) { return c >= to; });
   }
-  S = weight(end);
-  const double target = f.u * S;
-  Place at = find([&](uint32_t, double m) { return m > target; });
-  if (at.d > end.d) at = end;
-  if (at.d == end.d) at.n = min(at.n, end.n);
-  const double skip = floor((target - at.m) / wt.at(at.d));
-  d = at.d;
-  nth = skip > 0.0 ? (skip < (double)(at.n - 1) ? (uint32_t)skip : at.n - 1) : 0u;
-}
+  __device__ __forceinline__ static Place earlier(Place a, Place b) {
+    const bool is_b = b.d < a.d || (b.d == a.d && b.n < a.n);
+    return Place{is_b ? b.d : a.d, is_b ? b.n : a.n, is_b ? b.c : a.c, is_b ? b.m : a.m, is_b ? b.w : a.w};
+  }
+  // d: the drawn token's bin, nth: its place among the bin's tokens, S: the kept weight
+  __device__ __forceinline__ void pick(Place end, double u, int& d, uint32_t& nth, double& S) {
+    S = weight(end);
+    const double target = u * S;
+    Place at = find([&](uint32_t, double m) { return m > target; });
+    at = Place{min(at.d, end.d), at.d >= end.d ? (at.d == end.d ? min(at.n, end.n) : end.n) : at.n, 0,
+               at.d > end.d ? end.m : at.m, at.d > end.d ? end.w : at.w};
+    const double skip = floor((target - at.m) / at.w);
+    d = at.d;
+    nth = skip > 0.0 ? (skip < (double)(at.n - 1) ? (uint32_t)skip : at.n - 1) : 0u;
+  }
+};
 
 __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     const uint16_t* __restrict__ logits, int64_t ld, const float* __restrict__ temps,
     const float* __restrict__ uniforms, const int32_t* __restrict__ top_k, const float* __restrict__ top_p,
     const float* __restrict__ min_p, int V, int64_t* __restrict__ out, float* __restrict__ logprob) {
   __shared__ __attribute__((aligned(16))) uint32_t hist[kWindow];
-  __shared__ double mass[kChunks];
+  __shared__ __attribute__((aligned(16))) double mass[kChunks];
   __shared__ double drawn_s;
-  __shared__ uint32_t cnt[kChunks];
+  __shared__ __attribute__((aligned(16))) uint32_t cnt[kChunks];
   __shared__ uint32_t bins[kChunk];
   __shared__ uint32_t places[FNW + 1];
-  __shared__ uint32_t many_value, many_n, lost, drawn_n, list_n;
+  __shared__ uint32_t many_value, many_n, lost, drawn_n, list_n, min_ready;
   __shared__ __attribute__((aligned(16))) uint32_t list[kList];
   __shared__ int drawn_d, reaching;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ Place min_end;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t b = blockIdx.x;
   const uint16_t* row = logits + b * ld;
   // The row: `head` tokens up to a 16-byte boundary, `pieces` of 8, and the rest.
   const int head = min(V, (int)(-(uintptr_t)row >> 1 & 7)), pieces = (V - head) / 8;
   const uint4* body = reinterpret_cast<const uint4*>(row + head);
   // of the first 16 threads: a token outside the pieces, or -1
-  const int edge = tid < 8 ? (tid < head ? tid : -1) : tid < 16 && head + 8 * pieces + tid - 8 < V ? head + 8 * pieces + tid - 8 : -1;
+  const int edge = tid < 8 ? (tid < head ? tid : -1)
+                   : tid < 16 && head + 8 * pieces + tid - 8 < V ? head + 8 * pieces + tid - 8 : -1;
   // fn(piece, its number, whether it is one) over the pieces past `from`, FU of a thread's loaded together
   auto walk = [&](int from, auto&& fn) {
     for (int first = from; first < pieces; first += FU * FNT) {
@@ -311,7 +341,7 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   f.m = min_p != nullptr ? (double)min_p[b] : 0.0;
   f.u = fmin(fmax((double)uniforms[b], 0.0), 1.0 - 0x1p-24);  // a NaN counts as 0
   for (int i = tid; i < kWindow / 4; i += FNT) reinterpret_cast<uint4*>(hist)[i] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) many_n = lost = list_n = 0;
+  if (tid == 0) many_n = lost = list_n = min_ready = 0;
   if (wave == FNW - 1) {  // a value that 8 of 64 samples have
     const uint32_t v = row[(int64_t)lane * V >> 6];
     uint64_t alike = ~0ull;  // lanes with the same bits
@@ -382,29 +412,31 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     }
     sum += lo + hi;
     lo = scan_sum8(lo), hi = scan_sum8(hi);
-    if ((lane & 7) == 7) cnt[kChunks / 2 - 1 - pair] = lo, cnt[kChunks / 2 + pair] = hi;
+    if ((lane & 7) == 7) {
+      const int above = kChunks / 2 - 1 - pair, below = kChunks / 2 + pair;  // the chunks of the two
+      // what the words do not say: -0 counts as +0, NaN and -infinity not at all, the shared value is apart
+      if (pair == 0) lo += hist[0] >> 16, hi -= hist[0] >> 16;
+      if (above == 0) lo = hist[0x7F80] & 0xFFFFu, hi = 0;
+      const int extra = many != ~0u && bin_of(many) < kBins ? bin_of(many) / kChunk : -1;
+      cnt[above] = lo + (above == extra ? many_all : 0u);
+      cnt[below] = hi + (below == extra ? many_all : 0u);
+    }
   }
   sum = lane_u(scan_sum(sum), 63) + many_here - (wave == 0 ? (uint32_t)V : 0u);
   if (lane == 0 && sum != 0) atomicAdd(&lost, sum);  // modulo 2^32: 0 over the waves where every count fits
   __syncthreads();
   const bool counted = lost == 0;
-  if (tid == 0 && counted) {  // what the words do not say
-    if (many != ~0u && bin_of(many) < kBins) cnt[bin_of(many) / kChunk] += many_all;
-    const uint32_t minus = (hist[0] >> 16);  // -0, counted as +0
-    cnt[kChunks / 2] -= minus, cnt[kChunks / 2 - 1] += minus;
-    cnt[0] = bits_count(0x7F80u);  // NaN apart
-    cnt[kChunks - 1] = 0;          // -infinity, NaN
-  }
-  __syncthreads();
 
   // the largest logit
+  uint32_t have;  // a bit for each of the lane's chunks that is not empty
   auto first_chunk = [&]() -> int {
-    int c = kChunks;
+    have = 0;
 #pragma unroll
-    for (int i = CPL - 1; i >= 0; --i)
-      if (cnt[CPL * lane + i] != 0) c = CPL * lane + i;
-    const uint64_t any = __ballot(c < kChunks);
-    return any == 0 ? -1 : (int)lane_u((uint32_t)c, __builtin_ctzll(any));
+    for (int i = 0; i < CPL; ++i) have |= (cnt[CPL * lane + i] != 0 ? 1u : 0u) << i;
+    const uint64_t any = __ballot(have != 0);
+    if (any == 0) return -1;
+    const int src = __builtin_ctzll(any);
+    return CPL * src + __builtin_ctz(lane_u(have, src));
   };
   auto first_bin = [&](int chunk, uint32_t n0, uint32_t n1) -> int {
     const int src = __builtin_ctzll(__ballot(n0 + n1 != 0));
@@ -416,6 +448,7 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   uint32_t nth = 0;
   double S = 0.0;
   uint4 held[FH];
+  const int held_tid = tid - (FNT - FNH), held_wave = wave * 64 - (FNT - FNH);
   if (counted) {
     const int c0 = first_chunk();
     if (c0 < 0) {  // nothing can be drawn
@@ -427,40 +460,59 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     }
     wt.top = first_bin(c0, bin_count(c0 * kChunk + 2 * lane), bin_count(c0 * kChunk + 2 * lane + 1));
     wt.xmax = bin_value(wt.top);
-    // the last wave looks for min-p's last bin meanwhile
+    // The chunks that are not empty, dealt to the waves in turn; the last wave
+    // looks for min-p's last bin meanwhile.
     const int waves = f.m > 0.0 ? FNW - 1 : FNW;
     static_assert(kChunks <= 64 * (FNW - 1), "a lane for each of a wave's chunks");
-    const int mine = wave + waves * lane;
-    uint64_t some = __ballot(wave < waves && mine < kChunks && cnt[min(mine, kChunks - 1)] != 0);
-    while (some != 0) {  // two chunks at a time, for the latency of their exponentials and sums
-      const int c0 = wave + waves * __builtin_ctzll(some);
-      some &= some - 1;
-      const int c1 = some != 0 ? wave + waves * __builtin_ctzll(some) : c0;
-      some &= some - 1;
-      const int e0 = c0 * kChunk + 2 * lane, e1 = c1 * kChunk + 2 * lane;
-      auto weight = [&](int e) {  // bins before the first have no tokens and no finite weight
-        const uint32_t n = bin_count(e);
-        const double w = wt.at(e);
-        return n != 0 ? n * w : 0.0;
-      };
-      const double m0 = weight(e0) + weight(e0 + 1), m1 = weight(e1) + weight(e1 + 1);
-      const double all0 = lane_d(scan_sum(m0), 63), all1 = lane_d(scan_sum(m1), 63);
-      if (lane == 0) mass[c0] = all0, mass[c1] = all1;
+    const uint32_t upto = scan_sum((uint32_t)__popc(have)), chunks = lane_u(upto, 63);
+    int mine = 0, num = 0;  // the wave's, one a lane
+    for (uint32_t r = wave; wave < waves && r < chunks; r += waves, ++num) {
+      const int src = __builtin_ctzll(__ballot(upto > r));
+      uint32_t bits = lane_u(have, src);
+      for (uint32_t skip = r + __builtin_popcount(bits) - lane_u(upto, src); skip > 0; --skip) bits &= bits - 1;
+      mine = lane == num ? CPL * src + __builtin_ctz(bits) : mine;
+    }
+    // A chunk's values are evenly spaced: the weight of a bin 64 further is
+    // this times its own.
+    const double ratio = num > 0 ? wt.of(bin_value(mine * kChunk + 64) - bin_value(mine * kChunk)) : 0.0;
+    for (int i = 0; i < num; ++i) {
+      const int c = (int)lane_u((uint32_t)mine, i), e = c * kChunk + lane;
+      const uint32_t n0 = bin_count(e), n1 = bin_count(e + 64);
+      const double w0 = wt.at(e);
+      const double w1 = c == c0 ? wt.at(e + 64) : w0 * lane_d(ratio, i);  // bins before the first: no finite weight
+      const double all = lane_d(scan_sum((n0 != 0 ? n0 * w0 : 0.0) + (n1 != 0 ? n1 * w1 : 0.0)), 63);
+      if (lane == 0) mass[c] = all;
     }
     if (wave >= waves) {
-      const int lo = last_reaching(wt, f.m);
+      const int lo = last_reaching(wt, T, f.m);
       if (lane == 0) reaching = lo;
     }
     __syncthreads();
-    if (wave > 0) {  // the row again, for the search after the draw
+    if (held_wave >= 0) {  // the row again, for the search after the draw
 #pragma unroll
       for (int r = 0; r < FH; ++r)
-        if (r * FNH + wave * 64 - 64 < pieces) held[r] = body[min(r * FNH + tid - 64, pieces - 1)];
+        if (r * FNH + held_wave < pieces) held[r] = body[min(r * FNH + held_tid, pieces - 1)];
     } else {
-      draw(wt, f, reaching, cnt, mass, [&](int chunk, uint32_t (&n)[2]) {
+      auto hold_bins = [&](int chunk, uint32_t (&n)[2]) {
         n[0] = bin_count(chunk * kChunk + 2 * lane), n[1] = bin_count(chunk * kChunk + 2 * lane + 1);
-      }, d, nth, S);
-      if (lane == 0) drawn_d = d, drawn_n = nth, drawn_s = S;
+      };
+      Order<decltype(hold_bins)> order(wt, cnt, mass, hold_bins);
+      if (wave == 0) {
+        Place end = order.first_cuts(f);
+        if (f.m > 0.0) {  // wave 1's part, which waits for nothing; a barrier would also wait for the others' loads
+          while (__hip_atomic_load(&min_ready, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP) == 0)
+            __builtin_amdgcn_s_sleep(1);
+          end = order.earlier(end, min_end);
+        }
+        order.pick(end, f.u, d, nth, S);
+        if (lane == 0) drawn_d = d, drawn_n = nth, drawn_s = S;
+      } else if (f.m > 0.0) {
+        const Place at = order.min_cut(f, reaching);
+        if (lane == 0) {
+          min_end = at;
+          __hip_atomic_store(&min_ready, 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+      }
     }
     __syncthreads();
     d = drawn_d, nth = drawn_n, S = drawn_s;
@@ -512,10 +564,14 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
       }
       return;
     }
-    draw(wt, f, last_reaching(wt, f.m), cnt, mass, [&](int chunk, uint32_t (&n)[2]) {  // the whole workgroup, the same chunk
+    auto hold_bins = [&](int chunk, uint32_t (&n)[2]) {  // the whole workgroup, the same chunk
       recount(chunk * kChunk, kChunk, bins);
       n[0] = bins[2 * lane], n[1] = bins[2 * lane + 1];
-    }, d, nth, S);
+    };
+    Order<decltype(hold_bins)> order(wt, cnt, mass, hold_bins);
+    Place end = order.first_cuts(f);
+    if (f.m > 0.0) end = order.earlier(end, order.min_cut(f, last_reaching(wt, T, f.m)));
+    order.pick(end, f.u, d, nth, S);
   }
 
   // the nth of the bin's tokens by index
@@ -525,12 +581,11 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
   };
   // a half of a word matches where it is 0 here; +0 also meets -0
   const uint32_t same = bits_of(d) * 0x10001u, mask = d == 0x7FFF ? 0x7FFF7FFFu : ~0u;
-  // Top bits of the halves that are 0, and perhaps of a half above one (the
-  // borrow): exact on whether there is one
-  auto zeros = [&](uint32_t w) { return (w - 0x10001u) & ~w & 0x80008000u; };
-  auto any_match = [&](const uint4& x) {
-    return (zeros((x.x ^ same) & mask) | zeros((x.y ^ same) & mask) | zeros((x.z ^ same) & mask) |
-            zeros((x.w ^ same) & mask)) != 0;
+  auto any_match = [&](const uint4& x) {  // whether the least half is 0
+    auto halves = [&](uint32_t w) { return __builtin_bit_cast(u16x2, (w ^ same) & mask); };
+    const u16x2 least = __builtin_elementwise_min(__builtin_elementwise_min(halves(x.x), halves(x.y)),
+                                                  __builtin_elementwise_min(halves(x.z), halves(x.w)));
+    return least.x == 0 || least.y == 0;
   };
   auto matches = [&](const uint4& x) -> uint32_t {  // a bit for each of the eight
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -550,10 +605,10 @@ __global__ __launch_bounds__(FNT) void sample_filtered_kernel(
     if (!in || !any_match(x)) return;
     for (uint32_t m = matches(x); m != 0; m &= m - 1) note(head + 8 * i + __builtin_ctz(m));
   };
-  if (counted && wave > 0) {
+  if (counted && held_wave >= 0) {
 #pragma unroll
     for (int r = 0; r < FH; ++r)
-      if (r * FNH + wave * 64 - 64 < pieces) search(held[r], r * FNH + tid - 64, r * FNH + tid - 64 < pieces);
+      if (r * FNH + held_wave < pieces) search(held[r], r * FNH + held_tid, r * FNH + held_tid < pieces);
   }
   walk(counted ? FH * FNH : 0, search);
   auto equal_bits = [&](uint32_t h) { return ((h ^ same) & mask & 0xFFFFu) == 0; };

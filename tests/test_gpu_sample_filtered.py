@@ -48,6 +48,24 @@ def test_tokens(B, V, filters):
             rng.choice([0.0, 1e-6, 0.01, 0.5, 1.0, 2.0, -1.0], B) if "m" in filters else None)
 
 
+@pytest.mark.parametrize("spread", [1e-30, 1e-3, 1.0, 1e30])
+def test_min_p_cuts_anywhere(spread):
+    """The last token that reaches min-p beside the largest, far from it, and
+    next to 0, where neighbouring logits lie closer than 32 bits resolve the
+    cut; over all chunks of values, of both signs and none."""
+    B, V = 48, 3000
+    logits = logits_of(B, V, spread, 31)
+    logits[:, ::5] *= 1e-4
+    logits[40:, 1:] = -logits[40:, 1:].abs()
+    logits[44:, 0] = -0.0
+    T = np.full(B, spread, np.float32)
+    top = logits.double().amax(1).cpu().numpy() / T
+    rng = np.random.default_rng(8)
+    near = np.minimum(np.exp(-top * (1 + np.where(np.arange(B) % 3 == 0, 0, 1e-3) * rng.standard_normal(B))), 1.0)
+    run(logits, T, rng.random(B, np.float32), m=np.where(np.arange(B) % 4 == 1, rng.random(B), near))
+    run(logits, T, rng.random(B, np.float32), k=2000, p=0.99, m=near)
+
+
 def test_equal_logits():
     """Every cut falls inside one bin: also with more equal logits than 16 bits
     count, where the token is floor(u n)."""
