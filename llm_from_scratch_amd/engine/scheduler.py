@@ -57,38 +57,37 @@ class Scheduler:
         if scheduled:
             return scheduled, True
 
+        order = list(self.running)
+        stalled = False
         while self.running:
             seq = self.running.popleft()
             self.block_manager.release_behind(seq)
             if not self.block_manager.can_append(seq):
-                if self.running:
-                    self.running.appendleft(seq)
-                    victim = self._victim()
+                victim = self._victim([seq, *self.running])
+                if victim is None:  # seq waits for the blocks of those that go on
+                    stalled = True
+                    continue
+                if victim is not seq:  # seq is tried again with the freed blocks
                     self.running.remove(victim)
-                    self.preempt(victim)
-                    continue  # the first running sequence is tried with the freed blocks
-                self._victim([seq])
-                self.preempt(seq)
-                break
+                    self.running.appendleft(seq)
+                self.preempt(victim)
+                continue
             if num_tokens >= self.max_num_batched_tokens or len(scheduled) >= self.max_num_sequences:
-                self.running.appendleft(seq)
                 break
             self.block_manager.append(seq)
             scheduled.append(seq)
             num_tokens += 1
-        if scheduled:
-            self.running.extendleft(reversed(scheduled))
+        self.running = deque(s for s in order if s.status == SequenceStatus.RUNNING)
+        if stalled and not scheduled:
+            raise RuntimeError("the KV pool is full, and no running sequence fits it to be resumed later")
         return scheduled, False
 
-    def _victim(self, among=None) -> Sequence:
-        """The newest running sequence whose context the pool can hold at once,
-        as its prefill will ask: behind a sliding window one may outgrow the
-        pool, and could never be resumed."""
+    def _victim(self, among: list[Sequence]) -> Optional[Sequence]:
+        """The newest sequence whose context the pool can hold at once, as its
+        prefill will ask: behind a sliding window one may outgrow the pool, and
+        could never be resumed."""
         total = len(self.block_manager.blocks)
-        for seq in reversed(self.running if among is None else among):
-            if seq.num_blocks <= total:
-                return seq
-        raise RuntimeError("the KV pool is full, and no running sequence fits it to be resumed later")
+        return next((seq for seq in reversed(among) if seq.num_blocks <= total), None)
 
     def fork(self, seq: Sequence, n: int = 1) -> tuple[list[Sequence], list[tuple[int, int]]]:
         """n sequences that go on from a running one's tokens, on its blocks:

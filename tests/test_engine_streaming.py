@@ -290,3 +290,108 @@ def test_config_refusals():
     assert rc["sliding_window"] == 128 and rc["num_sink_tokens"] == 4
     assert cfg.reference_state_keys()["layers.0.att.q_norm.weight"] == (64,)
     assert DecodeModelConfig().reference_state_keys()["layers.0.att.q_norm.weight"] == (768,)
+
+
+def in_one_queue(sched, seqs):
+    """Every sequence is finished or in one queue once, and the blocks held are the running ones'."""
+    for s in seqs:
+        assert s.is_finished + sched.waiting.count(s) + sched.running.count(s) == 1, s.seq_id
+    consistent(sched.block_manager, list(sched.running))
+
+
+def drive(sched, seqs, steps=20000):
+    """Run to the end, the queues looked at after every step."""
+    for i in range(steps):
+        if sched.is_finished():
+            break
+        ran, _ = sched.schedule()
+        in_one_queue(sched, seqs)
+        sched.postprocess(ran, [i % 7] * len(ran))
+    assert all(s.is_finished for s in seqs)
+    assert not sched.block_manager.used_block_ids
+
+
+def test_a_sequence_past_the_pool_waits_for_one_that_runs_on():
+    """The last running sequence needs a block, is longer than the pool and so
+    cannot be preempted, but one before it goes on: it waits for its blocks."""
+    sched = Scheduler(8, 1000, 6, BS, eos=-1, sliding_window=48)
+    seqs = [Sequence([i] * n, SamplingParams(max_tokens=m)) for i, (n, m) in
+            enumerate([(7, 60), (71, 70), (53, 20), (54, 20)])]
+    for s in seqs:
+        sched.add_sequence(s)
+    drive(sched, seqs)
+    # a stream past its pool and its fork
+    sched = Scheduler(8, 1000, 5, BS, eos=-1, sliding_window=2 * BS)
+    stream = Sequence([1] * 10, SamplingParams(max_tokens=12 * BS))
+    sched.add_sequence(stream)
+    for i in range(8 * BS):
+        ran, _ = sched.schedule()
+        sched.postprocess(ran, [i % 5])
+    assert stream.num_blocks > 5
+    children, _ = sched.fork(stream, 1)
+    drive(sched, [stream, *children])
+
+
+def test_the_queues_stand_when_the_pool_is_too_small():
+    """Two sequences longer than the pool, both without a block to go on with:
+    the error takes neither out of its queue."""
+    sched = Scheduler(8, 1000, 4, BS, eos=-1, sliding_window=40)
+    stream = Sequence([1] * 10, SamplingParams(max_tokens=10 ** 6))
+    sched.add_sequence(stream)
+    while stream.num_tokens % BS or stream.num_blocks <= 5:
+        ran, _ = sched.schedule()
+        sched.postprocess(ran, [3] * len(ran))
+    seqs = [stream, *sched.fork(stream, 1)[0]]
+    held = None
+    for i in range(20 * BS):
+        try:
+            ran, _ = sched.schedule()
+        except RuntimeError as e:
+            assert "KV pool is full" in str(e)
+            held = [list(s.block_table) for s in seqs]
+            break
+        in_one_queue(sched, seqs)
+        sched.postprocess(ran, [3] * len(ran))
+    assert held is not None and list(sched.running) == seqs
+    in_one_queue(sched, seqs)
+    with pytest.raises(RuntimeError, match="KV pool is full"):  # again, with everything as it was
+        sched.schedule()
+    assert [s.block_table for s in seqs] == held and list(sched.running) == seqs
+    # one of them given up, the other goes on
+    sched.running.remove(seqs[0])
+    sched.block_manager.deallocate(seqs[0])
+    assert sched.schedule() == ([seqs[1]], False)
+
+
+@pytest.mark.parametrize("budget", [10 ** 6])
+def test_streams_of_any_lengths_finish_or_the_pool_is_full(budget):
+    """Random lengths, windows, pools and forks: every sequence finishes, or no
+    running one fits the pool or has a block to go on with."""
+    rnd = random.Random(budget)
+    ended = 0
+    for case in range(150):
+        pool, window = rnd.randrange(3, 12), rnd.choice([None, 1, BS, 32, 48, 100])
+        sched = Scheduler(rnd.randrange(1, 6), budget, pool, BS, eos=-1, sliding_window=window, num_sink_tokens=0 if window is None else rnd.choice([0, 4]))
+        longest = min(budget, (pool - 1) * BS)
+        seqs = [Sequence([rnd.randrange(3)] * rnd.randrange(1, longest), SamplingParams(max_tokens=rnd.randrange(1, 9 * BS)))
+                for _ in range(rnd.randrange(1, 6))]
+        for s in seqs:
+            sched.add_sequence(s)
+        for step in range(20000):
+            if sched.is_finished():
+                break
+            try:
+                ran, _ = sched.schedule()
+            except RuntimeError:
+                in_one_queue(sched, seqs)
+                assert sched.running and not sched.block_manager.free_block_ids
+                assert all(s.num_blocks > pool and s.num_tokens % BS == 1 for s in sched.running)
+                break
+            in_one_queue(sched, seqs)
+            sched.postprocess(ran, [step % 5] * len(ran))
+            if sched.running and rnd.random() < 0.01 and sched.block_manager.can_fork(sched.running[0]):
+                seqs += sched.fork(sched.running[0])[0]
+        else:
+            raise AssertionError("no end")
+        ended += sched.is_finished()
+    assert ended > 75
