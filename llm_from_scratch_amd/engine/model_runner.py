@@ -28,6 +28,7 @@ last_block_num_tokens (a full last block counts BS tokens).
 from __future__ import annotations
 
 import math
+from copy import copy
 from typing import Optional
 
 import torch
@@ -59,6 +60,24 @@ def prefill_metadata(seqs: list[Sequence], block_size: int) -> dict:
             slots.extend(range(seq.block_table[i] * BS, seq.block_table[i] * BS + n))
     return dict(input_ids=input_ids, positions=positions, cu_seqlens_q=cu_q, cu_seqlens_k=cu_k,
                 max_seqlen_q=max_q, max_seqlen_k=max_k, slot_mapping=slots)
+
+
+def prefill_parts(seqs: list[Sequence], block_size: int, budget: int) -> list[list[Sequence]]:
+    """The prefills that a scheduled batch takes, in turn: itself, or, where a
+    preempted sequence comes back alone and longer than ``budget`` tokens, as
+    many of its blocks at a time as the budget holds (at least one), each part
+    behind those before it as behind a cached prefix."""
+    seq = seqs[0]
+    if len(seqs) > 1 or seq.num_completion_tokens == 0 or seq.num_tokens - seq.num_cached_tokens <= budget:
+        return [seqs]
+    parts = []
+    step = max(1, budget // block_size) * block_size
+    for start in range(seq.num_cached_tokens, seq.num_tokens, step):
+        part = copy(seq)
+        part.num_cached_tokens, part.num_tokens = start, min(start + step, seq.num_tokens)
+        part.token_ids, part.block_table = seq.token_ids[:part.num_tokens], seq.block_table[:part.num_blocks]
+        parts.append([part])
+    return parts
 
 
 def decode_metadata(seqs: list[Sequence], block_size: int) -> dict:
@@ -141,6 +160,11 @@ class ModelRunner:
         assert layer == self.config["num_layers"], \
             f"found {layer} attention layers, expected {self.config['num_layers']}"
 
+    def token_budget(self) -> int:
+        """Tokens of a prefill, which the warm-up reserves memory for."""
+        cfg = self.config
+        return int(cfg.get("max_num_batched_tokens", cfg.get("max_num_batch_tokens", cfg.get("max_model_length", 4096))))
+
     @torch.inference_mode()
     def warmup_model(self) -> None:
         """One prefill of max_num_batched_tokens // max_model_length sequences
@@ -153,7 +177,7 @@ class ModelRunner:
         afterwards (its bytes count towards the reserved peak)."""
         cfg = self.config
         max_len = int(cfg.get("max_model_length", 4096))
-        budget = int(cfg.get("max_num_batched_tokens", cfg.get("max_num_batch_tokens", max_len)))
+        budget = self.token_budget()
         n_seq = max(1, budget // max_len)
         seq_len = min(max_len, budget)
         torch.cuda.empty_cache()
@@ -285,8 +309,11 @@ class ModelRunner:
 
     def run(self, seqs: list[Sequence], is_prefill: bool,
             generator: Optional[torch.Generator] = None) -> list[int]:
-        input_ids, positions = self.prepare_prefill(seqs) if is_prefill else self.prepare_decode(seqs)
-        logits = self.run_model(input_ids, positions, is_prefill)
+        if is_prefill:
+            for part in prefill_parts(seqs, self.block_size, self.token_budget()):
+                logits = self.run_model(*self.prepare_prefill(part), True)
+        else:
+            logits = self.run_model(*self.prepare_decode(seqs), False)
         if is_prefill:
             # one logit row per sequence: the last prompt token
             last = get_context().cu_seqlens_q[1:] - 1

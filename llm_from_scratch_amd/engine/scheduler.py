@@ -9,7 +9,10 @@ Behavioural fixes (the reference's bugs are not copied):
     with the freed blocks (the reference, :53-54, drops it);
   * ``max_tokens`` stops a sequence after exactly ``max_tokens`` completion
     tokens (the reference's ``1 + num_completion_tokens`` test, :89, stops
-    one token early).
+    one token early);
+  * a preempted sequence that grew past ``max_num_batched_tokens`` is
+    resumed (the reference's test at :33-34 never admits it again, and it
+    blocks the queue behind it).
 """
 from __future__ import annotations
 
@@ -44,8 +47,11 @@ class Scheduler:
         num_tokens = 0
         while self.waiting and len(scheduled) < self.max_num_sequences:
             seq = self.waiting[0]
+            # a preempted sequence that outgrew the budget while decoding comes
+            # back alone (the runner prefills it in parts)
+            outgrew = not scheduled and seq.num_completion_tokens > 0
             if (self.block_manager.can_allocate(seq)
-                    and len(seq) + num_tokens <= self.max_num_batched_tokens):
+                    and (len(seq) + num_tokens <= self.max_num_batched_tokens or outgrew)):
                 self.waiting.popleft()
                 self.block_manager.allocate(seq)
                 seq.status = SequenceStatus.RUNNING

@@ -9,7 +9,7 @@ from llm_from_scratch_amd.decode_model import DecodeModelConfig
 from llm_from_scratch_amd.engine import BlockManager, SamplingParams, Scheduler, Sequence
 from llm_from_scratch_amd.engine.block_manager import Block
 from llm_from_scratch_amd.engine.llm_engine import check_window
-from llm_from_scratch_amd.engine.model_runner import ModelRunner
+from llm_from_scratch_amd.engine.model_runner import ModelRunner, prefill_metadata, prefill_parts
 
 BS = 16
 
@@ -363,7 +363,7 @@ def test_the_queues_stand_when_the_pool_is_too_small():
     assert sched.schedule() == ([seqs[1]], False)
 
 
-@pytest.mark.parametrize("budget", [10 ** 6])
+@pytest.mark.parametrize("budget", [10 ** 6, 128, 40])
 def test_streams_of_any_lengths_finish_or_the_pool_is_full(budget):
     """Random lengths, windows, pools and forks: every sequence finishes, or no
     running one fits the pool or has a block to go on with."""
@@ -395,3 +395,60 @@ def test_streams_of_any_lengths_finish_or_the_pool_is_full(budget):
             raise AssertionError("no end")
         ended += sched.is_finished()
     assert ended > 75
+
+
+def test_a_sequence_past_the_token_budget_is_resumed():
+    """Preempted with more tokens than a prefill takes, it comes back alone,
+    and those behind it after it; a fresh prompt past the budget still waits."""
+    sched = Scheduler(8, 128, 10, BS, eos=-1, sliding_window=32)
+    seqs = [Sequence([i] * n, SamplingParams(max_tokens=60)) for i, n in enumerate([111, 15, 33, 123])]
+    for s in seqs:
+        sched.add_sequence(s)
+    drive(sched, seqs)
+    sched = Scheduler(8, 128, 20, BS, eos=-1)
+    old, other, fresh = Sequence([1] * 120, SamplingParams(max_tokens=60)), Sequence([2] * 9), Sequence([3] * 129)
+    sched.add_sequence(old)
+    for _ in range(30):
+        ran, _ = sched.schedule()
+        sched.postprocess(ran, [5])
+    sched.running.remove(old)
+    sched.preempt(old)
+    sched.add_sequence(other)
+    sched.add_sequence(fresh)
+    assert old.num_tokens == 150 and sched.schedule() == ([old], True)
+    sched.postprocess([old], [5])
+    assert sched.schedule() == ([other], True)
+    sched.postprocess([other], [5])
+    ran, prefill = sched.schedule()
+    assert ran == [old, other] and not prefill and list(sched.waiting) == [fresh]
+
+
+@pytest.mark.parametrize("budget", [1, 16, 40, 64, 1000])
+@pytest.mark.parametrize("n,shared", [(33, 0), (200, 0), (208, 0), (209, 96)])
+def test_parts_of_a_resumed_prefill(budget, n, shared):
+    """The parts together are the whole prefill: its tokens, positions and
+    slots, each behind those before it, whole blocks within the budget."""
+    bm = BlockManager(64, BS)
+    prompt = [i % 91 for i in range(n)]
+    other = Sequence(prompt[:shared] + [5])
+    bm.allocate(other)
+    s = Sequence(prompt[:20])
+    for t in prompt[20:]:
+        s.append_token(t)
+    bm.allocate(s)
+    assert s.num_cached_tokens == shared
+    parts = prefill_parts([s], BS, budget)
+    whole = prefill_metadata([s], BS)
+    each = [prefill_metadata(p, BS) for p in parts]
+    for key in ("input_ids", "positions", "slot_mapping"):
+        assert sum((m[key] for m in each), []) == whole[key]
+    at = shared
+    for i, m in enumerate(each):
+        size = len(m["input_ids"])
+        assert size <= max(budget, BS) and (size % BS == 0 or i == len(each) - 1)
+        at += size
+        assert m["cu_seqlens_q"] == [0, size] and m["cu_seqlens_k"] == [0, at]
+        assert parts[i][0].block_table == s.block_table[:-(-at // BS)]
+    assert s.num_tokens == n and len(s.block_table) == s.num_blocks  # as it was
+    fresh = Sequence(prompt)
+    assert prefill_parts([fresh], BS, budget) == [[fresh]] and prefill_parts([s, fresh], BS, budget) == [[s, fresh]]

@@ -15,6 +15,7 @@ import torch
 from llm_from_scratch_amd.context import reset_context
 from llm_from_scratch_amd.decode_model import DecodeModel, DecodeModelConfig
 from llm_from_scratch_amd.engine import BlockManager, LLMEngine, ModelRunner, Sampler, SamplingParams, Sequence
+from llm_from_scratch_amd.engine.model_runner import prefill_parts
 from oracle import paged_kv as P
 
 pytestmark = pytest.mark.gpu
@@ -229,3 +230,43 @@ def test_a_stream_outgrows_its_pool():
     eng = engine(num_kv_blocks=20)
     out = eng.generate([PROMPTS[0]], SamplingParams(top_k=20, max_tokens=490))["token_ids"][0]
     assert len(out) == 490
+
+
+@torch.inference_mode()
+def test_parts_of_a_resumed_prefill_teacher_forced():
+    """A sequence longer than the token budget, prefilled in parts: every layer
+    of every part, over the keys that the parts before it left in the pool."""
+    model = model_of(CFG, 6)
+    runner = ModelRunner(model, CFG.runner_config(block_size=BS, num_kv_blocks=40, enforce_eager=True,
+                                                  max_num_batched_tokens=72))
+    rng = np.random.default_rng(2)
+    s = Sequence(rng.integers(0, 1024, 9).tolist())
+    for t in rng.integers(0, 1024, 250).tolist():
+        s.append_token(t)
+    BlockManager(40, BS, CFG.sliding_window, CFG.num_sink_tokens).allocate(s)
+    parts = prefill_parts([s], BS, runner.token_budget())
+    assert [p[0].num_tokens for p in parts] == [64, 128, 192, 256, 259]
+    for part in parts:
+        model.trace = {}
+        runner.run_model(*runner.prepare_prefill(part), True)
+        reset_context()
+        pos = list(range(part[0].num_cached_tokens, part[0].num_tokens))
+        check_layers(model, CFG, part, [pos], [s.block_table])
+
+
+def test_streams_past_the_token_budget_are_resumed():
+    """Streams of 200 tokens in a pool of 224, 64 tokens a prefill: all finish,
+    and no prefill but of whole blocks within the budget."""
+    eng = engine(num_kv_blocks=14, max_num_batched_tokens=64, enforce_eager=True)
+    run_model, sizes, resumed = eng.model_runner.run_model, [], []
+
+    def noted(ids, positions, is_prefill):
+        if is_prefill:
+            sizes.append(ids.numel())
+            resumed.append(int(positions[0]) > 0)
+        return run_model(ids, positions, is_prefill)
+
+    eng.model_runner.run_model = noted
+    out = eng.generate([p[:60] for p in PROMPTS], SamplingParams(top_k=20, max_tokens=200))["token_ids"]
+    assert [len(t) for t in out] == [200] * 4
+    assert max(sizes) <= 64 and any(resumed)
