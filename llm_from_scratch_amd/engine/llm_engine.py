@@ -15,6 +15,7 @@ from typing import Optional, Sequence as Seq, Union
 
 import torch
 
+from .. import kernels
 from .model_runner import ModelRunner
 from .scheduler import Scheduler
 from .sequence import SamplingParams, Sequence
@@ -22,13 +23,17 @@ from .sequence import SamplingParams, Sequence
 
 def check_window(model: torch.nn.Module, window: Optional[int], sinks: int) -> None:
     """The engine frees the blocks behind ``window`` but the first ``sinks``
-    tokens': none of the model's attention layers may still see them."""
+    tokens': none of the model's attention layers may still see them.  Those
+    are the modules that the runner gives their share of the pool; one without
+    a ``window`` of its own sees everything."""
     if window is None:
         return
+    kernels._window_args(window, sinks)
     for name, m in model.named_modules():
-        if hasattr(m, "k_cache") and hasattr(m, "window"):
-            if m.window is None or m.window > window or m.sinks > sinks:
-                raise ValueError(f"{name} sees a window of {m.window} and {m.sinks} first tokens, but the engine keeps "
+        if hasattr(m, "k_cache") and hasattr(m, "v_cache"):
+            seen, first = getattr(m, "window", None), getattr(m, "sinks", 0)
+            if seen is None or seen > window or first > sinks:
+                raise ValueError(f"{name} sees a window of {seen} and {first} first tokens, but the engine keeps "
                                  f"{window} and {sinks}")
 
 

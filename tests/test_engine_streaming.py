@@ -452,3 +452,30 @@ def test_parts_of_a_resumed_prefill(budget, n, shared):
     assert s.num_tokens == n and len(s.block_table) == s.num_blocks  # as it was
     fresh = Sequence(prompt)
     assert prefill_parts([fresh], BS, budget) == [[fresh]] and prefill_parts([s, fresh], BS, budget) == [[s, fresh]]
+
+
+def test_a_layer_that_knows_no_window_is_refused():
+    """Layers that the runner gives a pool are those whose blocks are freed: one
+    without a window of its own sees everything."""
+    class Plain(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.k_cache = self.v_cache = torch.empty(0)
+
+    class Windowed(Plain):
+        window, sinks = 64, 4
+
+    class NoSinks(Plain):
+        window = 64
+
+    class Projection(torch.nn.Module):  # no pool: not asked
+        window = None
+
+    model = torch.nn.Sequential(Projection(), Windowed(), Plain())
+    check_window(model, None, 0)
+    with pytest.raises(ValueError, match="2 sees a window of None"):
+        check_window(model, 64, 4)
+    check_window(torch.nn.Sequential(Projection(), Windowed(), NoSinks()), 64, 4)
+    for bad in ((0, 0), (-1, 0), (64, -1)):
+        with pytest.raises(ValueError, match="window must be >= 1"):
+            check_window(torch.nn.Sequential(), *bad)
