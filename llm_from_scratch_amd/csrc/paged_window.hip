@@ -204,8 +204,9 @@ extern "C" int lfs_paged_decode_window(const void* q, const void* k_cache, const
   if (window_balanced(B, units, cus, tiles, G)) {
     const BalancedGeom bg = balanced_geom(Hkv);
     const int64_t rows = ((int64_t)bg.nwg + B * bg.ngroups) * bg.wpg * G;
-    LFS_REQUIRE((int64_t)bg.ngroups * B * (((int64_t)max_blocks * BS + tile - 1) / tile + 2) < (1ll << 31),
-                "paged_decode_window: too many context tiles for the balanced split");
+    const int64_t first = std::min<int64_t>(sinks, (int64_t)max_blocks * BS);  // of a sequence: the sinks' tiles, the window's
+    LFS_REQUIRE((int64_t)bg.ngroups * B * ((first + tile - 1) / tile + tiles) < (1ll << 31),
+                "paged_decode_window: too many visible tiles for the balanced split");
     float* ws_o = (float*)workspace;
     float* ws_ml = ws_o + rows * D;
     int* tp = (int*)(ws_ml + rows * 2);

@@ -356,3 +356,27 @@ def test_refusals():
         K.paged_attention_decode(q.float(), kc, kc, cl, bt, window=4)
     with pytest.raises(ValueError, match="GPU only"):
         K.paged_attention_decode(q.cpu(), kc, kc, cl, bt, window=4)
+
+
+def test_decode_tables_wider_than_any_window():
+    """What counts against the balanced split is what is seen, not the table's
+    width: 8192 rows of 32768 blocks, a few contexts of millions of tokens."""
+    rng = np.random.default_rng(51)
+    B, Hq, Hkv, D, BS, NB, width, window, sinks = 8192, 8, 8, 64, 256, 100, 32768, 4096, 4
+    kc, vc, q = bf16(rng, NB, BS, Hkv, D), bf16(rng, NB, BS, Hkv, D), bf16(rng, B, Hq, D)
+    lens = rng.integers(0, 300, B)
+    far = {0: width * BS, 17: width * BS - 1, 4000: 5000001, 8191: 70000}
+    bt = torch.full((B, width), -1, dtype=torch.int32, device=DEV)
+    bt[:, :2] = torch.from_numpy(rng.integers(0, NB, (B, 2)).astype(np.int32)).to(DEV)
+    for b, n in far.items():
+        lens[b] = n
+        lo, hi = (n - window) // BS, -(-n // BS)
+        bt[b, lo:hi] = torch.from_numpy(rng.integers(0, NB, hi - lo).astype(np.int32)).to(DEV)
+    o = K.paged_attention_decode(q, kc, vc, torch.from_numpy(lens).to(DEV), bt, window=window, sinks=sinks)
+    for b in list(far) + [1, 2, 3, 5000, 8190]:
+        n = int(lens[b])
+        t = np.r_[0:min(sinks, max(0, n - window)), max(0, n - window):n]
+        ids = bt[b].cpu().numpy()[t // BS]
+        k, v = (f64(c[torch.from_numpy(ids).long().to(DEV), torch.from_numpy(t % BS).to(DEV)]) for c in (kc, vc))
+        want = P.window_attention(f64(q[b:b + 1]), k, v, [len(t)], 0.125, 10 ** 9, 0)
+        close(o[b:b + 1], want if n else (np.zeros(1), np.zeros(1)), f"row {b}, context {n}")
