@@ -192,3 +192,35 @@ def test_no_rows_and_refusals():
                           ((x, one, one), dict(min_p=one.cpu()), ValueError), ((x[:, :0], one, one), {}, ValueError)):
         with pytest.raises(err):
             K.sample_filtered(*args, **kw)
+
+
+@pytest.mark.parametrize("filters", ["", "k", "p", "m", "kpm"])
+def test_several_values_past_16_bit_counts(filters):
+    """Rows in which a value that is not the shared one has more tokens than 16
+    bits count: above the others and below, of either sign, both signs of one
+    value (the halves of one word), -0 beside +0, values that are never drawn.
+    (p and the values put no border on a token: p n and m / w are no whole
+    numbers and no ratios of weights.)"""
+    rng = np.random.default_rng(61)
+    inf, low = float("inf"), float(torch.finfo(torch.bfloat16).min)
+    rows = [  # (value, tokens); the rest of a row is random
+        [(3.0, 75000), (1.5, 75001)], [(-2.0, 75000), (-2.5, 75001)], [(2.0, 75001), (-2.0, 75000)],
+        [(0.0, 75000), (-0.0, 75001)], [(-0.0, 75001), (0.0, 75000)], [(1.0, 70000), (0.5, 70000)],
+        [(float("nan"), 70000), (0.25, 70000)], [(-inf, 70000), (-1.0, 70000)], [(low, 70000), (2.0, 70000)],
+        [(2.0, 70000), (low, 70000)], [(88.0, 66000), (87.5, 65537)], [(inf, 70000), (5.0, 70000)]]
+    wide = [[(0.75, 90000), (1.25, 66000), (-1.25, 66000)], [(-3.0, 90000), (-0.5, 66000), (0.5, 70000)],
+            [(4.0, 90000), (0.0, 66000), (-0.0, 66000)], [(-inf, 90000), (float("nan"), 66000), (-1.0, 70000)]]
+    for V, batch in ((150001, rows), (230003, wide)):
+        x = rng.standard_normal((len(batch), V)).astype(np.float32)
+        for b, values in enumerate(batch):
+            # the first value's tokens at the front too, where the samples' first lanes find it
+            at, first = np.r_[np.arange(9000), 9000 + rng.permutation(V - 9000)], 0
+            for value, n in values:
+                x[b, at[first:first + n]] = value
+                first += n
+        logits = torch.from_numpy(x).to(DEV).to(torch.bfloat16)
+        B = len(batch)
+        run(logits, rng.uniform(0.6, 1.4, B), rng.random(B, np.float32),
+            rng.choice([1, 7001, 70011, 80001, 140001], B) if "k" in filters else None,
+            rng.choice([0.137, 0.533, 0.911, 0.9993], B) if "p" in filters else None,
+            rng.choice([1e-5, 0.013, 0.77], B) if "m" in filters else None)
