@@ -380,3 +380,62 @@ def test_decode_tables_wider_than_any_window():
         k, v = (f64(c[torch.from_numpy(ids).long().to(DEV), torch.from_numpy(t % BS).to(DEV)]) for c in (kc, vc))
         want = P.window_attention(f64(q[b:b + 1]), k, v, [len(t)], 0.125, 10 ** 9, 0)
         close(o[b:b + 1], want if n else (np.zeros(1), np.zeros(1)), f"row {b}, context {n}")
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,BS,window,sinks", [(45, 12, 4, 64, 16, 810, 4), (47, 32, 8, 128, 16, 790, 33),
+                                                       (70, 8, 8, 64, 16, 520, 0), (33, 8, 4, 64, 64, 4100, 70),
+                                                       (45, 12, 4, 64, 16, 810, 1500)])
+def test_decode_long_windows_over_freed_blocks(B, Hq, Hkv, D, BS, window, sinks):
+    """The equal share of all visible tiles per workgroup as the engine runs it:
+    blocks behind the window freed (-1), NaN in everything hidden; then with
+    entries outside the pool among the visible ones, which are skipped."""
+    rng = np.random.default_rng(B + sinks)
+    lens = rng.integers(0, 3 * window, B)
+    lens[:7] = 0, 1, window, window + 1, window + sinks, window + BS, 3 * window
+    kc, vc, bt, seqs = paged(rng, lens.tolist(), (lens - window).tolist(), BS, Hkv, D, sinks)
+    q = bf16(rng, B, Hq, D)
+    cl = torch.from_numpy(lens).to(DEV)
+    table = bt.cpu().numpy()
+    assert (table[6] == -1).sum() > 5
+    for bad in (False, True):
+        if bad:
+            seen = np.argwhere(table >= 0)
+            gone = seen[rng.permutation(len(seen))[:len(seen) // 5]]
+            table[gone[:, 0], gone[:, 1]] = np.where(np.arange(len(gone)) % 2, -1, len(kc) + 3)
+            bt = torch.from_numpy(table).to(DEV)
+        o, oq, os_ = K.paged_attention_decode(q, kc, vc, cl, bt, 0.1, quant=True, window=window, sinks=sinks)
+        assert torch.equal(o, K.paged_attention_decode(q, kc, vc, cl, bt, 0.1, window=window, sinks=sinks))
+        wq, ws = K.act_quant(o.view(B, -1))
+        assert torch.equal(oq.view(torch.uint8), wq.view(torch.uint8)) and torch.equal(os_, ws)
+        for b, (n, (k, v)) in enumerate(zip(lens.tolist(), seqs)):
+            t = np.arange(n)
+            ids = table[b][t // BS]
+            t = t[((t >= n - window) | (t < sinks)) & (ids >= 0) & (ids < len(kc))]
+            want = P.window_attention(f64(q[b:b + 1]), k[t], v[t], [len(t)], 0.1, 10 ** 9, 0) if len(t) else (np.zeros(1), np.zeros(1))
+            close(o[b:b + 1], want, f"row {b}, context {n}")
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,BS,window,sinks", [(1, 12, 4, 64, 256, 64, 4096), (3, 32, 8, 128, 16, 17, 1000),
+                                                       (2, 8, 8, 64, 48, 1, 333), (5, 8, 1, 128, 64, 1000, 2000),
+                                                       (90, 12, 4, 64, 16, 40, 700)])
+def test_many_sinks_before_a_short_window(B, Hq, Hkv, D, BS, window, sinks):
+    """A long beginning that stays visible: contexts inside it, at its end and
+    past it, in the decode and as a chunk of new tokens."""
+    rng = np.random.default_rng(B + sinks)
+    lens = rng.integers(1, 2 * sinks, B)
+    lens[:4] = [sinks + window + 40, sinks, sinks + 1, sinks // 2][:min(B, 4)]
+    new = np.minimum(lens, 70)
+    kc, vc, bt, seqs = paged(rng, lens.tolist(), (lens - new - window + 1).tolist(), BS, Hkv, D, sinks)
+    q = bf16(rng, B, Hq, D)
+    o = K.paged_attention_decode(q, kc, vc, torch.from_numpy(lens).to(DEV), bt, window=window, sinks=sinks)
+    cq, ck = (torch.from_numpy(np.concatenate([[0], np.cumsum(x)]).astype(np.int32)).to(DEV) for x in (new, lens))
+    pq = bf16(rng, int(new.sum()), Hq, D)
+    po = K.flash_attn_varlen_func(pq, kc, vc, cq, ck, int(new.max()), int(lens.max()), block_table=bt, window=window,
+                                  sinks=sinks)
+    at = 0
+    for b, (n, m, (k, v)) in enumerate(zip(lens.tolist(), new.tolist(), seqs)):
+        close(o[b:b + 1], P.window_attention(f64(q[b:b + 1]), k, v, [n - 1], D ** -0.5, window, sinks), f"context {n}")
+        if b < 8:
+            close(po[at:at + m], P.window_attention(f64(pq[at:at + m]), k, v, np.arange(n - m, n), D ** -0.5, window,
+                                                    sinks), f"{m} new of {n}")
+        at += m
