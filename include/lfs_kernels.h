@@ -397,7 +397,8 @@ int lfs_prefill_attention_window(const void* q, const void* k, const void* v, co
  * lfs_paged_decode over a sliding window with sinks: with L =
  * context_lens[b] tokens, the newest at L - 1, the tokens t < L with t >= L -
  * window or t < sinks.  Hidden tokens are never read: the table entries of
- * blocks that hold only such tokens may be -1.  workspace: at least
+ * blocks that hold only such tokens may be -1.  Visible keys and values must be
+ * finite.  workspace: at least
  * lfs_paged_decode_window_workspace_bytes(...) bytes, sized on the device that
  * runs the call, 16-byte aligned.  q_out / q_scale as for lfs_paged_decode.  window >= 1,
  * sinks >= 0.  The grid depends only on the shapes and the window.

@@ -150,7 +150,8 @@ __global__ __launch_bounds__(256) void qk_head_norm_rope_store_rows(HeadNorm a) 
 // Tokens from which a wave takes a whole token.  A thread per chunk / a wave per
 // token, us: 32 / 8 heads of 128, 128 tokens 2.9 / 6.3, 1024 8.3 / 9.2, 2048
 // 12.2 / 12.2, 4096 20.2 / 19.8, 16383 97 / 73.6; 12 / 4 of 64, 128 tokens
-// 2.6 / 3.1, 2048 4.5 / 4.3, 4096 7.9 / 7.2, 16383 19.4 / 20.5.
+// 2.6 / 3.1, 2048 4.5 / 4.3, 4096 7.9 / 7.2, 16383 19.4 / 20.5 (one number for
+// all shapes: the wrong side costs 6 % there).
 constexpr int64_t kHeadRowsT = 2048;
 
 }  // namespace

@@ -101,7 +101,9 @@ class Sampler:
 
     With any of ``top_k`` (int32 [B]), ``top_p`` and ``min_p`` (fp32 [B]) the
     tokens come from kernels.sample_filtered instead, on uniform numbers of
-    torch's generator with the same seed and an offset that advances alike."""
+    torch's generator with the same seed and an offset that advances alike;
+    this goes for every row, so a row without filters draws another token there
+    than in a batch where no row has one."""
 
     def __init__(self):
         self._seed: Optional[int] = None

@@ -555,7 +555,7 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     With ``window`` (>= 1) a token sees only the last ``window`` tokens of
     its context, itself among them, and the first ``sinks`` ones; the others
     are never read, and table entries of blocks that hold no visible token
-    may be -1.  The kernel then splits the work itself (``blocks_per_split``
+    may be -1; visible keys and values must be finite.  The kernel then splits the work itself (``blocks_per_split``
     must be None); a ``workspace`` takes
     ``paged_decode_window_workspace_bytes`` bytes.
     """
