@@ -11,8 +11,8 @@ Behavioural fixes (the reference's bugs are not copied):
     tokens (the reference's ``1 + num_completion_tokens`` test, :89, stops
     one token early);
   * a preempted sequence that grew past ``max_num_batched_tokens`` is
-    resumed (the reference's test at :33-34 never admits it again, and it
-    blocks the queue behind it).
+    resumed (asked for its whole length within the budget, it would wait at
+    the queue's head for good).
 """
 from __future__ import annotations
 
