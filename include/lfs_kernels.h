@@ -119,7 +119,7 @@
 extern "C" {
 #endif
 
-#define LFS_ABI_VERSION 18
+#define LFS_ABI_VERSION 19
 
 /* argument errors (negative); launch errors are positive hipError_t values */
 #define LFS_EINVAL (-1)
@@ -686,6 +686,93 @@ int64_t lfs_scatter_add_weighted_workspace_bytes(int64_t n, int64_t num_tokens);
 int lfs_scatter_add_weighted(const void* x, int32_t x_is_f32, int64_t ldx, const void* weights,
                              int32_t w_is_f32, const int64_t* token_idx, int64_t n, int64_t num_tokens,
                              int32_t d, void* y, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------- KV pool in 8 bits */
+
+/*
+ * A pool in 8 bits: codes e4m3fn [num_blocks, block_size, Hkv, D] and scales
+ * fp32 [num_blocks, Hkv, block_size], one per token and kv head.
+ *
+ * store_kvcache_fp8, for tokens t with 0 <= slot_mapping[t] <
+ * num_blocks * block_size (others are skipped), per kv head of key and value
+ * (bf16 [T, Hkv, D], heads and dims contiguous, any token stride):
+ *   s = max(amax over the head's D values, 1e-4) * fp32(1/448),
+ *   code = e4m3fn(clamp(x / s, -448, 448))
+ * as lfs_act_quant with a group of D.  Two tokens of one slot leave either's
+ * values.  D = 64 or 128; caches 8-byte aligned.
+ */
+int lfs_store_kvcache_fp8(const void* key, int64_t k_stride_t, const void* value, int64_t v_stride_t,
+                          void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                          const int64_t* slot_mapping, int64_t T, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t block_size, int64_t num_blocks, void* stream);
+
+/*
+ * load_kvcache_fp8: the cached rows as bf16(code * s): row cu_seqlens[i] + t
+ * of k and v (bf16 [total, Hkv, D]) is position t of sequence i, through
+ * block_tables[i].  Positions without a valid block, and rows of no sequence,
+ * are zeros.  cu_seqlens int32 [B + 1], non-decreasing.  D = 64 or 128; all
+ * 16-byte aligned but the scales.
+ */
+int lfs_load_kvcache_fp8(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                         const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                         const int32_t* cu_seqlens, int64_t B, int64_t total, void* k, void* v,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int64_t num_blocks,
+                         void* stream);
+
+/*
+ * paged_decode_fp8: lfs_paged_decode over such a pool (keys code * k_scale,
+ * values code * v_scale, fp32), which splits the work itself.  Codes and scales
+ * of visible tokens must be finite.  k_scale and v_scale 16-byte aligned; a
+ * workspace of lfs_paged_decode_fp8_workspace_bytes bytes, 16-byte aligned.
+ */
+int64_t lfs_paged_decode_fp8_workspace_bytes(int64_t B, int32_t num_q_heads, int32_t head_dim);
+int lfs_paged_decode_fp8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                         const float* v_scale, const int64_t* context_lens, const int32_t* block_tables,
+                         int64_t bt_stride, void* out, void* workspace, int64_t workspace_bytes, int64_t B,
+                         int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                         int64_t num_blocks, int32_t max_blocks, float scale, void* q_out, float* q_scale,
+                         void* stream);
+
+/*
+ * paged_decode_shared: lfs_paged_decode for a batch in groups whose sequences
+ * have their first blocks in common, which are then read once a group.  Rows
+ * cu_groups[g] .. cu_groups[g + 1] - 1 (int32 [num_groups + 1], non-decreasing)
+ * are group g; the first shared_blocks[g] (int32) entries of their block tables
+ * must be equal.  Rows of no group share nothing; a context may end within the
+ * shared blocks.  A workspace of lfs_paged_decode_shared_workspace_bytes bytes,
+ * 16-byte aligned.
+ */
+int64_t lfs_paged_decode_shared_workspace_bytes(int64_t B, int64_t num_groups, int32_t num_q_heads,
+                                                int32_t num_kv_heads, int32_t head_dim);
+int lfs_paged_decode_shared(const void* q, const void* k_cache, const void* v_cache, const int64_t* context_lens,
+                            const int32_t* block_tables, int64_t bt_stride, const int32_t* cu_groups,
+                            const int32_t* shared_blocks, int64_t num_groups, void* out, void* workspace,
+                            int64_t workspace_bytes, int64_t B, int32_t num_q_heads, int32_t num_kv_heads,
+                            int32_t head_dim, int32_t block_size, int64_t num_blocks, int32_t max_blocks,
+                            float scale, void* q_out, float* q_scale, void* stream);
+
+/* ---------------------------------------------------- logits of a batch */
+
+/*
+ * apply_penalties, for row b of logits (bf16, or fp32 with is_f32, [B, V], row
+ * stride ld) with the history tokens[b][0 .. seq_lens[b]) (int32 [B, width],
+ * lengths int32 [B]), of which the first prompt_lens[b] are the prompt's; c(v)
+ * counts token v among the others, seen(v): it is in the history.  In fp32:
+ *   x = seen(v) ? (x > 0 ? x / repetition[b] : x * repetition[b]) : x
+ *   x = x - frequency[b] * c(v) - presence[b] * [c(v) > 0]
+ *   x = x + bias[b][i] for each i with bias_ids[b][i] == v, in order
+ *   x = -infinity unless bit v % 32 of allowed[b][v / 32] is set
+ * rounded once to the logits' type, to out (row stride ld_out, may be logits).
+ * Token ids outside [0, V) are ignored.  Each of repetition, presence and
+ * frequency (fp32 [B]), the lists (int32 and fp32 [B, num_biases], at most 1024
+ * a row), allowed (int32, ceil(V / 32) words a row) and, without penalties,
+ * tokens, prompt_lens and seq_lens may be NULL.
+ */
+int lfs_apply_penalties(const void* logits, int64_t ld, void* out, int64_t ld_out, int32_t is_f32,
+                        const int32_t* tokens, int64_t tokens_stride, int32_t width, const int32_t* prompt_lens,
+                        const int32_t* seq_lens, const float* repetition, const float* presence,
+                        const float* frequency, const int32_t* bias_ids, const float* bias, int32_t num_biases,
+                        const int32_t* allowed, int64_t allowed_stride, int64_t B, int32_t V, void* stream);
 
 #ifdef __cplusplus
 }

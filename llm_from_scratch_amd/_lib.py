@@ -11,7 +11,7 @@ import ctypes
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "liblfs_kernels.so"
-ABI_VERSION = 18
+ABI_VERSION = 19
 # size of the library's static paged-decode workspace (LFS_DECODE_SCRATCH_BYTES)
 DECODE_SCRATCH_BYTES = 64 << 20
 
@@ -85,6 +85,19 @@ SIGNATURES = {
     "lfs_sample_filtered": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_p,
                                            _c_p]),
     "lfs_copy_kv_blocks": (ctypes.c_int, [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p]),
+    "lfs_store_kvcache_fp8": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32,
+                                             _c_i32, _c_i32, _c_i64, _c_p]),
+    "lfs_load_kvcache_fp8": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i64, _c_p,
+                                            _c_p, _c_i32, _c_i32, _c_i32, _c_i64, _c_p]),
+    "lfs_paged_decode_fp8_workspace_bytes": (ctypes.c_int64, [_c_i64, _c_i32, _c_i32]),
+    "lfs_paged_decode_fp8": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i64,
+                                            _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_f, _c_p, _c_p, _c_p]),
+    "lfs_paged_decode_shared_workspace_bytes": (ctypes.c_int64, [_c_i64, _c_i64, _c_i32, _c_i32, _c_i32]),
+    "lfs_paged_decode_shared": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p, _c_p,
+                                               _c_i64, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32, _c_i64, _c_i32, _c_f,
+                                               _c_p, _c_p, _c_p]),
+    "lfs_apply_penalties": (ctypes.c_int, [_c_p, _c_i64, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_p, _c_p,
+                                           _c_p, _c_p, _c_p, _c_p, _c_i32, _c_p, _c_i64, _c_i64, _c_i32, _c_p]),
     "lfs_moe_align_tiles": (ctypes.c_int64, [_c_i64, _c_i32, _c_i32, _c_i32]),
     "lfs_moe_align": (ctypes.c_int, [_c_p, _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_p, _c_i64, _c_p,
                                      _c_p, _c_i64, _c_p]),

@@ -22,6 +22,17 @@ Same names, arguments and return values as the reference's operators:
       temperature, top-k, top-p and min-p sampling from given random numbers
   copy_kv_blocks(kv_cache, src, dst)
       blocks of the KV pool copied to others
+  store_kvcache_fp8(key, value, k_cache, v_cache, k_scale, v_scale,
+                    slot_mapping)
+  load_kvcache_fp8(k_cache, v_cache, k_scale, v_scale, block_tables,
+                   cu_seqlens, total) -> (k, v)
+      a KV pool in 8 bits written and read back; paged_attention_decode takes
+      it with its scales
+  paged_attention_decode_shared(q, k_cache, v_cache, context_lens,
+                                block_tables, cu_groups, shared_blocks) -> o
+      decode for groups of sequences whose first blocks are the same ones
+  apply_penalties(logits, tokens, prompt_lens, seq_lens, ...) -> logits
+      penalties for repeated tokens, biases and a mask of allowed tokens
   qk_head_norm_rope_store(...) -> q
       per-head norms, rotation and KV slot write
   sample_gumbel(logits, temperatures, seed, offset) -> tokens
@@ -427,6 +438,81 @@ def copy_kv_blocks(kv_cache: torch.Tensor, src, dst) -> None:
             _ptr(kv_cache), planes, NB, block, s.buffer_info()[0], d.buffer_info()[0], len(s))
 
 
+def _fp8_pool(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+    """(NB, BS, Hkv, D) of a pool in 8 bits, checked."""
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if t.dtype is not FP8:
+            _dtype(t, FP8, n)
+        assert t.dim() == 4 and t.is_contiguous(), f"{n} must be contiguous [num_blocks, block_size, Hkv, D]"
+    NB, BS, Hkv, D = k_cache.shape
+    assert v_cache.shape == k_cache.shape, "k_cache and v_cache must have one shape"
+    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if t.dtype is not torch.float32:
+            _dtype(t, torch.float32, n)
+        assert t.shape == (NB, Hkv, BS) and t.is_contiguous(), f"{n} must be contiguous [num_blocks, Hkv, block_size]"
+    return NB, BS, Hkv, D
+
+
+def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """store_kvcache into a pool in 8 bits: every kv head of a token is
+    quantised as by act_quant, with a group of D: s = max(amax, 1e-4) *
+    fp32(1/448), code = e4m3fn(clamp(x / s, -448, 448)).
+
+    key/value: bf16 [T, Hkv, D], D 64 or 128 (heads and dims contiguous, any
+    token stride); caches e4m3fn [num_blocks, block_size, Hkv, D] and scales
+    fp32 [num_blocks, Hkv, block_size], contiguous; slot_mapping: int64 [T].
+    Slots outside the pool are skipped like -1; a slot may appear once."""
+    NB, BS, Hkv, D = _fp8_pool(k_cache, v_cache, k_scale, v_scale)
+    assert key.dim() == 3 and value.shape == key.shape and key.shape[1:] == (Hkv, D), "key and value must be [T, Hkv, D]"
+    assert key.stride(2) == value.stride(2) == 1 and key.stride(1) == value.stride(1) == D, \
+        "heads and dims of key and value must be contiguous"
+    T = key.size(0)
+    assert slot_mapping.shape == (T,) and slot_mapping.is_contiguous(), "slot_mapping must be contiguous [T]"
+    _on_gpu(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    if not (key.dtype is value.dtype is torch.bfloat16 and slot_mapping.dtype is torch.int64):
+        _dtype(key, torch.bfloat16, "key")
+        _dtype(value, torch.bfloat16, "value")
+        _dtype(slot_mapping, torch.int64, "slot_mapping")
+    _launch("store_kvcache_fp8", _lib.load().lfs_store_kvcache_fp8, key,
+            key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(), T, Hkv, D, BS, NB)
+
+
+def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     block_tables: torch.Tensor, cu_seqlens: torch.Tensor, total: int
+                     ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cached keys and values of a pool in 8 bits (store_kvcache_fp8) read back
+    as bf16(code * scale), one sequence behind the other: what
+    flash_attn_varlen_func takes without a block table.
+
+    block_tables: int32 [B, max_blocks]; cu_seqlens: int32 [B + 1], first 0: row
+    cu_seqlens[i] + t of the results is position t of sequence i; total: rows of
+    the results, bf16 [total, Hkv, D].  Positions without a block of the pool,
+    and rows past the last sequence, are zeros."""
+    NB, BS, Hkv, D = _fp8_pool(k_cache, v_cache, k_scale, v_scale)
+    assert block_tables.dim() == 2 and block_tables.stride(1) == 1, "block_tables must be [B, max_blocks]"
+    B, max_blocks = block_tables.shape
+    assert cu_seqlens.shape == (B + 1,) and cu_seqlens.is_contiguous(), "cu_seqlens must be contiguous [B + 1]"
+    if total < 0:
+        raise ValueError(f"total must be >= 0, got {total}")
+    _on_gpu(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens)
+    if not block_tables.dtype is cu_seqlens.dtype is torch.int32:
+        _dtype(block_tables, torch.int32, "block_tables")
+        _dtype(cu_seqlens, torch.int32, "cu_seqlens")
+    k, v = torch.empty(2, total, Hkv, D, dtype=torch.bfloat16, device=k_cache.device).unbind(0)
+    _launch("load_kvcache_fp8", _lib.load().lfs_load_kvcache_fp8, k_cache,
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+            _row_stride(block_tables), max_blocks, cu_seqlens.data_ptr(), B, total, k.data_ptr(), v.data_ptr(), Hkv, D,
+            BS, NB)
+    return k, v
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Stride between the rows of a matrix; a single row's is its width."""
+    return t.stride(0) if t.size(0) > 1 else t.size(1)
+
+
 BALANCED_MAX_BATCH = 8192  # the balanced split scans the batch's tile counts in LDS
 
 
@@ -534,7 +620,8 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                            context_lens: torch.Tensor, block_tables: torch.Tensor,
                            scale: Optional[float] = None, blocks_per_split: Optional[int] = None,
                            workspace: Optional[torch.Tensor] = None, quant: bool = False,
-                           window: Optional[int] = None, sinks: int = 0):
+                           window: Optional[int] = None, sinks: int = 0,
+                           k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
     """One decode step of GQA attention over a paged KV pool.
 
     q: bf16 [B, Hq, D]; caches bf16 [num_blocks, block_size, Hkv, D];
@@ -558,8 +645,18 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     may be -1; visible keys and values must be finite.  The kernel then splits the work itself (``blocks_per_split``
     must be None); a ``workspace`` takes
     ``paged_decode_window_workspace_bytes`` bytes.
+    With ``k_scale`` and ``v_scale`` (fp32 [num_blocks, Hkv, block_size]) the
+    caches are a pool in 8 bits (store_kvcache_fp8): keys and values are codes
+    times scales.  The kernel splits the work itself there too; a ``workspace``
+    takes ``paged_decode_fp8_workspace_bytes`` bytes; not with a ``window``.
     """
     windowed = _window_args(window, sinks)
+    if k_scale is not None or v_scale is not None:
+        assert k_scale is not None and v_scale is not None, "k_scale and v_scale go together"
+        if windowed:
+            raise ValueError("a window over a pool in 8 bits is not provided")
+        assert blocks_per_split is None, "blocks_per_split does not go with a pool in 8 bits"
+        return _decode_fp8(q, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables, scale, workspace, quant)
     assert q.dim() == 3 and q.is_contiguous(), "q must be contiguous [B, Hq, D]"
     assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_cache.shape == v_cache.shape
     assert k_cache.dim() == 4, "caches must be [num_blocks, block_size, Hkv, D]"
@@ -616,6 +713,111 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                                       B, Hq, Hkv, D, BS, NB, max_blocks, float(scale), bps,
                                       _ptr(oq), _ptr(os_), _stream(q))
     _lib.check(rc, "paged_attention_decode")
+    return (o, oq, os_) if quant else o
+
+
+def paged_decode_fp8_workspace_bytes(batch: int, num_q_heads: int, head_dim: int) -> int:
+    return int(_lib.load().lfs_paged_decode_fp8_workspace_bytes(batch, num_q_heads, head_dim))
+
+
+def paged_decode_shared_workspace_bytes(batch: int, num_groups: int, num_q_heads: int, num_kv_heads: int,
+                                        head_dim: int) -> int:
+    return int(_lib.load().lfs_paged_decode_shared_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads,
+                                                                   head_dim))
+
+
+@functools.lru_cache(maxsize=256)
+def _fp8_workspace(device: int, *shape: int) -> int:
+    """paged_decode_fp8_workspace_bytes on a device (by its number of CUs)."""
+    with torch.cuda.device(device):
+        return paged_decode_fp8_workspace_bytes(*shape)
+
+
+@functools.lru_cache(maxsize=256)
+def _shared_workspace(device: int, *shape: int) -> int:
+    with torch.cuda.device(device):
+        return paged_decode_shared_workspace_bytes(*shape)
+
+
+def _decode_args(q: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor, need: int,
+                 workspace: Optional[torch.Tensor], quant: bool):
+    """Checks of what a decode takes beside the pool; its workspace and outputs."""
+    B, Hq, D = q.shape
+    assert block_tables.dim() == 2 and block_tables.size(0) == B and block_tables.stride(1) == 1, \
+        "block_tables must be [B, max_blocks]"
+    assert context_lens.shape == (B,) and context_lens.is_contiguous(), "context_lens must be contiguous [B]"
+    if not (q.dtype is torch.bfloat16 and context_lens.dtype is torch.int64 and block_tables.dtype is torch.int32):
+        _dtype(q, torch.bfloat16, "q")
+        _dtype(context_lens, torch.int64, "context_lens")
+        _dtype(block_tables, torch.int32, "block_tables")
+    if workspace is not None:
+        _on_gpu(q, workspace)
+        assert workspace.is_contiguous(), "workspace must be contiguous"
+    elif need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    o, oq, os_ = torch.empty_like(q), None, None
+    if quant:
+        assert Hq * D % 128 == 0, "the quantised output needs Hq * D to be a multiple of 128"
+        oq = torch.empty(B, Hq * D, dtype=FP8, device=q.device)
+        os_ = torch.empty(B, Hq * D // 128, dtype=torch.float32, device=q.device)
+    return workspace, o, oq, os_
+
+
+def _decode_fp8(q, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables, scale, workspace, quant):
+    assert q.dim() == 3 and q.is_contiguous(), "q must be contiguous [B, Hq, D]"
+    NB, BS, Hkv, Dk = _fp8_pool(k_cache, v_cache, k_scale, v_scale)
+    B, Hq, D = q.shape
+    assert Dk == D, "head_dim mismatch between q and the caches"
+    _on_gpu(q, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables)
+    workspace, o, oq, os_ = _decode_args(q, context_lens, block_tables, _fp8_workspace(q.get_device(), B, Hq, D),
+                                         workspace, quant)
+    _launch("paged_attention_decode", _lib.load().lfs_paged_decode_fp8, q,
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            context_lens.data_ptr(), block_tables.data_ptr(), _row_stride(block_tables), o.data_ptr(), _ptr(workspace),
+            0 if workspace is None else workspace.nbytes, B, Hq, Hkv, D, BS, NB, block_tables.size(1),
+            1.0 / math.sqrt(D) if scale is None else scale, _ptr(oq), _ptr(os_))
+    return (o, oq, os_) if quant else o
+
+
+def paged_attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                  context_lens: torch.Tensor, block_tables: torch.Tensor, cu_groups: torch.Tensor,
+                                  shared_blocks: torch.Tensor, scale: Optional[float] = None,
+                                  workspace: Optional[torch.Tensor] = None, quant: bool = False):
+    """paged_attention_decode for a batch in groups whose sequences have their
+    first blocks in common (branches of one sequence, prompts behind one system
+    prompt): a group's shared blocks are read once for all of its sequences.
+
+    q, caches, context_lens and block_tables as there.  cu_groups: int32
+    [num_groups + 1], non-decreasing: rows cu_groups[g] .. cu_groups[g + 1] - 1
+    of the batch are group g (none, where equal); shared_blocks: int32
+    [num_groups]: as many first entries of their block tables are the same.
+    Rows of no group share nothing.  context_lens counts the shared tokens too,
+    and may end among them.  Returns what paged_attention_decode returns.  The
+    grid depends only on the shapes, so the call can be captured in a HIP graph,
+    with a ``workspace`` of ``paged_decode_shared_workspace_bytes`` bytes of its
+    own; the groups may change between replays."""
+    assert q.dim() == 3 and q.is_contiguous(), "q must be contiguous [B, Hq, D]"
+    assert k_cache.dim() == 4 and k_cache.is_contiguous() and v_cache.is_contiguous() \
+        and v_cache.shape == k_cache.shape, "caches must be contiguous [num_blocks, block_size, Hkv, D]"
+    B, Hq, D = q.shape
+    NB, BS, Hkv, Dk = k_cache.shape
+    assert Dk == D, "head_dim mismatch between q and the caches"
+    assert shared_blocks.dim() == 1 and shared_blocks.is_contiguous(), "shared_blocks must be contiguous [num_groups]"
+    NG = shared_blocks.size(0)
+    assert cu_groups.shape == (NG + 1,) and cu_groups.is_contiguous(), "cu_groups must be contiguous [num_groups + 1]"
+    _on_gpu(q, k_cache, v_cache, context_lens, block_tables, cu_groups, shared_blocks)
+    if not (k_cache.dtype is v_cache.dtype is torch.bfloat16 and cu_groups.dtype is shared_blocks.dtype is torch.int32):
+        _dtype(k_cache, torch.bfloat16, "k_cache")
+        _dtype(v_cache, torch.bfloat16, "v_cache")
+        _dtype(cu_groups, torch.int32, "cu_groups")
+        _dtype(shared_blocks, torch.int32, "shared_blocks")
+    workspace, o, oq, os_ = _decode_args(q, context_lens, block_tables,
+                                         _shared_workspace(q.get_device(), B, NG, Hq, Hkv, D), workspace, quant)
+    _launch("paged_attention_decode_shared", _lib.load().lfs_paged_decode_shared, q,
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(),
+            _row_stride(block_tables), cu_groups.data_ptr(), shared_blocks.data_ptr(), NG, o.data_ptr(),
+            _ptr(workspace), 0 if workspace is None else workspace.nbytes, B, Hq, Hkv, D, BS, NB, block_tables.size(1),
+            1.0 / math.sqrt(D) if scale is None else scale, _ptr(oq), _ptr(os_))
     return (o, oq, os_) if quant else o
 
 
@@ -918,6 +1120,85 @@ def sample_filtered(logits: torch.Tensor, temperatures: torch.Tensor, uniforms: 
 
 _SAMPLE_TYPES = (torch.float32, torch.float32, torch.int32, torch.float32, torch.float32)
 _SAMPLE_NAMES = ("temperatures", "uniforms", "top_k", "top_p", "min_p")
+
+
+def apply_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
+                    prompt_lens: Optional[torch.Tensor] = None, seq_lens: Optional[torch.Tensor] = None,
+                    repetition: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                    frequency: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
+                    bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Logits with penalties for the tokens of each row's history, biases and a
+    mask of allowed tokens: what goes to sample_gumbel or sample_filtered.
+
+    logits: bf16 or fp32 [B, V] (unit column stride).  Row b's history is
+    tokens[b, :seq_lens[b]] (int32 [B, L] and [B]), its first prompt_lens[b]
+    (int32 [B]) the prompt; c(v) counts token v among the others.  In fp32, each
+    step where its argument is given:
+      repetition (fp32 [B], > 0)  tokens of the history: x / r if x > 0, else x * r
+      frequency, presence (fp32 [B])  x - frequency * c(v) - presence * [c(v) > 0]
+      bias_ids, bias (int32 and fp32 [B, n], n <= 1024)  x + each of v's biases
+      allowed (int32 [B, ceil(V / 32)])  -infinity unless bit v % 32 of word
+                                         v / 32 is set
+    then one rounding to the logits' type.  Token ids outside [0, V) are ignored
+    (-1: none).  Returns a new tensor, or ``out`` (which may be ``logits``)."""
+    assert logits.dim() == 2 and logits.stride(1) == 1, "logits must be [B, V] with unit column stride"
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"logits must be torch.bfloat16 or torch.float32, got {logits.dtype}")
+    _on_gpu(logits)
+    B, V = logits.shape
+    dev, rows = logits.get_device(), [prompt_lens, seq_lens, repetition, presence, frequency]
+    for i, t in enumerate(rows):
+        if t is None:
+            continue
+        if t.get_device() != dev:
+            _on_gpu(logits, t)
+        if t.dtype is not _PENALTY_TYPES[i]:
+            _dtype(t, _PENALTY_TYPES[i], _PENALTY_NAMES[i])
+        assert t.shape == (B,), f"{_PENALTY_NAMES[i]} must be [B]"
+        if not t.is_contiguous():
+            rows[i] = t.contiguous()
+    if not (tokens is None) == (prompt_lens is None) == (seq_lens is None):
+        raise ValueError("tokens, prompt_lens and seq_lens go together")
+    if tokens is None and not repetition is presence is frequency is None:
+        raise ValueError("penalties need tokens, prompt_lens and seq_lens")
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids and bias go together")
+    for t, n, dt, width in ((tokens, "tokens", torch.int32, None), (bias_ids, "bias_ids", torch.int32, None),
+                            (bias, "bias", torch.float32, None if bias is None else bias_ids.size(-1)),
+                            (allowed, "allowed", torch.int32, -(-V // 32))):
+        if t is None:
+            continue
+        if t.get_device() != dev:
+            _on_gpu(logits, t)
+        if t.dtype is not dt:
+            _dtype(t, dt, n)
+        assert t.dim() == 2 and t.size(0) == B and (width is None or t.size(1) == width), \
+            f"{n} must be [B, {'n' if width is None else width}]"
+    if tokens is not None and tokens.stride(1) != 1:
+        tokens = tokens.contiguous()
+    if bias is not None:
+        bias_ids, bias = bias_ids.contiguous(), bias.contiguous()
+    if allowed is not None and allowed.stride(1) != 1:
+        allowed = allowed.contiguous()
+    if out is None:
+        out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
+    else:
+        if out.get_device() != dev:
+            _on_gpu(logits, out)
+        if out.dtype is not logits.dtype:
+            _dtype(out, logits.dtype, "out")
+        assert out.shape == logits.shape and out.stride(1) == 1, "out must be [B, V] with unit column stride"
+    _launch("apply_penalties", _lib.load().lfs_apply_penalties, logits,
+            logits.data_ptr(), _row_stride(logits), out.data_ptr(), _row_stride(out), logits.dtype is torch.float32,
+            _ptr(tokens), 0 if tokens is None else _row_stride(tokens), 0 if tokens is None else tokens.size(1),
+            *map(_ptr, rows), _ptr(bias_ids), _ptr(bias), 0 if bias is None else bias.size(1), _ptr(allowed),
+            0 if allowed is None else _row_stride(allowed), B, V)
+    return out
+
+
+_PENALTY_TYPES = (torch.int32, torch.int32, torch.float32, torch.float32, torch.float32)
+_PENALTY_NAMES = ("prompt_lens", "seq_lens", "repetition", "presence", "frequency")
 
 
 # ------------------------------------------------- fused decode-step rows --

@@ -101,3 +101,23 @@ def sample_filtered(logits, temperature, u, top_k=0, top_p=1.0, min_p=0.0):
     c = np.cumsum(w[:n])
     i = min(int(np.count_nonzero(c <= u * c[-1])), n - 1)
     return int(order[i]), e[i] - np.log(c[-1])
+
+
+def apply_penalties(logits, history, prompt_len, repetition=None, presence=0.0, frequency=0.0, biases=(), allowed=None):
+    """One row in 64 bits: repetition divides or multiplies the logits of the
+    history's tokens, frequency and presence count those past the prompt,
+    ``biases`` are (token, value) pairs, ``allowed`` truth values per token."""
+    x = np.asarray(logits, np.float64).copy()
+    V = len(x)
+    history = [int(t) for t in history]
+    if repetition is not None:
+        for t in set(history):
+            if 0 <= t < V:
+                x[t] = x[t] / repetition if x[t] > 0 else x[t] * repetition
+    for t in set(history[max(0, prompt_len):]):
+        if 0 <= t < V:
+            x[t] -= frequency * history[max(0, prompt_len):].count(t) + presence
+    for t, value in biases:
+        if 0 <= t < V:
+            x[t] += value
+    return x if allowed is None else np.where(allowed, x, -np.inf)
