@@ -773,6 +773,30 @@ __global__ __launch_bounds__(128) void paged_decode_merge_quant_group(
   }
 }
 
+// tp[b] = sum of count(b') for b' < b, b <= B <= BAL_MAXB, in LDS (each thread a
+// run of sequences); wsum: one int per wave.
+template <class Count>
+__device__ __forceinline__ void scan_tiles(int* tp, int* wsum, int B, Count&& count) {
+  const int tid = threadIdx.x, nthr = blockDim.x, wave = tid >> 6, lane = tid & 63;
+  const int per = (B + nthr - 1) / nthr;
+  const int lo = min(B, tid * per), hi = min(B, lo + per);
+  int run = 0;
+  for (int i = lo; i < hi; ++i) tp[i + 1] = run += count(i);
+  int incl = run;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 63) wsum[wave] = incl;
+  __syncthreads();
+  int excl = incl - run;
+  for (int w = 0; w < wave; ++w) excl += wsum[w];
+  for (int i = lo; i < hi; ++i) tp[i + 1] += excl;
+  if (tid == 0) tp[0] = 0;
+  __syncthreads();
+}
+
 template <int D, int G, bool WIN>
 void launch_balanced(unsigned nwg, dim3 block, hipStream_t st, const uint16_t* q, const uint16_t* kc,
                      const uint16_t* vc, const int64_t* cl, const int32_t* bt, int64_t bts, float* wo,
@@ -837,6 +861,32 @@ int paged_decode_merge_launch(float* ws_o, float* ws_ml, const int64_t* context_
   hipLaunchKernelGGL(paged_decode_merge, dim3((unsigned)((Hq * D + MERGE_THREADS - 1) / MERGE_THREADS), (unsigned)B),
                      dim3(MERGE_THREADS), 0, st, ws_o, ws_ml, context_lens, (uint16_t*)out, Hq, D, BS, max_blocks, pm);
   return check_launch("paged_decode(merge)");
+}
+
+// Arguments of a decode that splits the work itself.
+int check_decode(const char* what, const void* q, const void* k_cache, const void* v_cache, const int64_t* context_lens,
+                 const int32_t* block_tables, int64_t bt_stride, const void* out, const void* workspace,
+                 int64_t workspace_bytes, int64_t need, int64_t B, int Hq, int Hkv, int D, int BS, int64_t num_blocks,
+                 int max_blocks, const void* q_out, const float* q_scale) {
+  LFS_REQUIRE(B >= 0 && Hq > 0 && Hkv > 0 && BS > 0 && num_blocks >= 0 && max_blocks >= 0, "%s: bad shape", what);
+  LFS_REQUIRE(D == 64 || D == 128, "%s: head_dim must be 64 or 128 (got %d)", what, D);
+  LFS_REQUIRE(Hq % Hkv == 0 && Hq / Hkv <= 8, "%s: num_q_heads (%d) must be a multiple of num_kv_heads (%d), ratio <= 8",
+              what, Hq, Hkv);
+  LFS_REQUIRE(BS % 16 == 0, "%s: block_size must be a multiple of 16 (got %d)", what, BS);
+  LFS_REQUIRE(bt_stride >= max_blocks, "%s: block table stride < max_blocks", what);
+  LFS_REQUIRE(num_blocks >= 1 || max_blocks == 0, "%s: empty KV pool", what);
+  LFS_REQUIRE(B < 65536, "%s: batch too large", what);
+  if (B == 0) return 0;
+  LFS_REQUIRE(q && k_cache && v_cache && context_lens && out, "%s: null pointer", what);
+  LFS_REQUIRE(max_blocks == 0 || block_tables, "%s: null block table", what);
+  LFS_REQUIRE(((((uintptr_t)q) | ((uintptr_t)k_cache) | ((uintptr_t)v_cache) | ((uintptr_t)out)) & 15u) == 0,
+              "%s: q, caches and out must be 16-byte aligned", what);
+  LFS_REQUIRE((q_out == nullptr) == (q_scale == nullptr), "%s: q_out and q_scale go together", what);
+  LFS_REQUIRE(q_out == nullptr || Hq * D % 128 == 0, "%s: the quantised output needs Hq*D %% 128 == 0", what);
+  LFS_REQUIRE(((uintptr_t)workspace & 15u) == 0, "%s: the workspace must be 16-byte aligned", what);
+  LFS_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "%s: workspace of %lld bytes < required %lld", what,
+              (long long)workspace_bytes, (long long)need);
+  return 0;
 }
 
 }  // namespace
