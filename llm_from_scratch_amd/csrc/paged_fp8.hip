@@ -2,341 +2,14 @@
 // fp32 [NB, Hkv, BS] per token and kv head.  With K = s_k k and V = s_v v,
 //   o = sum_t w_t s_v,t v_t / sum_t w_t,   w_t = exp(scale s_k,t (q . k_t) - m).
 //
-// One wave per (sequence, kv head, range of tiles of T tokens).  Per tile:
-//   S = k q^T  v_mfma_f32_16x16x32_bf16, the codes converted (exactly) two at a
-//              time.  Not the FP8 MFMAs: on gfx950 their sums are off by up to
-//              2^-12 of the largest product (measured on sums of 32 to 128 random
-//              products), which a weight would show.  Columns j and j + 8 of q^T
-//              are the same head;
-//   softmax    online, log2 domain; lane l holds the scores of head l % 8 for
-//              tokens 4 (l / 16) .. +3 of every 16-token group;
-//   O^T += v^T P^T  v_mfma_f32_16x16x32_bf16 (codes are exact in bf16): P^T is the
-//              B operand straight from the softmax registers, k-index 8 kq + i
-//              standing for token 4 kq + i of the pair's first 16-token group (i <
-//              4) or 4 kq + i - 4 of its second.  Lane (m, kq) loads D / 16 codes of
-//              those eight tokens, at dims m D / 16 on: pairs of tokens are put
-//              beside each other by byte permutes and converted, so V is transposed
-//              in registers.  Columns j and j + 8 are the weight s_v w rounded to
-//              bf16 and what that left: 16 bits of it;
-//   loads      a tile ahead, in two sets of registers, through buffer descriptors
-//              that end behind the last visible row: rows past the context and of
-//              blocks outside the pool read as zeros, whatever they hold.
-// Work per CU is that of the balanced split of decode_wave.h: one 4-wave workgroup
-// a CU, its waves on adjacent heads of the same rows.
-#include "decode_wave.h"
+// The walk of a wave over its tiles is pool_wave.h's.  Work is shared by the
+// balanced split of decode_wave.h: one 4-wave workgroup a CU, its waves on
+// adjacent heads of the same rows, so that both halves of a 128-byte line (two
+// heads of 64 codes) are asked for together.
+#include "pool_wave.h"
 
 namespace lfs {
 namespace {
-
-
-template <int D>
-struct Fp8Geom {
-  static constexpr int T = D == 64 ? 128 : 64;  // tokens per tile: 16 KiB of codes
-  static constexpr int NG = T / 16;             // 16-token groups
-  static constexpr int TU = T / 64;             // scales per lane
-  static constexpr int KL = D / 64;             // 16-byte K loads per lane and group
-  static constexpr int DB = D / 16;             // V codes per lane and token
-};
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t pool_rows(const uint8_t* base, int64_t off, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base) + off, 0, bytes, 0x00020000);
-}
-// eight codes -> bf16 (exact)
-__device__ __forceinline__ uint32_t bf16_lo(uint32_t w) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
-}
-__device__ __forceinline__ uint32_t bf16_hi(uint32_t w) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true));
-}
-__device__ __forceinline__ v8bf codes_bf16(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(v8bf, make_uint4(bf16_lo(a), bf16_hi(a), bf16_lo(b), bf16_hi(b)));
-}
-constexpr int kNt = 2;  // nontemporal: every row is read once
-
-template <int D, bool ONE>
-struct Fp8Wave {
-  using Geo = Fp8Geom<D>;
-  static constexpr int NG = Geo::NG, TU = Geo::TU, KL = Geo::KL, DB = Geo::DB, T = Geo::T;
-  struct Tile {
-    u32x4 k[NG][KL];
-    uint32_t v[NG][4][DB / 4];
-    float ks[TU], vs[TU];
-    int n;         // tokens up to the context's end (at most T)
-    uint32_t bad;  // bit g: group g lies in no block of the pool
-  };
-
-  int lane, j, kq, kh, Hkv, BS, row;
-  int64_t NB;
-  const uint8_t *kc, *vc;
-  const float *ksc, *vsc;
-  v8bf q[D / 32];
-  float scale_log2, acc[DB][4], m_run, l_run;
-  // the walk: columns and offsets of the next tile whose ids are asked for
-  const int32_t* btrow;
-  int64_t id_end, left;
-  int col[TU], off[TU], ids[TU], idoff[TU], sq, sr;
-
-  // Lane (j, kq) holds dims 64 x + 16 kq .. +15 of head j % 8.
-  __device__ __forceinline__ void load_q(const uint16_t* qp, int G) {
-    const int h = j & 7;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (h < G) w = *reinterpret_cast<const uint4*>(qp + h * D + (c >> 1) * 64 + kq * 16 + (c & 1) * 8);
-      q[c] = __builtin_bit_cast(v8bf, w);
-    }
-  }
-
-  __device__ __forceinline__ void start(const int32_t* bt_row, int64_t t_begin, int64_t t_end) {
-    btrow = bt_row;
-    id_end = block_of(t_end - 1, BS) + 1;
-    left = t_end - t_begin;
-#pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      const int64_t t = t_begin + u * 64 + (lane >> 4) * 16, c = block_of(t, BS);
-      col[u] = (int)c;
-      off[u] = (int)(t - c * BS);
-    }
-    sq = T / BS;
-    sr = T - sq * BS;
-#pragma unroll
-    for (int e = 0; e < DB; ++e)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[e][r] = 0.f;
-    m_run = -INFINITY;
-    l_run = 0.f;
-  }
-  // Ask for the next tile's block ids; columns past the context's are not read.
-  __device__ __forceinline__ void ask() {
-#pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      ids[u] = -1;
-      if (col[u] < id_end) ids[u] = btrow[col[u]];
-      idoff[u] = off[u];
-      col[u] += sq;
-      off[u] += sr;
-      if (off[u] >= BS) off[u] -= BS, ++col[u];
-    }
-  }
-  // Load the tile whose ids were asked for.
-  __device__ __forceinline__ void load(Tile& t) {
-    const int n = (int)max((int64_t)0, min((int64_t)T, left));
-    left -= T;
-    t.n = n;
-    uint32_t bad = 0;
-    int64_t at[TU];
-#pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      const bool ok = ids[u] >= 0 && (int64_t)ids[u] < NB;
-      const int64_t slot = (int64_t)(ok ? ids[u] : 0) * BS + idoff[u];
-      at[u] = slot * row + (int64_t)kh * D;
-      const int tok = u * 64 + lane;
-      const int64_t sat = ((int64_t)(ok ? ids[u] : 0) * Hkv + kh) * BS + idoff[u] + (lane & 15);
-      const bool use = ok && tok < n;
-      const float a = ksc[sat], b = vsc[sat];
-      t.ks[u] = use ? a : 0.f;
-      t.vs[u] = use ? b : 0.f;
-      const uint64_t m = __ballot(!ok);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) bad |= (uint32_t)(m >> (16 * k) & 1) << (u * 4 + k);
-    }
-    t.bad = bad;
-    auto base_of = [&](int g) {
-      const int u = g >> 2, l = (g & 3) * 16;
-      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)at[u], l);
-      const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at[u] >> 32), l);
-      return (int64_t)((uint64_t)hi << 32 | lo);
-    };
-    const int kat = j * row + kq * 16, vat = kq * 4 * row + j * DB;
-    const int64_t b0 = base_of(0);
-    const int all = ONE && n > 0 && !(bad & 1) ? (n - 1) * row + D : 0;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      int64_t b = b0;
-      int bytes = all, soff = g * 16 * row;
-      if constexpr (!ONE) {
-        b = base_of(g);
-        const int rows = min(16, n - g * 16);
-        bytes = rows > 0 && !(bad >> g & 1) ? (rows - 1) * row + D : 0;
-        soff = 0;
-      }
-      const auto kr = pool_rows(kc, b, bytes);
-#pragma unroll
-      for (int x = 0; x < KL; ++x)
-        t.k[g][x] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kr, kat + x * 64, soff, kNt));
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      int64_t b = b0;
-      int bytes = all, soff = g * 16 * row;
-      if constexpr (!ONE) {
-        b = base_of(g);
-        const int rows = min(16, n - g * 16);
-        bytes = rows > 0 && !(bad >> g & 1) ? (rows - 1) * row + D : 0;
-        soff = 0;
-      }
-      const auto vr = pool_rows(vc, b, bytes);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if constexpr (DB == 4) {
-          t.v[g][r][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, vat + r * row, soff, kNt);
-        } else {
-          const auto w = __builtin_amdgcn_raw_buffer_load_b64(vr, vat + r * row, soff, kNt);
-          t.v[g][r][0] = w[0];
-          t.v[g][r][1] = w[1];
-        }
-      }
-    }
-  }
-
-  // pw: the wave's LDS slice, 2 T floats.
-  __device__ __forceinline__ void compute(const Tile& t, float* __restrict__ pw) {
-#pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      pw[u * 64 + lane] = t.ks[u];
-      pw[T + u * 64 + lane] = t.vs[u];
-    }
-    wave_lds_sync();
-    float s[NG][4];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      v4f sc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int x = 0; x < KL; ++x)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const v8bf a = codes_bf16(t.k[g][x][2 * c], t.k[g][x][2 * c + 1]);
-          sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, q[2 * x + c], sc, 0, 0, 0);
-        }
-      const float4 ks = *reinterpret_cast<const float4*>(pw + g * 16 + kq * 4);
-      const float kf[4] = {ks.x, ks.y, ks.z, ks.w};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[g][r] = sc[r] * (scale_log2 * kf[r]);
-    }
-    if (t.n < T || t.bad) {
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if ((t.bad >> g & 1) || g * 16 + kq * 4 + r >= t.n) s[g][r] = -INFINITY;
-    }
-    float tmax = -INFINITY;
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) tmax = fmaxf(tmax, s[g][r]);
-    tmax = max_xor32(max_xor16(tmax));
-    const float m_new = fmaxf(m_run, tmax);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    if (__any(m_new != m_run)) {
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-      l_run *= alpha;
-#pragma unroll
-      for (int e = 0; e < DB; ++e)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[e][r] *= alpha;
-      m_run = m_new;
-    }
-    const uint32_t low = j < 8 ? 0u : 0xFFFF0000u;  // columns 8 .. 15 take what the rounding left
-#pragma unroll
-    for (int p = 0; p < NG / 2; ++p) {
-      uint32_t w[4];
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int g = 2 * p + y;
-        const float4 vs = *reinterpret_cast<const float4*>(pw + T + g * 16 + kq * 4);
-        const float vf[4] = {vs.x, vs.y, vs.z, vs.w};
-        float x[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[r] = __builtin_amdgcn_exp2f(s[g][r] - m_use);
-          l_run += x[r];
-          x[r] *= vf[r];
-        }
-#pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          const uint32_t hi = pack_bf16x2(x[r], x[r + 1]);
-          w[y * 2 + r / 2] = pack_bf16x2(x[r] - __uint_as_float(hi << 16 & low), x[r + 1] - __uint_as_float(hi & low));
-        }
-      }
-      const v8bf pb = __builtin_bit_cast(v8bf, make_uint4(w[0], w[1], w[2], w[3]));
-#pragma unroll
-      for (int d = 0; d < DB / 4; ++d) {
-        uint32_t a[4][4];  // [code of the dword][pair of tokens]
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t t0 = t.v[2 * p + i / 2][(i & 1) * 2][d], t1 = t.v[2 * p + i / 2][(i & 1) * 2 + 1][d];
-          const uint32_t x01 = __builtin_amdgcn_perm(t1, t0, 0x05010400u), x23 = __builtin_amdgcn_perm(t1, t0, 0x07030602u);
-          a[0][i] = bf16_lo(x01), a[1][i] = bf16_hi(x01), a[2][i] = bf16_lo(x23), a[3][i] = bf16_hi(x23);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v4f c = {acc[4 * d + e][0], acc[4 * d + e][1], acc[4 * d + e][2], acc[4 * d + e][3]};
-          c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(v8bf, make_uint4(a[e][0], a[e][1], a[e][2], a[e][3])), pb, c, 0, 0, 0);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[4 * d + e][r] = c[r];
-        }
-      }
-    }
-    wave_lds_sync();
-  }
-
-  __device__ __forceinline__ void walk(const int32_t* bt_row, int64_t t_begin, int64_t t_end, float* __restrict__ pw) {
-    start(bt_row, t_begin, t_end);
-    const int nt = (int)((t_end - t_begin + T - 1) / T);
-    Tile a, b;
-    ask();
-    load(a);
-    ask();
-    for (int i = 0; i < nt; i += 2) {
-      __builtin_amdgcn_sched_barrier(0);
-      load(b);
-      ask();
-      __builtin_amdgcn_sched_barrier(0);
-      compute(a, pw);
-      if (i + 1 >= nt) break;
-      __builtin_amdgcn_sched_barrier(0);
-      load(a);
-      ask();
-      __builtin_amdgcn_sched_barrier(0);
-      compute(b, pw);
-    }
-  }
-
-  // The normalised output of the whole context, or the partial (o, m, l) of
-  // query head kh G + j to row prow + j of the workspace.
-  __device__ __forceinline__ void finish(bool whole, uint16_t* __restrict__ out, float* __restrict__ ws_o,
-                                         float* __restrict__ ws_ml, int64_t prow, int G) {
-    const float l = sum_xor32(sum_xor16(l_run));
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    float o[4][DB];
-#pragma unroll
-    for (int e = 0; e < DB; ++e)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[r][e] = xor_sum<8>(acc[e][r]) * (whole ? inv : 1.f);
-    if (j >= G) return;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = (kq * 4 + r) * DB;
-      if (whole) {
-#pragma unroll
-        for (int e = 0; e < DB; e += 4)
-          *reinterpret_cast<uint2*>(out + (int64_t)j * D + d + e) =
-              make_uint2(pack_bf16x2(o[r][e], o[r][e + 1]), pack_bf16x2(o[r][e + 2], o[r][e + 3]));
-      } else {
-#pragma unroll
-        for (int e = 0; e < DB; e += 4)
-          *reinterpret_cast<float4*>(ws_o + (prow + j) * D + d + e) =
-              make_float4(o[r][e], o[r][e + 1], o[r][e + 2], o[r][e + 3]);
-      }
-    }
-    if (!whole && kq == 0) {
-      ws_ml[(prow + j) * 2 + 0] = m_run;
-      ws_ml[(prow + j) * 2 + 1] = l;
-    }
-  }
-};
 
 // SCAN: a fixed grid shares the tiles of the batch (paged_decode_balanced's
 // split); else a workgroup per (sequence, group of kv heads) walks the whole
@@ -348,18 +21,15 @@ __global__ __launch_bounds__(256) void paged_fp8_kernel(
     const int32_t* __restrict__ bt, int64_t bt_stride, float* __restrict__ ws_o, float* __restrict__ ws_ml,
     int* __restrict__ tp_out, uint16_t* __restrict__ out, int Hkv, int G, int BS, int64_t NB, int max_blocks, int B,
     float scale_log2, int ngroups) {
-  constexpr int T = Fp8Geom<D>::T;
+  constexpr int T = PoolGeom<D, true>::T;
   __shared__ __attribute__((aligned(16))) float scales[4][2 * T];
   __shared__ int tp[SCAN ? BAL_MAXB + 1 : 1];
   __shared__ int wsum[4];
   const int tid = threadIdx.x, wpg = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int64_t cap = (int64_t)max_blocks * BS;
-  Fp8Wave<D, ONE> w;
-  w.lane = lane, w.j = lane & 15, w.kq = lane >> 4;
-  w.Hkv = Hkv, w.BS = BS, w.row = Hkv * D, w.NB = NB;
-  w.scale_log2 = scale_log2;
-  w.kc = kc, w.vc = vc, w.ksc = ksc, w.vsc = vsc;
+  PoolWave<D, true, ONE> w;
+  w.init(lane, kc, vc, ksc, vsc, Hkv, BS, NB, scale_log2);
   auto range = [&](int b, int grp, int64_t i0, int64_t i1, int64_t slot) {
     const int kh = grp * wpg + wave;
     if (kh >= Hkv) return;

@@ -301,14 +301,14 @@ def test_decode_in_graphs_and_on_streams():
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             o, oq, os_ = decode(q, pool, lens, bt, workspace=ws, quant=True)
-        graphs.append((g, lens, o, oq))
+        graphs.append((g, lens, o, oq, ws))  # a captured call's workspace lives as long as its graph
     full = lens_of(seqs)
     for turn in range(3):
         cuts = [torch.clamp(full - 17 * turn - 5 * i, min=0) for i in range(2)]
-        for (g, lens, o, oq), n in zip(graphs, cuts):
+        for (g, lens, o, oq, _), n in zip(graphs, cuts):
             lens.copy_(n)
             g.replay()
-        for (g, lens, o, oq), n in zip(graphs, cuts):
+        for (g, lens, o, oq, _), n in zip(graphs, cuts):
             assert torch.equal(o, decode(q, pool, n, bt))
             assert np.array_equal(bits(oq), bits(K.act_quant(o.view(4, -1))[0]))
     want = decode(q, pool, full, bt)

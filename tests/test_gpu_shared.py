@@ -226,16 +226,16 @@ def test_graphs_and_streams():
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             o = run()
-        graphs.append((g, state, o))
+        graphs.append((g, state, o, ws))  # a captured call's workspace lives as long as its graph
     for turn in range(4):
         now = []
-        for i, (g, state, o) in enumerate(graphs):
+        for i, (g, state, o, _) in enumerate(graphs):
             plan = plans[(turn + i) % 4]
             now.append([torch.tensor(x, dtype=torch.int32, device=DEV) for x in plan] + [(lens - turn * 3 - i).clamp_(min=0)])
             for dst, src in zip(state, now[-1]):
                 dst.copy_(src)
             g.replay()
-        for (g, state, o), (cu, shared, n) in zip(graphs, now):
+        for (g, state, o, _), (cu, shared, n) in zip(graphs, now):
             assert torch.equal(o, K.paged_attention_decode_shared(q, kc, vc, n, bt, cu, shared))
             close(o, q, [[x[:int(m)] for x in s] for s, m in zip(seqs, n)], 0.125, f"turn {turn}")
     side = torch.cuda.Stream()
