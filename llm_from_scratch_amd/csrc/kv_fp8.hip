@@ -6,50 +6,92 @@
 // [NB, Hkv, BS]: a head's scales of a block's tokens follow each other, so a
 // decode tile reads its tokens' scales as one run.
 //
-//  store  D / 8 lanes per (token, K or V, kv head): one 16-byte load, the
-//         group's amax by an xor butterfly, one 8-byte store.  Bound: HBM, 2 D
-//         bytes in and D + 4 out a row.
-//  load   8 values a thread of the same rows back as bf16(code * s), through
-//         the block tables.  Bound: HBM, D + 4 bytes in and 2 D out a row.
-#include "common.h"
+//  store  D / 8 lanes per (token, K or V, kv head): one 16-byte load, the row's
+//         amax by an xor butterfly, one 8-byte store.  A workgroup takes TOK
+//         tokens and writes their scales last, through LDS, a run of tokens a
+//         head.  Bound: HBM, 2 D bytes in and D + 4 out a row.
+//  load   16 values a thread of the same rows back as bf16(code * s).  A workgroup
+//         takes 16 rows of the result, whose slots its first threads find (the
+//         sequence by a binary search, its block by the table).  Bound: HBM, D + 4
+//         bytes in and 2 D out a row.
+#include "tile32.h"
 
 namespace lfs {
 namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+constexpr int SU = 4;  // rows in flight per thread of a store
+constexpr int MAX_ROWS = 4096;
 
 template <int D, bool VEC>
 __global__ __launch_bounds__(256) void store_kvcache_fp8_kernel(
     const uint16_t* __restrict__ key, int64_t ks, const uint16_t* __restrict__ value, int64_t vs,
     uint8_t* __restrict__ kc, uint8_t* __restrict__ vc, float* __restrict__ ksc, float* __restrict__ vsc,
-    const int64_t* __restrict__ slots, int64_t rows, int Hkv, int BS, int64_t num_slots) {
+    const int64_t* __restrict__ slots, int64_t T, int tok, int Hkv, Div rows_tok, Div dBS, int64_t num_slots) {
   constexpr int LPR = D / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = i / LPR;  // (token, K or V, kv head)
-  const int c = (int)(i % LPR);
-  if (row >= rows) return;  // a row's lanes all in or all out
-  const int64_t t = row / (2 * Hkv);
-  const int r = (int)(row - t * 2 * Hkv), h = r < Hkv ? r : r - Hkv;
-  const int64_t slot = slots[t];
-  if (slot < 0 || slot >= num_slots) return;
-  const uint16_t* src = (r < Hkv ? key + t * ks : value + t * vs) + h * D + c * 8;
-  uint4 w;
-  if constexpr (VEC) {
-    w = *reinterpret_cast<const uint4*>(src);
-  } else {
-    uint32_t p[4];
+  __shared__ float sc[MAX_ROWS];  // [token][K or V, head]
+  const int64_t t0 = (int64_t)blockIdx.x * tok;
+  const int nt = (int)min((int64_t)tok, T - t0), rows = nt * (int)rows_tok.d;
+  const int c = threadIdx.x % LPR;
+  for (int i0 = threadIdx.x / LPR; i0 < rows; i0 += SU * 256 / LPR) {
+    uint4 w[SU];
+    int64_t slot[SU];
+    int hd[SU];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) p[e] = (uint32_t)src[2 * e] | (uint32_t)src[2 * e + 1] << 16;
-    w = make_uint4(p[0], p[1], p[2], p[3]);
+    for (int u = 0; u < SU; ++u) {
+      const int i = i0 + u * (256 / LPR);
+      if (i >= rows) break;
+      const int t = (unsigned)i / rows_tok, r = i - t * (int)rows_tok.d;  // K's heads, then V's
+      hd[u] = r;
+      slot[u] = slots[t0 + t];
+      const uint16_t* src = (r < Hkv ? key + (t0 + t) * ks + r * D : value + (t0 + t) * vs + (r - Hkv) * D) + c * 8;
+      if constexpr (VEC) {
+        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src));
+        w[u] = make_uint4(x[0], x[1], x[2], x[3]);
+      } else {
+        __builtin_memcpy(&w[u], src, 16);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < SU; ++u) {
+      const int i = i0 + u * (256 / LPR);
+      if (i >= rows) break;  // a row's lanes all in or all out
+      float f[8], amax = 0.f;
+      unpack8(w[u], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
+      amax = group_max<LPR>(amax);
+      const float s = scale_from_amax(amax, false);
+      if (c == 0) sc[i] = s;
+      if (slot[u] >= 0 && slot[u] < num_slots) {
+        const int h = hd[u] < Hkv ? hd[u] : hd[u] - Hkv;
+        const uint2 q = quant8(f, s);
+        __builtin_nontemporal_store(
+            u32x2{q.x, q.y}, reinterpret_cast<u32x2*>((hd[u] < Hkv ? kc : vc) + (slot[u] * Hkv + h) * D + c * 8));
+      }
+    }
   }
-  float f[8], amax = 0.f;
-  unpack8(w, f);
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows; i += 256) {
+    const int r = i / nt, t = i - r * nt;
+    const int64_t slot = slots[t0 + t];
+    if (slot < 0 || slot >= num_slots) continue;
+    const int h = r < Hkv ? r : r - Hkv;
+    const int64_t blk = slot >> 31 ? slot / (int64_t)dBS.d : (int64_t)((unsigned)slot / dBS);
+    (r < Hkv ? ksc : vsc)[(blk * Hkv + h) * (int)dBS.d + (slot - blk * dBS.d)] = sc[t * (int)rows_tok.d + r];
+  }
+}
+
+constexpr int LT = 16;  // rows of the result a workgroup of a load takes
+constexpr int LU = 4;   // pieces in flight per thread
+
+__device__ __forceinline__ void values16(const u32x4& w, float s, u32x4 (&o)[2]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[e]));
-  amax = group_max<LPR>(amax);
-  const float s = scale_from_amax(amax, false);
-  *reinterpret_cast<uint2*>((r < Hkv ? kc : vc) + (slot * Hkv + h) * D + c * 8) = quant8(f, s);
-  if (c == 0) {
-    const int64_t blk = slot / BS;
-    (r < Hkv ? ksc : vsc)[(blk * Hkv + h) * BS + (slot - blk * BS)] = s;
+  for (int d = 0; d < 4; ++d) {
+    float f[4];
+    e4m3x4_to_f32(w[d], f);
+    o[d / 2][d % 2 * 2] = pack_bf16x2(f[0] * s, f[1] * s);
+    o[d / 2][d % 2 * 2 + 1] = pack_bf16x2(f[2] * s, f[3] * s);
   }
 }
 
@@ -58,40 +100,64 @@ __global__ __launch_bounds__(256) void load_kvcache_fp8_kernel(
     const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, const float* __restrict__ ksc,
     const float* __restrict__ vsc, const int32_t* __restrict__ bt, int64_t bt_stride, int max_blocks,
     const int32_t* __restrict__ cu, int B, int64_t total, uint16_t* __restrict__ k, uint16_t* __restrict__ v, int Hkv,
-    int BS, int64_t NB) {
-  constexpr int LPR = D / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t t = i / (LPR * Hkv);
-  const int c = (int)(i - t * LPR * Hkv), h = c / LPR;
-  if (t >= total) return;
-  int lo = 0, hi = B;  // the last sequence that begins at or before row t
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
+    Div pieces, int BS, int64_t NB) {
+  constexpr int LPR = D / 16;
+  __shared__ int64_t block[LT];  // of a row, -1: none
+  __shared__ int offset[LT];
+  const int64_t t0 = (int64_t)blockIdx.x * LT;
+  const int nt = (int)min((int64_t)LT, total - t0);
+  if (threadIdx.x < nt) {
+    const int64_t t = t0 + threadIdx.x;
+    int lo = 0, hi = B;  // the last sequence that begins at or before row t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid] <= t) lo = mid;
+      else hi = mid;
+    }
+    int64_t blk = -1;
+    int off = 0;
+    if (B > 0 && t >= cu[lo] && t < cu[lo + 1]) {
+      const unsigned pos = (unsigned)(t - cu[lo]), col = pos / (unsigned)BS;
+      off = (int)(pos - col * BS);
+      if (col < (unsigned)max_blocks) blk = bt[lo * bt_stride + col];
+    }
+    block[threadIdx.x] = blk >= 0 && blk < NB ? blk : -1;
+    offset[threadIdx.x] = off;
   }
-  int64_t blk = -1;
-  int off = 0;
-  if (B > 0 && t >= cu[lo] && t < cu[lo + 1]) {
-    const int64_t pos = t - cu[lo], col = pos / BS;
-    off = (int)(pos - col * BS);
-    if (col < max_blocks) blk = bt[lo * bt_stride + col];
+  __syncthreads();
+  const int n = nt * (int)pieces.d;  // pieces: 16 values each, Hkv * D / 16 a row
+  for (int i0 = threadIdx.x; i0 < n; i0 += LU * 256) {
+    u32x4 kw[LU], vw[LU];
+    float a[LU], b[LU];
+#pragma unroll
+    for (int u = 0; u < LU; ++u) {
+      const int i = i0 + u * 256;
+      if (i >= n) break;
+      const int t = (unsigned)i / pieces, c = i - t * (int)pieces.d, h = c / LPR;
+      const int64_t blk = block[t];
+      a[u] = b[u] = 0.f;
+      kw[u] = vw[u] = u32x4{0, 0, 0, 0};
+      if (blk >= 0) {
+        const int64_t at = (blk * BS + offset[t]) * Hkv * D + c * 16, sat = (blk * Hkv + h) * BS + offset[t];
+        kw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kc + at));
+        vw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vc + at));
+        a[u] = ksc[sat], b[u] = vsc[sat];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < LU; ++u) {
+      const int i = i0 + u * 256;
+      if (i >= n) break;
+      const int64_t to = (t0 * (int)pieces.d + i) * 16;
+      u32x4 o[2];
+      values16(kw[u], a[u], o);
+      __builtin_nontemporal_store(o[0], reinterpret_cast<u32x4*>(k + to));
+      __builtin_nontemporal_store(o[1], reinterpret_cast<u32x4*>(k + to) + 1);
+      values16(vw[u], b[u], o);
+      __builtin_nontemporal_store(o[0], reinterpret_cast<u32x4*>(v + to));
+      __builtin_nontemporal_store(o[1], reinterpret_cast<u32x4*>(v + to) + 1);
+    }
   }
-  uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
-  if (blk >= 0 && blk < NB) {
-    const int64_t at = (blk * BS + off) * Hkv * D + c * 8, sat = (blk * Hkv + h) * BS + off;
-    const uint2 kw = *reinterpret_cast<const uint2*>(kc + at), vw = *reinterpret_cast<const uint2*>(vc + at);
-    const float a = ksc[sat], b = vsc[sat];
-    float f[8];
-    e4m3x4_to_f32(kw.x, f), e4m3x4_to_f32(kw.y, f + 4);
-    ko = make_uint4(pack_bf16x2(f[0] * a, f[1] * a), pack_bf16x2(f[2] * a, f[3] * a),
-                    pack_bf16x2(f[4] * a, f[5] * a), pack_bf16x2(f[6] * a, f[7] * a));
-    e4m3x4_to_f32(vw.x, f), e4m3x4_to_f32(vw.y, f + 4);
-    vo = make_uint4(pack_bf16x2(f[0] * b, f[1] * b), pack_bf16x2(f[2] * b, f[3] * b),
-                    pack_bf16x2(f[4] * b, f[5] * b), pack_bf16x2(f[6] * b, f[7] * b));
-  }
-  *reinterpret_cast<uint4*>(k + (t * Hkv * LPR + c) * 8) = ko;
-  *reinterpret_cast<uint4*>(v + (t * Hkv * LPR + c) * 8) = vo;
 }
 
 }  // namespace
@@ -114,11 +180,14 @@ extern "C" int lfs_store_kvcache_fp8(const void* key, int64_t k_stride_t, const 
               "store_kvcache_fp8: the caches must be 8-byte aligned");
   LFS_REQUIRE(T < (1ll << 31) / Hkv / 2, "store_kvcache_fp8: too many tokens");
   const bool vec = k_stride_t % 8 == 0 && v_stride_t % 8 == 0 && ((((uintptr_t)key) | ((uintptr_t)value)) & 15u) == 0;
-  const int64_t rows = T * 2 * Hkv, wgs = (rows * (D / 8) + 255) / 256;
+  LFS_REQUIRE(Hkv <= MAX_ROWS / 8, "store_kvcache_fp8: at most %d kv heads (got %d)", MAX_ROWS / 8, Hkv);
+  const int tok = T >= 2048 && Hkv <= MAX_ROWS / 32 ? 16 : 4;
+  const int64_t wgs = (T + tok - 1) / tok;
 #define LFS_STORE(DD, VEC)                                                                                            \
   hipLaunchKernelGGL((store_kvcache_fp8_kernel<DD, VEC>), dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,     \
                      (const uint16_t*)key, k_stride_t, (const uint16_t*)value, v_stride_t, (uint8_t*)k_cache,         \
-                     (uint8_t*)v_cache, k_scale, v_scale, slot_mapping, rows, Hkv, BS, num_blocks * BS)
+                     (uint8_t*)v_cache, k_scale, v_scale, slot_mapping, T, tok, Hkv, div_by(2 * Hkv), div_by(BS),     \
+                     num_blocks * BS)
   if (D == 64 && vec) LFS_STORE(64, true);
   else if (D == 64) LFS_STORE(64, false);
   else if (vec) LFS_STORE(128, true);
@@ -144,11 +213,13 @@ extern "C" int lfs_load_kvcache_fp8(const void* k_cache, const void* v_cache, co
   LFS_REQUIRE(num_blocks == 0 || (k_cache && v_cache && k_scale && v_scale), "load_kvcache_fp8: null pointer");
   LFS_REQUIRE(((((uintptr_t)k_cache) | ((uintptr_t)v_cache) | ((uintptr_t)k) | ((uintptr_t)v)) & 15u) == 0,
               "load_kvcache_fp8: caches, k and v must be 16-byte aligned");
-  const int64_t wgs = (total * Hkv * (D / 8) + 255) / 256;
+  LFS_REQUIRE(Hkv <= 65536, "load_kvcache_fp8: too many kv heads (%d)", Hkv);
+  const int64_t wgs = (total + LT - 1) / LT;
 #define LFS_LOAD(DD)                                                                                                  \
   hipLaunchKernelGGL((load_kvcache_fp8_kernel<DD>), dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,           \
                      (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, block_tables, bt_stride,     \
-                     max_blocks, cu_seqlens, (int)B, total, (uint16_t*)k, (uint16_t*)v, Hkv, BS, num_blocks)
+                     max_blocks, cu_seqlens, (int)B, total, (uint16_t*)k, (uint16_t*)v, Hkv, div_by(Hkv * DD / 16),   \
+                     BS, num_blocks)
   if (D == 64) LFS_LOAD(64);
   else LFS_LOAD(128);
 #undef LFS_LOAD

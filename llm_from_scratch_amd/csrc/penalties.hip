@@ -11,16 +11,19 @@
 //
 // A workgroup takes CHUNK tokens of the vocabulary of one row: it counts the
 // history's tokens among them in LDS (integers: any order gives the same), then
-// streams the logits past the counts.  The few biased tokens are written again
-// at the end, after a barrier.  Bound: HBM, a read and a write of the logits.
+// streams the logits past the counts, eight a thread and step, chunks beginning
+// where a row of out is 16-byte aligned.  Eight logits without a count among them
+// (nearly all) pass as they are, through the mask.  The few biased tokens are
+// written again at the end, after a barrier.  Bound: HBM, a read and a write of the
+// logits.
 #include "common.h"
 
 namespace lfs {
 namespace {
 
-constexpr int PT = 256;           // threads
+constexpr int PT = 512;           // threads
 constexpr int MAX_BIAS = 1024;    // a row's list of biases lies in LDS
-constexpr uint32_t SEEN = 1u << 31;  // in the prompt; the bits below count the other tokens
+constexpr int HIST = 4;           // of a history's tokens each thread holds this many at a time
 
 struct PenaltyIn {
   const int32_t* tokens;
@@ -49,41 +52,76 @@ __device__ __forceinline__ T logit_out(float x) {
   else return x;
 }
 
-__device__ __forceinline__ float penalised(float x, uint32_t c, float rep, float pres, float freq) {
-  if (c != 0) x = x > 0.f ? x / rep : x * rep;
-  const uint32_t n = c & ~SEEN;
+// seen: in the history; n: times past the prompt
+__device__ __forceinline__ float penalised(float x, bool seen, uint32_t n, float rep, float pres, float freq) {
+  if (seen) x = x > 0.f ? x / rep : x * rep;
   if (n != 0) x = x - freq * (float)n - pres;
   return x;
 }
 
-template <class T, int CHUNK>
+// A token's count: its top bit says that it is in the prompt.  32 bits, or 16
+// where the history is shorter than 2^15, which halves the LDS: two tokens a word.
+template <bool WIDE>
+struct Counts {
+  static constexpr int PER = WIDE ? 1 : 2;
+  static constexpr uint32_t SEEN = WIDE ? 1u << 31 : 1u << 15;
+  static __device__ __forceinline__ void add(uint32_t* c, uint32_t at, bool prompt) {
+    const int sh = WIDE ? 0 : (at & 1) * 16;
+    if (prompt) atomicOr(&c[at / PER], SEEN << sh);
+    else atomicAdd(&c[at / PER], 1u << sh);
+  }
+  static __device__ __forceinline__ uint32_t get(const uint32_t* c, uint32_t at) {
+    return WIDE ? c[at] : (c[at / 2] >> ((at & 1) * 16)) & 0xFFFFu;
+  }
+};
+
+template <class T, bool WIDE, int CHUNK>
 __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t ld, T* out, int64_t ldo,
                                                        int V, PenaltyIn in) {
-  __shared__ __attribute__((aligned(16))) uint32_t count[CHUNK];
+  using C = Counts<WIDE>;
+  // a chunk's tokens from index 8 on; the first chunk's few before the first aligned one from 8 - head
+  __shared__ __attribute__((aligned(16))) uint32_t count[(CHUNK + 8) / C::PER];
   __shared__ int32_t ids[MAX_BIAS];
   const int b = blockIdx.y, tid = threadIdx.x;
-  const int v0 = blockIdx.x * CHUNK, nv = min(CHUNK, V - v0);
-  const bool counts = in.seq_lens != nullptr;
+  T* orow = out + (int64_t)b * ldo;
+  const T* xrow = logits + (int64_t)b * ld;
+  const int head = min(V, (int)(-((uintptr_t)orow / sizeof(T)) & 7));
+  const int body = head + (int)blockIdx.x * CHUNK;         // the chunk's first aligned token
+  const int v0 = blockIdx.x == 0 ? 0 : body;               // and its first
+  const int v1 = min(V, body + CHUNK);                     // and its end
+  const int zero = body - 8;                               // token of LDS index 0
   const float rep = in.repetition ? in.repetition[b] : 1.f;
   const float pres = in.presence ? in.presence[b] : 0.f, freq = in.frequency ? in.frequency[b] : 0.f;
-  for (int i = tid; i < CHUNK; i += PT) count[i] = 0;
-  for (int i = tid; i < in.nbias; i += PT) ids[i] = in.bias_ids[(int64_t)b * in.nbias + i];
-  __syncthreads();
+  const bool counts = in.seq_lens != nullptr;
   if (counts) {
     const int n = max(0, min(in.seq_lens[b], in.width)), np = in.prompt_lens[b];
     const int32_t* row = in.tokens + (int64_t)b * in.tokens_stride;
-    for (int i = tid; i < n; i += PT) {
-      const uint32_t at = (uint32_t)row[i] - (uint32_t)v0;
-      if (at < (uint32_t)nv) {
-        if (i < np) atomicOr(&count[at], SEEN);
-        else atomicAdd(&count[at], 1u);
+    int32_t h[HIST];
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int k = 0; k < HIST; ++k) {
+        const int i = i0 + k * PT + tid;
+        h[k] = i < n ? row[i] : -1;
       }
+    };
+    fetch(0);
+    for (int i = tid * 4; i < (CHUNK + 8) / C::PER; i += PT * 4) *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (int i0 = 0; i0 < n; i0 += HIST * PT) {
+      int32_t now[HIST];
+#pragma unroll
+      for (int k = 0; k < HIST; ++k) now[k] = h[k];
+      fetch(i0 + HIST * PT);
+#pragma unroll
+      for (int k = 0; k < HIST; ++k)
+        if (now[k] >= v0 && now[k] < v1) C::add(count, (uint32_t)(now[k] - zero), i0 + k * PT + tid < np);
     }
   }
-  __syncthreads();
-  const T* x = logits + (int64_t)b * ld + v0;
-  T* o = out + (int64_t)b * ldo + v0;
   const uint32_t* mask = in.allowed ? in.allowed + (int64_t)b * in.allowed_stride : nullptr;
+  auto one = [&](float x, int v) {
+    const uint32_t c = counts ? C::get(count, v - zero) : 0u;
+    return penalised(x, c != 0, c & (C::SEEN - 1), rep, pres, freq);
+  };
   auto allowed = [&](int v) { return mask == nullptr || (mask[v >> 5] >> (v & 31) & 1u); };
   // the biased tokens' logits are read before anything is written: out may be logits
   constexpr int BU = MAX_BIAS / PT;
@@ -91,13 +129,69 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
 #pragma unroll
   for (int u = 0; u < BU; ++u) {
     const int i = tid + u * PT;
-    const uint32_t at = i < in.nbias ? (uint32_t)ids[i] - (uint32_t)v0 : ~0u;
-    bx[u] = at < (uint32_t)nv ? logit_in<T>(x[at]) : 0.f;
+    const int id = i < in.nbias ? in.bias_ids[(int64_t)b * in.nbias + i] : -1;
+    ids[i] = id;
+    bx[u] = id >= v0 && id < v1 ? logit_in<T>(xrow[id]) : 0.f;
   }
   __syncthreads();
-  for (int i = tid; i < nv; i += PT) {
-    const float y = penalised(logit_in<T>(x[i]), count[i], rep, pres, freq);
-    o[i] = logit_out<T>(allowed(v0 + i) ? y : -INFINITY);
+  // tokens before the first aligned one, and past the last eight
+  const int tail = body + (max(0, v1 - body) & ~7);
+  for (int k = tid; k < (body - v0) + (v1 - tail); k += PT) {
+    const int v = k < body - v0 ? v0 + k : tail + k - (body - v0);
+    if (v >= v1) continue;
+    orow[v] = logit_out<T>(allowed(v) ? one(logit_in<T>(xrow[v]), v) : -INFINITY);
+  }
+  constexpr int NQ = 8 * sizeof(T) / 16;  // 16-byte pieces of eight logits
+  const int nwords = (V + 31) >> 5;
+  for (int v = body + tid * 8; v + 8 <= v1; v += PT * 8) {
+    uint4 x[NQ];
+    __builtin_memcpy(x, xrow + v, sizeof(x));
+    uint32_t ok = 0xFFu;
+    if (mask != nullptr) {
+      const int wi = v >> 5, sh = v & 31;
+      const uint32_t w0 = mask[wi], w1 = sh > 24 && wi + 1 < nwords ? mask[wi + 1] : 0u;
+      ok = __builtin_amdgcn_alignbit(w1, w0, sh);
+    }
+    bool any = false;
+    if (counts) {
+      const uint4* c = reinterpret_cast<const uint4*>(count + (v - zero) / C::PER);
+      uint4 q = c[0];
+      uint32_t bits = q.x | q.y | q.z | q.w;
+      if constexpr (WIDE) {
+        q = c[1];
+        bits |= q.x | q.y | q.z | q.w;
+      }
+      any = bits != 0;
+    }
+    if (any) {
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 2)
+            w[e] = pack_bf16x2(one(bf16lo(w[e]), v + 2 * e), one(bf16hi(w[e]), v + 2 * e + 1));
+          else
+            w[e] = __float_as_uint(one(__uint_as_float(w[e]), v + 4 * i + e));
+        }
+        x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t lo = (uint32_t)__builtin_amdgcn_sbfe((int)ok, 2 * e, 1), hi = (uint32_t)__builtin_amdgcn_sbfe((int)ok, 2 * e + 1, 1);
+          const uint32_t m = (lo & 0xFFFFu) | (hi & 0xFFFF0000u);
+          w[e] = (w[e] & m) | (0xFF80FF80u & ~m);
+        } else {
+          w[e] = ok >> (4 * i + e) & 1u ? w[e] : 0xFF800000u;
+        }
+      }
+      reinterpret_cast<uint4*>(orow + v)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
   if (in.nbias == 0) return;
   __syncthreads();
@@ -105,18 +199,30 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
   for (int u = 0; u < BU; ++u) {
     const int i = tid + u * PT;
     if (i >= in.nbias) break;
-    const int32_t id = ids[i];
-    const uint32_t at = (uint32_t)id - (uint32_t)v0;
-    if (at >= (uint32_t)nv || !allowed(id)) continue;
+    const int id = ids[i];
+    if (id < v0 || id >= v1 || !allowed(id)) continue;
     bool first = true;
-    float y = penalised(bx[u], count[at], rep, pres, freq);
+    float y = one(bx[u], id);
     for (int j = 0; j < in.nbias; ++j)
       if (ids[j] == id) {
         first &= j >= i;
         y += in.bias[(int64_t)b * in.nbias + j];
       }
-    if (first) o[at] = logit_out<T>(y);
+    if (first) orow[id] = logit_out<T>(y);
   }
+}
+
+template <class T, bool WIDE>
+void launch_penalties(const void* x, int64_t ld, void* out, int64_t ldo, int64_t B, int V, const PenaltyIn& in,
+                      hipStream_t st) {
+  // few rows: small chunks, so that the vocabulary spreads over the CUs
+  constexpr int BIG = 16384, SMALL = 4096;
+  const bool big = B * ((V + BIG - 1) / BIG) >= 512;
+  const dim3 grid((unsigned)(V / (big ? BIG : SMALL) + 1), (unsigned)B);
+  if (big)
+    hipLaunchKernelGGL((penalties_kernel<T, WIDE, BIG>), grid, dim3(PT), 0, st, (const T*)x, ld, (T*)out, ldo, V, in);
+  else
+    hipLaunchKernelGGL((penalties_kernel<T, WIDE, SMALL>), grid, dim3(PT), 0, st, (const T*)x, ld, (T*)out, ldo, V, in);
 }
 
 }  // namespace
@@ -130,7 +236,8 @@ extern "C" int lfs_apply_penalties(const void* logits, int64_t ld, void* out, in
                                    const float* presence, const float* frequency, const int32_t* bias_ids,
                                    const float* bias, int32_t num_biases, const int32_t* allowed,
                                    int64_t allowed_stride, int64_t B, int32_t V, void* stream) {
-  LFS_REQUIRE(B >= 0 && B < 65536 && V >= 0 && V < (1 << 30) && width >= 0, "apply_penalties: bad shape");
+  LFS_REQUIRE(B >= 0 && B < 65536 && V >= 0 && V < (1 << 30) && width >= 0 && width < (1 << 30),
+              "apply_penalties: bad shape");
   LFS_REQUIRE(num_biases >= 0 && num_biases <= MAX_BIAS, "apply_penalties: at most %d biases a row (got %d)", MAX_BIAS,
               num_biases);
   if (B == 0 || V == 0) return 0;
@@ -143,13 +250,12 @@ extern "C" int lfs_apply_penalties(const void* logits, int64_t ld, void* out, in
   LFS_REQUIRE(!allowed || B == 1 || allowed_stride >= (V + 31) / 32, "apply_penalties: allowed has too few words a row");
   const PenaltyIn in{tokens, tokens_stride, width, prompt_lens, seq_lens, repetition, presence, frequency, bias_ids, bias,
                      num_biases, (const uint32_t*)allowed, allowed_stride};
-  constexpr int CHUNK = 4096;
-  const dim3 grid((unsigned)((V + CHUNK - 1) / CHUNK), (unsigned)B);
-  if (is_f32)
-    hipLaunchKernelGGL((penalties_kernel<float, CHUNK>), grid, dim3(PT), 0, (hipStream_t)stream, (const float*)logits, ld,
-                       (float*)out, ld_out, V, in);
-  else
-    hipLaunchKernelGGL((penalties_kernel<uint16_t, CHUNK>), grid, dim3(PT), 0, (hipStream_t)stream,
-                       (const uint16_t*)logits, ld, (uint16_t*)out, ld_out, V, in);
+  LFS_REQUIRE((((uintptr_t)out | (uintptr_t)logits) & (is_f32 ? 3u : 1u)) == 0, "apply_penalties: unaligned logits");
+  const bool wide = width >= 1 << 15;
+  hipStream_t st = (hipStream_t)stream;
+  if (is_f32 && wide) launch_penalties<float, true>(logits, ld, out, ld_out, B, V, in, st);
+  else if (is_f32) launch_penalties<float, false>(logits, ld, out, ld_out, B, V, in, st);
+  else if (wide) launch_penalties<uint16_t, true>(logits, ld, out, ld_out, B, V, in, st);
+  else launch_penalties<uint16_t, false>(logits, ld, out, ld_out, B, V, in, st);
   return check_launch("apply_penalties");
 }
