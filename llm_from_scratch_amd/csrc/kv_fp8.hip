@@ -10,7 +10,7 @@
 //         amax by an xor butterfly, one 8-byte store.  A workgroup takes TOK
 //         tokens and writes their scales last, through LDS, a run of tokens a
 //         head.  Bound: HBM, 2 D bytes in and D + 4 out a row.
-//  load   16 values a thread of the same rows back as bf16(code * s).  A workgroup
+//  load   8 values a thread and piece of the same rows back as bf16(code * s).  A workgroup
 //         takes 16 rows of the result, whose slots its first threads find (the
 //         sequence by a binary search, its block by the table).  Bound: HBM, D + 4
 //         bytes in and 2 D out a row.
@@ -83,16 +83,13 @@ __global__ __launch_bounds__(256) void store_kvcache_fp8_kernel(
 }
 
 constexpr int LT = 16;  // rows of the result a workgroup of a load takes
-constexpr int LU = 4;   // pieces in flight per thread
+constexpr int LU = 8;   // pieces in flight per thread
 
-__device__ __forceinline__ void values16(const u32x4& w, float s, u32x4 (&o)[2]) {
-#pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    float f[4];
-    e4m3x4_to_f32(w[d], f);
-    o[d / 2][d % 2 * 2] = pack_bf16x2(f[0] * s, f[1] * s);
-    o[d / 2][d % 2 * 2 + 1] = pack_bf16x2(f[2] * s, f[3] * s);
-  }
+__device__ __forceinline__ u32x4 values8(const u32x2& w, float s) {
+  float f[8];
+  e4m3x4_to_f32(w[0], f), e4m3x4_to_f32(w[1], f + 4);
+  return u32x4{pack_bf16x2(f[0] * s, f[1] * s), pack_bf16x2(f[2] * s, f[3] * s), pack_bf16x2(f[4] * s, f[5] * s),
+               pack_bf16x2(f[6] * s, f[7] * s)};
 }
 
 template <int D>
@@ -101,7 +98,7 @@ __global__ __launch_bounds__(256) void load_kvcache_fp8_kernel(
     const float* __restrict__ vsc, const int32_t* __restrict__ bt, int64_t bt_stride, int max_blocks,
     const int32_t* __restrict__ cu, int B, int64_t total, uint16_t* __restrict__ k, uint16_t* __restrict__ v, int Hkv,
     Div pieces, int BS, int64_t NB) {
-  constexpr int LPR = D / 16;
+  constexpr int LPR = D / 8;
   __shared__ int64_t block[LT];  // of a row, -1: none
   __shared__ int offset[LT];
   const int64_t t0 = (int64_t)blockIdx.x * LT;
@@ -125,9 +122,9 @@ __global__ __launch_bounds__(256) void load_kvcache_fp8_kernel(
     offset[threadIdx.x] = off;
   }
   __syncthreads();
-  const int n = nt * (int)pieces.d;  // pieces: 16 values each, Hkv * D / 16 a row
+  const int n = nt * (int)pieces.d;  // pieces: 8 values each, Hkv * D / 8 a row
   for (int i0 = threadIdx.x; i0 < n; i0 += LU * 256) {
-    u32x4 kw[LU], vw[LU];
+    u32x2 kw[LU], vw[LU];
     float a[LU], b[LU];
 #pragma unroll
     for (int u = 0; u < LU; ++u) {
@@ -136,11 +133,11 @@ __global__ __launch_bounds__(256) void load_kvcache_fp8_kernel(
       const int t = (unsigned)i / pieces, c = i - t * (int)pieces.d, h = c / LPR;
       const int64_t blk = block[t];
       a[u] = b[u] = 0.f;
-      kw[u] = vw[u] = u32x4{0, 0, 0, 0};
+      kw[u] = vw[u] = u32x2{0, 0};
       if (blk >= 0) {
-        const int64_t at = (blk * BS + offset[t]) * Hkv * D + c * 16, sat = (blk * Hkv + h) * BS + offset[t];
-        kw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kc + at));
-        vw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vc + at));
+        const int64_t at = (blk * BS + offset[t]) * Hkv * D + c * 8, sat = (blk * Hkv + h) * BS + offset[t];
+        kw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kc + at));
+        vw[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(vc + at));
         a[u] = ksc[sat], b[u] = vsc[sat];
       }
     }
@@ -148,14 +145,9 @@ __global__ __launch_bounds__(256) void load_kvcache_fp8_kernel(
     for (int u = 0; u < LU; ++u) {
       const int i = i0 + u * 256;
       if (i >= n) break;
-      const int64_t to = (t0 * (int)pieces.d + i) * 16;
-      u32x4 o[2];
-      values16(kw[u], a[u], o);
-      __builtin_nontemporal_store(o[0], reinterpret_cast<u32x4*>(k + to));
-      __builtin_nontemporal_store(o[1], reinterpret_cast<u32x4*>(k + to) + 1);
-      values16(vw[u], b[u], o);
-      __builtin_nontemporal_store(o[0], reinterpret_cast<u32x4*>(v + to));
-      __builtin_nontemporal_store(o[1], reinterpret_cast<u32x4*>(v + to) + 1);
+      const int64_t to = (t0 * (int)pieces.d + i) * 8;
+      __builtin_nontemporal_store(values8(kw[u], a[u]), reinterpret_cast<u32x4*>(k + to));
+      __builtin_nontemporal_store(values8(vw[u], b[u]), reinterpret_cast<u32x4*>(v + to));
     }
   }
 }
@@ -218,7 +210,7 @@ extern "C" int lfs_load_kvcache_fp8(const void* k_cache, const void* v_cache, co
 #define LFS_LOAD(DD)                                                                                                  \
   hipLaunchKernelGGL((load_kvcache_fp8_kernel<DD>), dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,           \
                      (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, block_tables, bt_stride,     \
-                     max_blocks, cu_seqlens, (int)B, total, (uint16_t*)k, (uint16_t*)v, Hkv, div_by(Hkv * DD / 16),   \
+                     max_blocks, cu_seqlens, (int)B, total, (uint16_t*)k, (uint16_t*)v, Hkv, div_by(Hkv * DD / 8),   \
                      BS, num_blocks)
   if (D == 64) LFS_LOAD(64);
   else LFS_LOAD(128);

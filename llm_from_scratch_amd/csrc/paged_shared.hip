@@ -410,6 +410,7 @@ __global__ __launch_bounds__(256, 2) void paged_shared_kernel(SharedArgs a) {
 // One wave per 64 elements of an output row: the weights of up to 64 parts at a
 // time, one a lane, then their values in order.  With qo also the act_quant of
 // the 128 values that a workgroup holds, as paged_decode_merge_quant_group.
+constexpr int MU = 16;
 template <int D>
 __global__ __launch_bounds__(128) void paged_shared_merge(SharedArgs a, uint16_t* __restrict__ out,
                                                           uint8_t* __restrict__ qo, float* __restrict__ qs, int64_t E) {
@@ -460,10 +461,16 @@ __global__ __launch_bounds__(128) void paged_shared_merge(SharedArgs a, uint16_t
       den = fmaf(den, old, group_sum<64>(w * l));
       M = Mn;
       const int cnt = min(64, np + ns - c);
-      for (int s = 0; s < cnt; ++s) {
-        const int k = c + s;
-        const float* o = k < np ? a.po + (prow + (int64_t)k * PROWS) * D : a.so + (srow + (int64_t)(k - np) * a.hg * a.G) * D;
-        num = fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s)), o[d], num);
+      for (int s0 = 0; s0 < cnt; s0 += MU) {  // MU values in flight
+        float o[MU];
+#pragma unroll
+        for (int s = 0; s < MU; ++s) {
+          const int k = c + min(s0 + s, cnt - 1);
+          o[s] = (k < np ? a.po + (prow + (int64_t)k * PROWS) * D : a.so + (srow + (int64_t)(k - np) * a.hg * a.G) * D)[d];
+        }
+#pragma unroll
+        for (int s = 0; s < MU; ++s)
+          if (s0 + s < cnt) num = fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s0 + s)), o[s], num);
       }
     }
     v = (uint16_t)f32_to_bf16(den > 0.f ? num / den : 0.f);

@@ -90,6 +90,25 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
   const int v0 = blockIdx.x == 0 ? 0 : body;               // and its first
   const int v1 = min(V, body + CHUNK);                     // and its end
   const int zero = body - 8;                               // token of LDS index 0
+  // the thread's logits and mask words, in flight while the history is counted
+  constexpr int NQ = 8 * sizeof(T) / 16;  // 16-byte pieces of eight logits
+  constexpr int ITER = CHUNK / (PT * 8);
+  const uint32_t* mask = in.allowed ? in.allowed + (int64_t)b * in.allowed_stride : nullptr;
+  const int nwords = (V + 31) >> 5;
+  uint4 x[ITER][NQ];
+  uint32_t ok[ITER];
+#pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const int v = body + (k * PT + tid) * 8;
+    ok[k] = 0xFFu;
+    if (v + 8 > v1) break;
+    __builtin_memcpy(x[k], xrow + v, sizeof(x[k]));
+    if (mask != nullptr) {
+      const int wi = v >> 5, sh = v & 31;
+      const uint32_t w0 = mask[wi], w1 = sh > 24 && wi + 1 < nwords ? mask[wi + 1] : 0u;
+      ok[k] = __builtin_amdgcn_alignbit(w1, w0, sh);
+    }
+  }
   const float rep = in.repetition ? in.repetition[b] : 1.f;
   const float pres = in.presence ? in.presence[b] : 0.f, freq = in.frequency ? in.frequency[b] : 0.f;
   const bool counts = in.seq_lens != nullptr;
@@ -117,7 +136,6 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
         if (now[k] >= v0 && now[k] < v1) C::add(count, (uint32_t)(now[k] - zero), i0 + k * PT + tid < np);
     }
   }
-  const uint32_t* mask = in.allowed ? in.allowed + (int64_t)b * in.allowed_stride : nullptr;
   auto one = [&](float x, int v) {
     const uint32_t c = counts ? C::get(count, v - zero) : 0u;
     return penalised(x, c != 0, c & (C::SEEN - 1), rep, pres, freq);
@@ -141,17 +159,10 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
     if (v >= v1) continue;
     orow[v] = logit_out<T>(allowed(v) ? one(logit_in<T>(xrow[v]), v) : -INFINITY);
   }
-  constexpr int NQ = 8 * sizeof(T) / 16;  // 16-byte pieces of eight logits
-  const int nwords = (V + 31) >> 5;
-  for (int v = body + tid * 8; v + 8 <= v1; v += PT * 8) {
-    uint4 x[NQ];
-    __builtin_memcpy(x, xrow + v, sizeof(x));
-    uint32_t ok = 0xFFu;
-    if (mask != nullptr) {
-      const int wi = v >> 5, sh = v & 31;
-      const uint32_t w0 = mask[wi], w1 = sh > 24 && wi + 1 < nwords ? mask[wi + 1] : 0u;
-      ok = __builtin_amdgcn_alignbit(w1, w0, sh);
-    }
+#pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const int v = body + (k * PT + tid) * 8;
+    if (v + 8 > v1) break;
     bool any = false;
     if (counts) {
       const uint4* c = reinterpret_cast<const uint4*>(count + (v - zero) / C::PER);
@@ -166,7 +177,7 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
     if (any) {
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
-        uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t w[4] = {x[k][i].x, x[k][i].y, x[k][i].z, x[k][i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if constexpr (sizeof(T) == 2)
@@ -174,20 +185,20 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
           else
             w[e] = __float_as_uint(one(__uint_as_float(w[e]), v + 4 * i + e));
         }
-        x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        x[k][i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
-      uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      uint32_t w[4] = {x[k][i].x, x[k][i].y, x[k][i].z, x[k][i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if constexpr (sizeof(T) == 2) {
-          const uint32_t lo = (uint32_t)__builtin_amdgcn_sbfe((int)ok, 2 * e, 1), hi = (uint32_t)__builtin_amdgcn_sbfe((int)ok, 2 * e + 1, 1);
+          const uint32_t lo = (uint32_t)__builtin_amdgcn_sbfe((int)ok[k], 2 * e, 1), hi = (uint32_t)__builtin_amdgcn_sbfe((int)ok[k], 2 * e + 1, 1);
           const uint32_t m = (lo & 0xFFFFu) | (hi & 0xFFFF0000u);
           w[e] = (w[e] & m) | (0xFF80FF80u & ~m);
         } else {
-          w[e] = ok >> (4 * i + e) & 1u ? w[e] : 0xFF800000u;
+          w[e] = ok[k] >> (4 * i + e) & 1u ? w[e] : 0xFF800000u;
         }
       }
       reinterpret_cast<uint4*>(orow + v)[i] = make_uint4(w[0], w[1], w[2], w[3]);
