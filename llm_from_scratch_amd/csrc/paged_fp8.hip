@@ -23,32 +23,46 @@ __global__ __launch_bounds__(256) void paged_fp8_kernel(
     float scale_log2, int ngroups) {
   constexpr int T = PoolGeom<D, true>::T;
   __shared__ __attribute__((aligned(16))) float scales[4][2 * T];
-  __shared__ int tp[SCAN ? BAL_MAXB + 1 : 1];
+  __shared__ int tp[SCAN ? BAL_MAXB + 1 : 1], lens[SCAN ? BAL_MAXB : 1];
   __shared__ int wsum[4];
   const int tid = threadIdx.x, wpg = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int64_t cap = (int64_t)max_blocks * BS;
+  const int cap = max_blocks * BS;
   PoolWave<D, true, ONE> w;
-  w.init(lane, kc, vc, ksc, vsc, Hkv, BS, NB, scale_log2);
-  auto range = [&](int b, int grp, int64_t i0, int64_t i1, int64_t slot) {
-    const int kh = grp * wpg + wave;
-    if (kh >= Hkv) return;
-    const int64_t Lc = min(ctx_lens[b], cap), t0 = i0 * T, t1 = min(Lc, i1 * T);
-    uint16_t* o = out + ((int64_t)b * Hkv + kh) * G * D;
-    if (t0 >= t1) {  // no context (SCAN: never)
-      for (int i = lane; i < G * D / 2; i += 64) reinterpret_cast<uint32_t*>(o)[i] = 0;
-      return;
-    }
-    w.kh = kh;
-    w.load_q(q + ((int64_t)b * Hkv + kh) * G * D, G);
-    w.walk(bt + (int64_t)b * bt_stride, t0, t1, scales[wave]);
-    w.finish(t0 == 0 && t1 >= Lc, o, ws_o, ws_ml, (slot * wpg + wave) * G, G);
+  w.init(lane, kc, vc, ksc, vsc, Hkv, G, BS, NB, scale_log2);
+  // a range of tiles of (sequence, group of kv heads), for the wave's head
+  auto range = [&](PoolRange& r, int b, int kh, int L, int i0, int i1, int64_t slot) {
+    const int64_t h = (int64_t)b * Hkv + kh;
+    r.btrow = bt + (int64_t)b * bt_stride;
+    r.q = q + h * G * D;
+    r.t0 = i0 * T, r.t1 = min(L, i1 * T), r.kh = kh;
+    r.out = r.t0 == 0 && r.t1 >= L ? out + h * G * D : nullptr;
+    r.prow = (slot * wpg + wave) * G;
   };
   if constexpr (!SCAN) {
     const int b = (int)(blockIdx.x / (unsigned)ngroups), grp = (int)(blockIdx.x - (unsigned)b * ngroups);
-    range(b, grp, 0, 1ll << 40, 0);
+    const int kh = grp * wpg + wave, L = (int)min(ctx_lens[b], (int64_t)cap);
+    if (kh >= Hkv) return;
+    if (L <= 0) {
+      uint16_t* o = out + ((int64_t)b * Hkv + kh) * G * D;
+      for (int i = lane; i < G * D / 2; i += 64) reinterpret_cast<uint32_t*>(o)[i] = 0;
+      return;
+    }
+    bool left = true;
+    w.run(
+        [&](PoolRange& r) {
+          if (!left) return false;
+          left = false;
+          range(r, b, kh, L, 0, (L + T - 1) / T, 0);
+          return true;
+        },
+        scales[wave], ws_o, ws_ml);
   } else {
-    scan_tiles(tp, wsum, B, [&](int b) { return decode_tiles(ctx_lens, b, cap, T); });
+    scan_tiles(tp, wsum, B, [&](int b) {
+      const int L = (int)max((int64_t)0, min(ctx_lens[b], (int64_t)cap));
+      lens[b] = L;
+      return (L + T - 1) / T;
+    });
     if (blockIdx.x == 0)
       for (int i = tid; i <= B; i += blockDim.x) tp_out[i] = tp[i];
     const unsigned total = (unsigned)ngroups * (unsigned)tp[B], nwg = gridDim.x;
@@ -62,17 +76,29 @@ __global__ __launch_bounds__(256) void paged_fp8_kernel(
       if ((unsigned)ngroups * (unsigned)tp[mid] <= u) b = mid;
       else b_hi = mid - 1;
     }
-    while (u < u_end) {
-      const unsigned nb = tp[b + 1] - tp[b], base = (unsigned)ngroups * (unsigned)tp[b];
-      const unsigned grp = (u - base) / nb, i0 = (u - base) - grp * nb;
-      const unsigned seg_end = min(u_end, base + (grp + 1) * nb);
-      range(b, (int)grp, i0, i0 + (seg_end - u), (int64_t)blockIdx.x + (int64_t)b * ngroups + grp);
-      u = seg_end;
-      if (u >= base + ngroups * nb) {
-        ++b;
-        while (b < B && tp[b + 1] == tp[b]) ++b;
-      }
-    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    w.run(
+        [&](PoolRange& r) {
+          while (u < u_end) {
+            const unsigned t0 = __builtin_amdgcn_readfirstlane(tp[b]), t1 = __builtin_amdgcn_readfirstlane(tp[b + 1]);
+            const unsigned nb = t1 - t0, base = (unsigned)ngroups * t0;
+            if (u >= base + (unsigned)ngroups * nb) {  // past the sequence, or none of it
+              ++b;
+              continue;
+            }
+            const unsigned grp = (u - base) / nb, i0 = (u - base) - grp * nb;
+            const unsigned stop = min(u_end, base + (grp + 1) * nb);
+            const int kh = grp * wpg + wave;
+            const int i1 = (int)(i0 + (stop - u));
+            u = stop;
+            if (kh >= Hkv) continue;
+            range(r, b, kh, __builtin_amdgcn_readfirstlane(lens[b]), (int)i0, i1,
+                  (int64_t)blockIdx.x + (int64_t)b * ngroups + grp);
+            return true;
+          }
+          return false;
+        },
+        scales[wave], ws_o, ws_ml);
   }
 }
 
@@ -103,11 +129,12 @@ extern "C" int lfs_paged_decode_fp8(const void* q, const void* k_cache, const vo
   LFS_REQUIRE(((((uintptr_t)k_scale) | ((uintptr_t)v_scale)) & 15u) == 0,
               "paged_decode_fp8: the scales must be 16-byte aligned");
   LFS_REQUIRE((int64_t)Hkv * D * 128 < (1ll << 31), "paged_decode_fp8: too many kv heads (%d)", Hkv);
-  const int T = D == 64 ? 128 : 64, G = Hq / Hkv;
+  const int T = 64, G = Hq / Hkv;
   const BalancedGeom bg = balanced_geom(Hkv);
   const bool scan = B <= BAL_MAXB, one = BS % T == 0;
   LFS_REQUIRE((int64_t)bg.ngroups * B * (((int64_t)max_blocks * BS + T - 1) / T) < (1ll << 31),
               "paged_decode_fp8: too many context tiles");
+  LFS_REQUIRE((int64_t)max_blocks * BS < (1ll << 31) - 256, "paged_decode_fp8: block tables of 2^31 tokens");
   const int64_t rows = ((int64_t)bg.nwg + B * bg.ngroups) * bg.wpg * G;
   float* ws_o = (float*)workspace;
   float* ws_ml = ws_o + rows * D;

@@ -371,30 +371,37 @@ __device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, in
     if ((unsigned)a.ngroups * (unsigned)tp[mid] <= u) b = mid;
     else hi = mid - 1;
   }
+  b = __builtin_amdgcn_readfirstlane(b);
   PoolWave<D, false, ONE> wv;
-  wv.init(lane, a.kc, a.vc, nullptr, nullptr, a.Hkv, a.BS, a.NB, a.scale_log2);
-  while (u < u_end) {
-    const unsigned nb = tp[b + 1] - tp[b], base = (unsigned)a.ngroups * (unsigned)tp[b];
-    const unsigned grp = (u - base) / nb, i0 = (u - base) - grp * nb;
-    const unsigned stop = min(u_end, base + (grp + 1) * nb);
-    const int kh = grp * a.hg + head;
-    if (kh < a.Hkv) {
-      int64_t tokens;
-      group_of(a, starts, b, tokens);
-      const int64_t Lc = min(a.ctx_lens[b], cap);
-      const int64_t t0 = tokens + (int64_t)i0 * T, t1 = min(Lc, tokens + (int64_t)(i0 + (stop - u)) * T);
-      wv.kh = kh;
-      wv.load_q(a.q + ((int64_t)b * a.Hkv + kh) * a.G * D, a.G);
-      wv.walk(a.bt + (int64_t)b * a.bt_stride, t0, t1, nullptr);
-      const int64_t slot = ((int64_t)v + (int64_t)b * a.ngroups + grp) * a.hg + head;
-      wv.finish(false, nullptr, a.so, a.sml, slot * a.G, a.G);
-    }
-    u = stop;
-    if (u >= base + a.ngroups * nb) {
-      ++b;
-      while (b < a.B && tp[b + 1] == tp[b]) ++b;
-    }
-  }
+  wv.init(lane, a.kc, a.vc, nullptr, nullptr, a.Hkv, a.G, a.BS, a.NB, a.scale_log2);
+  wv.run(
+      [&](PoolRange& r) {
+        while (u < u_end) {
+          const unsigned t0 = __builtin_amdgcn_readfirstlane(tp[b]), t1 = __builtin_amdgcn_readfirstlane(tp[b + 1]);
+          const unsigned nb = t1 - t0, base = (unsigned)a.ngroups * t0;
+          if (u >= base + (unsigned)a.ngroups * nb) {  // past the sequence, or none of it
+            ++b;
+            continue;
+          }
+          const unsigned grp = (u - base) / nb, i0 = (u - base) - grp * nb;
+          const unsigned stop = min(u_end, base + (grp + 1) * nb);
+          const int kh = grp * a.hg + head, i1 = (int)(i0 + (stop - u));
+          u = stop;
+          if (kh >= a.Hkv) continue;
+          int64_t tokens;
+          group_of(a, starts, b, tokens);
+          const int start = __builtin_amdgcn_readfirstlane((int)tokens);
+          const int L = __builtin_amdgcn_readfirstlane((int)min(a.ctx_lens[b], cap));
+          r.btrow = a.bt + (int64_t)b * a.bt_stride;
+          r.q = a.q + ((int64_t)b * a.Hkv + kh) * a.G * D;
+          r.out = nullptr;
+          r.prow = (((int64_t)v + (int64_t)b * a.ngroups + grp) * a.hg + head) * a.G;
+          r.t0 = start + (int)i0 * T, r.t1 = min(L, start + i1 * T), r.kh = kh;
+          return true;
+        }
+        return false;
+      },
+      nullptr, a.so, a.sml);
 }
 
 template <int D, bool ONE>

@@ -35,7 +35,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <int D, bool FP8>
 struct PoolGeom {
   static constexpr int ES = FP8 ? 1 : 2;             // bytes of a value
-  static constexpr int T = (D == 64 ? 128 : 64) / ES;  // tokens per tile: 16 KiB
+  static constexpr int T = FP8 || D == 64 ? 64 : 32;   // tokens per tile
   static constexpr int NG = T / 16;                  // 16-token groups
   static constexpr int TU = (T + 63) / 64;           // tokens per lane, one each: its scale, its group's block
   static constexpr int KL = D * ES / 64;             // 16-byte K loads per lane and group
@@ -56,76 +56,80 @@ __device__ __forceinline__ uint32_t bf16_hi(uint32_t w) {
 __device__ __forceinline__ v8bf codes_bf16(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(v8bf, make_uint4(bf16_lo(a), bf16_hi(a), bf16_lo(b), bf16_hi(b)));
 }
-constexpr int kNt = 2;  // nontemporal: every row is read once
+
+// Tokens t0 .. t1 - 1 of a context (t0 a multiple of 16, of T or the block size's
+// end where ONE), for kv head kh: G query heads at q, the partial to rows prow ..
+// or, where out is given, the normalised output there.
+struct PoolRange {
+  const int32_t* btrow;
+  const uint16_t* q;
+  uint16_t* out;
+  int64_t prow;
+  int t0, t1, kh;
+};
 
 template <int D, bool FP8, bool ONE>
 struct PoolWave {
   using Geo = PoolGeom<D, FP8>;
   static constexpr int NG = Geo::NG, TU = Geo::TU, KL = Geo::KL, DB = Geo::DB, T = Geo::T, ES = Geo::ES, VD = Geo::VD;
+  // Every row is read once: nontemporal, but where a head's codes are half a line,
+  // whose other half another wave asks for (64 sequences of 8192 tokens, 16 / 4
+  // heads of 64: 65.4 us nontemporal, 61.1 not; of 128 92 and 102).
+  static constexpr int kNt = D * ES >= 128 ? 2 : 0;
   struct Tile {
     u32x4 k[NG][KL];
     uint32_t v[NG][4][VD];
     float ks[TU], vs[TU];
-    int n;         // tokens up to the context's end (at most T)
+    int n;         // tokens up to the range's end (at most T)
     uint32_t bad;  // bit g: group g lies in no block of the pool
+    bool first, last;  // of its range
+    PoolRange at;
   };
 
-  int lane, j, kq, kh, Hkv, BS, row;  // row: bytes of a token
+  int lane, j, kq, Hkv, G, BS, row;  // row: bytes of a token
   int64_t NB;
   const uint8_t *kc, *vc;
   const float *ksc, *vsc;
-  v8bf q[D / 32];
+  v8bf q[D / 32], qnext[D / 32];
   float scale_log2, acc[DB][4], m_run, l_run;
-  // the walk: columns and offsets of the next tile whose ids are asked for
-  const int32_t* btrow;
-  int64_t id_end, left;
-  int col[TU], off[TU], ids[TU], idoff[TU], sq, sr;
+  // the tile asked for: its range, place, block ids and offsets, and the next's columns
+  PoolRange ask_at;
+  int pos, ask_n, col[TU], off[TU], ids[TU], idoff[TU], sq, sr;
+  bool ask_first, ask_last, more;
 
   __device__ __forceinline__ void init(int lane_, const void* kc_, const void* vc_, const float* ksc_, const float* vsc_,
-                                       int Hkv_, int BS_, int64_t NB_, float scale_log2_) {
+                                       int Hkv_, int G_, int BS_, int64_t NB_, float scale_log2_) {
     lane = lane_, j = lane & 15, kq = lane >> 4;
     kc = (const uint8_t*)kc_, vc = (const uint8_t*)vc_, ksc = ksc_, vsc = vsc_;
-    Hkv = Hkv_, BS = BS_, row = Hkv * D * ES, NB = NB_;
+    Hkv = Hkv_, G = G_, BS = BS_, row = Hkv * D * ES, NB = NB_;
     scale_log2 = scale_log2_;
-  }
-
-  // Lane (j, kq) holds of head j % 8 the dims of its K loads.
-  __device__ __forceinline__ void load_q(const uint16_t* qp, int G) {
-    const int h = j & 7;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      const int d = FP8 ? (c >> 1) * 64 + kq * 16 + (c & 1) * 8 : c * 32 + kq * 8;
-      if (h < G) w = *reinterpret_cast<const uint4*>(qp + h * D + d);
-      q[c] = __builtin_bit_cast(v8bf, w);
-    }
-  }
-
-  __device__ __forceinline__ void start(const int32_t* bt_row, int64_t t_begin, int64_t t_end) {
-    btrow = bt_row;
-    id_end = block_of(t_end - 1, BS) + 1;
-    left = t_end - t_begin;
-#pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      const int64_t t = t_begin + u * 64 + (lane >> 4) * 16, c = block_of(t, BS);
-      col[u] = (int)c;
-      off[u] = (int)(t - c * BS);
-    }
     sq = T / BS;
     sr = T - sq * BS;
-#pragma unroll
-    for (int e = 0; e < DB; ++e)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[e][r] = 0.f;
-    m_run = -INFINITY;
-    l_run = 0.f;
   }
-  // Ask for the next tile's block ids; columns past the context's are not read.
-  __device__ __forceinline__ void ask() {
+
+  // Of the next tile (of the range under way, else of the one that next() fills
+  // in) ask for the block ids; columns past the range's are not read.
+  template <class Next>
+  __device__ __forceinline__ void ask(Next&& next) {
+    ask_first = pos >= ask_at.t1;
+    if (ask_first) {
+      more = next(ask_at);
+      pos = ask_at.t0;
+#pragma unroll
+      for (int u = 0; u < TU; ++u) {
+        const unsigned t = pos + u * 64 + (lane >> 4) * 16, c = t / (unsigned)BS;
+        col[u] = (int)c;
+        off[u] = (int)(t - c * BS);
+      }
+    }
+    ask_n = more ? min(T, ask_at.t1 - pos) : 0;
+    pos += T;
+    ask_last = pos >= ask_at.t1;
 #pragma unroll
     for (int u = 0; u < TU; ++u) {
-      ids[u] = -1;
-      if (col[u] < id_end) ids[u] = btrow[col[u]];
+      const int end = (int)((unsigned)(ask_at.t1 - 1) / (unsigned)BS);
+      const int id = ask_at.btrow[min(col[u], end)];
+      ids[u] = col[u] <= end ? id : -1;
       idoff[u] = off[u];
       col[u] += sq;
       off[u] += sr;
@@ -134,9 +138,20 @@ struct PoolWave {
   }
   // Load the tile whose ids were asked for.
   __device__ __forceinline__ void load(Tile& t) {
-    const int n = (int)max((int64_t)0, min((int64_t)T, left));
-    left -= T;
+    const int n = ask_n, kh = ask_at.kh;
     t.n = n;
+    t.first = ask_first, t.last = ask_last;
+    t.at = ask_at;
+    // the range's query, with its first tile: lane (j, kq) holds of head j % 8 the
+    // dims of its K loads
+    {
+      const auto qr = pool_rows(reinterpret_cast<const uint8_t*>(ask_at.q), 0, ask_first ? G * D * 2 : 0);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const int d = FP8 ? (c >> 1) * 64 + kq * 16 + (c & 1) * 8 : c * 32 + kq * 8;
+        qnext[c] = __builtin_bit_cast(v8bf, __builtin_amdgcn_raw_buffer_load_b128(qr, ((j & 7) * D + d) * 2, 0, 0));
+      }
+    }
     uint32_t bad = 0;
     int64_t at[TU];
 #pragma unroll
@@ -317,32 +332,49 @@ struct PoolWave {
     if constexpr (FP8) wave_lds_sync();
   }
 
-  __device__ __forceinline__ void walk(const int32_t* bt_row, int64_t t_begin, int64_t t_end, float* __restrict__ pw) {
-    start(bt_row, t_begin, t_end);
-    const int nt = (int)((t_end - t_begin + T - 1) / T);
+  // Work through the ranges that next(range) fills in until it says false, as one
+  // stream of tiles: the first tile and the query of a range are in flight while
+  // the last of the one before is computed.  pw: LDS for compute().
+  template <class Next>
+  __device__ __forceinline__ void run(Next&& next, float* __restrict__ pw, float* __restrict__ ws_o,
+                                      float* __restrict__ ws_ml) {
+    ask_at.t1 = 0;
+    pos = 0;
+    more = true;
+    ask(next);
+    if (!more) return;
     Tile a, b;
-    ask();
     load(a);
-    ask();
-    for (int i = 0; i < nt; i += 2) {
+    ask(next);
+    auto step = [&](Tile& cur, Tile& nxt) {
       __builtin_amdgcn_sched_barrier(0);
-      load(b);
-      ask();
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) q[c] = cur.first ? qnext[c] : q[c];
+      load(nxt);
+      ask(next);
       __builtin_amdgcn_sched_barrier(0);
-      compute(a, pw);
-      if (i + 1 >= nt) break;
-      __builtin_amdgcn_sched_barrier(0);
-      load(a);
-      ask();
-      __builtin_amdgcn_sched_barrier(0);
-      compute(b, pw);
+      if (cur.first) {
+        m_run = -INFINITY;
+        l_run = 0.f;
+#pragma unroll
+        for (int e = 0; e < DB; ++e)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[e][r] = 0.f;
+      }
+      compute(cur, pw);
+      if (cur.last) finish(cur.at, ws_o, ws_ml);
+    };
+    while (true) {
+      step(a, b);
+      if (b.n == 0) break;
+      step(b, a);
+      if (a.n == 0) break;
     }
   }
 
-  // The normalised output of the whole context, or the partial (o, m, l) of
-  // query head kh G + j to row prow + j of the workspace.
-  __device__ __forceinline__ void finish(bool whole, uint16_t* __restrict__ out, float* __restrict__ ws_o,
-                                         float* __restrict__ ws_ml, int64_t prow, int G) {
+  __device__ __forceinline__ void finish(const PoolRange& at, float* __restrict__ ws_o, float* __restrict__ ws_ml) {
+    const bool whole = at.out != nullptr;
+    const int64_t prow = at.prow;
     const float l = sum_xor32(sum_xor16(l_run));
     const float inv = l > 0.f ? 1.f / l : 0.f;
     float o[4][DB];
@@ -357,7 +389,7 @@ struct PoolWave {
       if (whole) {
 #pragma unroll
         for (int e = 0; e < DB; e += 4)
-          *reinterpret_cast<uint2*>(out + (int64_t)j * D + d + e) =
+          *reinterpret_cast<uint2*>(at.out + (int64_t)j * D + d + e) =
               make_uint2(pack_bf16x2(o[r][e], o[r][e + 1]), pack_bf16x2(o[r][e + 2], o[r][e + 3]));
       } else {
 #pragma unroll
