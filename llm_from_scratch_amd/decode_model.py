@@ -186,6 +186,7 @@ class PagedGQAAttention(nn.Module):
         self.rope = rope
         self.k_cache = torch.empty(0)  # pool views attached by the model runner
         self.v_cache = torch.empty(0)
+        self.k_scale = self.v_scale = None  # scales of a pool in 8 bits
 
     def forward(self, xq: torch.Tensor, xs: torch.Tensor, positions: torch.Tensor,
                 trace: Optional[dict] = None) -> torch.Tensor:
@@ -195,8 +196,12 @@ class PagedGQAAttention(nn.Module):
         T = xq.size(0)
         assert self.k_cache.numel(), "PagedGQAAttention needs the KV pool (ModelRunner.allocate_kv_cache)"
         qkv = self.qkv_proj.gemm(xq, xs)
+        if self.k_scale is not None:
+            return self.forward_fp8(qkv, positions, trace)
+        # (a decode over shared prefixes does not take the norms and the slot write into its launch)
         shape = (T, self.num_heads, self.num_kv_heads, self.head_dim, ctx.block_tables.size(1),
-                 self.k_cache.size(1)) if not ctx.is_prefill and self.window is None and not self.head_norm else None
+                 self.k_cache.size(1)) if not ctx.is_prefill and self.window is None and not self.head_norm \
+            and ctx.cu_groups is None else None
         # the paired order (one workgroup per (sequence, kv head), a long and
         # a short one per CU) when the output projection can quantise its
         # input itself; else one workgroup per pair of kv heads with the
@@ -240,8 +245,42 @@ class PagedGQAAttention(nn.Module):
             out = self.output_proj(o)
         else:
             # the merge also writes the output projection's FP8 input (act_quant fused)
+            if ctx.cu_groups is not None:
+                o, oq, os_ = kernels.paged_attention_decode_shared(
+                    q, self.k_cache, self.v_cache, ctx.context_lens, ctx.block_tables, ctx.cu_groups,
+                    ctx.shared_blocks, self.scale, quant=True)
+            else:
+                o, oq, os_ = kernels.paged_attention_decode(q, self.k_cache, self.v_cache, ctx.context_lens,
+                                                            ctx.block_tables, self.scale, quant=True, **seen)
+            o = o.reshape(T, -1)
+            out = self.output_proj.gemm(oq, os_)
+        if trace is not None:
+            trace.update(qkv=qkv, q=q, att_o=o, att_out=out)
+        return out
+
+
+    def forward_fp8(self, qkv: torch.Tensor, positions: torch.Tensor, trace: Optional[dict] = None) -> torch.Tensor:
+        """forward from the QKV projection on, over a pool in 8 bits.  Whole
+        prompts attend to their keys and values as computed; what later tokens
+        attend to are the codes times the scales."""
+        ctx = get_context()
+        T = qkv.size(0)
+        pool = (self.k_cache, self.v_cache, self.k_scale, self.v_scale)
+        norm_rope = kernels.qk_head_norm_rope_store if self.head_norm else kernels.qk_norm_rope_store
+        q, k, v = norm_rope(qkv, self.q_norm.weight, self.k_norm.weight, self.rope.cos_sin_cached, positions,
+                            self.num_heads, self.num_kv_heads, self.q_norm.eps, return_kv=True)
+        kernels.store_kvcache_fp8(k, v, *pool, ctx.slot_mapping)
+        if ctx.is_prefill:
+            if ctx.block_tables is not None:  # prefix-cache hit: all keys from the pool
+                total = ctx.total_seqlen_k if ctx.total_seqlen_k is not None else int(ctx.cu_seqlens_k[-1])
+                k, v = kernels.load_kvcache_fp8(*pool, ctx.block_tables, ctx.cu_seqlens_k, total)
+            o = kernels.flash_attn_varlen_func(q, k, v, ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.max_seqlen_q,
+                                               ctx.max_seqlen_k, self.scale).reshape(T, -1)
+            out = self.output_proj(o)
+        else:
             o, oq, os_ = kernels.paged_attention_decode(q, self.k_cache, self.v_cache, ctx.context_lens,
-                                                        ctx.block_tables, self.scale, quant=True, **seen)
+                                                        ctx.block_tables, self.scale, quant=True, k_scale=self.k_scale,
+                                                        v_scale=self.v_scale)
             o = o.reshape(T, -1)
             out = self.output_proj.gemm(oq, os_)
         if trace is not None:

@@ -31,6 +31,7 @@ import math
 from copy import copy
 from typing import Optional
 
+import numpy as np
 import torch
 
 from .. import kernels
@@ -90,6 +91,63 @@ def decode_metadata(seqs: list[Sequence], block_size: int) -> dict:
                 slot_mapping=[s.block_table[-1] * block_size + s.last_block_num_tokens - 1 for s in seqs])
 
 
+def shared_groups(tables: list[list[int]]) -> tuple[list[int], list[int]]:
+    """Runs of neighbouring rows whose block tables begin alike: (first row of
+    each and the end, blocks that each shares), for
+    kernels.paged_attention_decode_shared.  A row joins the run before it while
+    that leaves at least half of what the run shares without it; a run of one
+    shares nothing."""
+    starts, shared = [0], []
+    for i, row in enumerate(tables):
+        common = 0
+        if i > 0:
+            first = tables[starts[-1]]
+            most = min(len(first), len(row), shared[-1] if i - starts[-1] > 1 else len(first))
+            while common < most and first[common] == row[common] >= 0:
+                common += 1
+        if common > 0 and (i - starts[-1] == 1 or 2 * common >= shared[-1]):
+            shared[-1] = common
+            continue
+        if i > 0:
+            starts.append(i)
+        shared.append(0)
+    return (starts + [len(tables)] if tables else [0]), shared
+
+
+def penalty_metadata(seqs: list[Sequence], vocab: int) -> dict:
+    """Host arrays of what the batch's logits go through before sampling
+    (kernels.apply_penalties): of each kind, if any of its sequences has it."""
+    B = len(seqs)
+    out = {}
+    if any(s.has_penalties for s in seqs):
+        rows = [s.history() if s.has_penalties else np.empty(0, np.int32) for s in seqs]
+        tokens = np.zeros((B, max(len(r) for r in rows)), np.int32)
+        for b, r in enumerate(rows):
+            tokens[b, :len(r)] = r
+        out.update(tokens=tokens, seq_lens=np.array([len(r) for r in rows], np.int32),
+                   prompt_lens=np.array([s.num_prompt_tokens for s in seqs], np.int32))
+        for name in ("repetition", "presence", "frequency"):
+            out[name] = np.array([getattr(s, name + "_penalty") for s in seqs], np.float32)
+    if any(s.logit_bias for s in seqs):
+        pairs = [list((s.logit_bias or {}).items()) for s in seqs]
+        out["bias_ids"] = np.full((B, max(map(len, pairs))), -1, np.int32)
+        out["bias"] = np.zeros(out["bias_ids"].shape, np.float32)
+        for b, p in enumerate(pairs):
+            if p:
+                out["bias_ids"][b, :len(p)], out["bias"][b, :len(p)] = zip(*p)
+    if any(s.allowed_token_ids is not None for s in seqs):
+        words = -(-vocab // 32)
+        allowed = np.full((B, words), -1, np.int32)
+        for b, s in enumerate(seqs):
+            if s.allowed_token_ids is not None:
+                ids = np.asarray(s.allowed_token_ids, np.int64)
+                bits = np.zeros(words * 32, np.uint8)
+                bits[ids[(ids >= 0) & (ids < vocab)]] = 1
+                allowed[b] = np.packbits(bits, bitorder="little").view(np.int32)
+        out["allowed"] = allowed
+    return out
+
+
 class Sampler:
     """Temperature + Gumbel-max sampling (utils/sampler.py:35-53): argmax of
     softmax(logits / T) / Exp(1) noise, in one kernel (kernels.sample_gumbel).
@@ -143,6 +201,7 @@ class ModelRunner:
         self.block_size = config.get("block_size", 256)
         self.enforce_eager = config.get("enforce_eager", False)
         self.sampler = Sampler()
+        self.check_config()
         self.graphs: dict[int, torch.cuda.CUDAGraph] = {}
         self.graph_vars: dict[str, torch.Tensor] = {}
         if "num_kv_blocks" not in config:
@@ -151,13 +210,44 @@ class ModelRunner:
         if not self.enforce_eager:
             self.capture_cudagraph()
 
+    def check_config(self) -> None:
+        """What a pool in 8 bits ("kv_dtype" torch.float8_e4m3fn) and decode over
+        shared prefixes ("share_prefixes") do not go with."""
+        self.fp8_pool = self.config.get("kv_dtype", torch.bfloat16) == kernels.FP8
+        self.share_prefixes = bool(self.config.get("share_prefixes", False))
+        if not (self.fp8_pool or self.share_prefixes):
+            return
+        if self.fp8_pool and self.share_prefixes:
+            raise ValueError("share_prefixes needs a pool in bf16")
+        for name, m in self.model.named_modules():
+            if not (hasattr(m, "k_cache") and hasattr(m, "v_cache")):
+                continue
+            if getattr(m, "window", None) is not None:
+                raise ValueError(f"{name} attends over a sliding window: neither a pool in 8 bits nor share_prefixes "
+                                 f"goes with it")
+            if self.fp8_pool and not (hasattr(m, "k_scale") and hasattr(m, "v_scale")):
+                raise ValueError(f"{name} takes no scales (k_scale, v_scale): a pool in 8 bits needs them")
+
     # ------------------------------------------------------------ KV pool --
-    def _attach_pool(self, pool: torch.Tensor) -> None:
+    def _new_pool(self, blocks: int) -> tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """A pool [2, L, blocks, BS, Hkv, D] and, in 8 bits, its scales [2, L,
+        blocks, Hkv, BS]."""
+        cfg = self.config
+        layers, heads = cfg["num_layers"], cfg["num_kv_heads"]
+        pool = torch.empty(2, layers, blocks, self.block_size, heads,
+                           cfg.get("head_dim", cfg["hidden_size"] // cfg["num_heads"]),
+                           device=self.device, dtype=cfg.get("kv_dtype", torch.bfloat16))
+        scales = torch.empty(2, layers, blocks, heads, self.block_size, device=self.device) if self.fp8_pool else None
+        return pool, scales
+
+    def _attach_pool(self, pool: torch.Tensor, scales: Optional[torch.Tensor] = None) -> None:
         layer = 0
         for module in self.model.modules():
             if hasattr(module, "k_cache") and hasattr(module, "v_cache"):
                 module.k_cache = pool[0, layer]
                 module.v_cache = pool[1, layer]
+                if scales is not None:
+                    module.k_scale, module.v_scale = scales[0, layer], scales[1, layer]
                 layer += 1
         assert layer == self.config["num_layers"], \
             f"found {layer} attention layers, expected {self.config['num_layers']}"
@@ -185,10 +275,8 @@ class ModelRunner:
         torch.cuda.empty_cache()
         torch.cuda.reset_peak_memory_stats(self.device)
         nblk = n_seq * math.ceil(seq_len / self.block_size)
-        pool = torch.empty(2, cfg["num_layers"], nblk, self.block_size, cfg["num_kv_heads"],
-                           cfg.get("head_dim", cfg["hidden_size"] // cfg["num_heads"]),
-                           device=self.device, dtype=cfg.get("kv_dtype", torch.bfloat16))
-        self._attach_pool(pool)
+        pool, scales = self._new_pool(nblk)
+        self._attach_pool(pool, scales)
         seqs = [Sequence([0] * seq_len) for _ in range(n_seq)]
         per = math.ceil(seq_len / self.block_size)
         for i, sq in enumerate(seqs):
@@ -201,7 +289,9 @@ class ModelRunner:
             if hasattr(module, "k_cache") and hasattr(module, "v_cache"):
                 module.k_cache = torch.empty(0)
                 module.v_cache = torch.empty(0)
-        del pool, ids, pos
+                if scales is not None:
+                    module.k_scale = module.v_scale = None
+        del pool, scales, ids, pos
         torch.cuda.empty_cache()
 
     def allocate_kv_cache(self) -> None:
@@ -210,7 +300,8 @@ class ModelRunner:
         num_kv_heads = cfg["num_kv_heads"]
         head_dim = cfg.get("head_dim", cfg["hidden_size"] // cfg["num_heads"])
         dtype = cfg.get("kv_dtype", torch.bfloat16)
-        block_bytes = self.block_size * 2 * num_layers * num_kv_heads * head_dim * dtype.itemsize
+        row_bytes = head_dim * dtype.itemsize + (4 if self.fp8_pool else 0)
+        block_bytes = self.block_size * 2 * num_layers * num_kv_heads * row_bytes
         if "num_kv_blocks" in cfg:
             nb = int(cfg["num_kv_blocks"])
         else:
@@ -225,9 +316,8 @@ class ModelRunner:
             self.kv_reserved_bytes = reserve
         assert nb >= 1, "Not enough memory to hold at least one block of KV cache"
         self.num_available_kv_blocks = nb
-        self.kv_cache = torch.empty(2, num_layers, nb, self.block_size, num_kv_heads, head_dim,
-                                    device=self.device, dtype=dtype)
-        self._attach_pool(self.kv_cache)
+        self.kv_cache, self.kv_scales = self._new_pool(nb)
+        self._attach_pool(self.kv_cache, self.kv_scales)
 
     # ----------------------------------------------------------- metadata --
     def _pad_tables(self, seqs: list[Sequence]) -> torch.Tensor:
@@ -245,7 +335,7 @@ class ModelRunner:
         block_tables = self._pad_tables(seqs) if m["cu_seqlens_q"][-1] < m["cu_seqlens_k"][-1] else None
         set_context(True, dev(m["cu_seqlens_q"], torch.int32), dev(m["cu_seqlens_k"], torch.int32),
                     m["max_seqlen_q"], m["max_seqlen_k"], dev(m["slot_mapping"], torch.int64),
-                    None, block_tables)
+                    None, block_tables, total_seqlen_k=m["cu_seqlens_k"][-1])
         return dev(m["input_ids"], torch.int64), dev(m["positions"], torch.int64)
 
     def prepare_decode(self, seqs: list[Sequence]):
@@ -255,8 +345,12 @@ class ModelRunner:
         def dev(x, dtype):
             return torch.tensor(x, dtype=dtype, **pin).to(self.device, non_blocking=True)
 
+        groups = {}
+        if self.share_prefixes:
+            starts, shared = shared_groups([s.block_table for s in seqs])
+            groups = dict(cu_groups=dev(starts, torch.int32), shared_blocks=dev(shared, torch.int32))
         set_context(False, None, None, 0, 0, dev(m["slot_mapping"], torch.int64),
-                    dev(m["context_lens"], torch.int64), self._pad_tables(seqs))
+                    dev(m["context_lens"], torch.int64), self._pad_tables(seqs), **groups)
         return dev(m["input_ids"], torch.int64), dev(m["positions"], torch.int64)
 
     def prepare_sample(self, seqs: list[Sequence]) -> torch.Tensor:
@@ -272,10 +366,27 @@ class ModelRunner:
                 filters[name] = torch.tensor(values, dtype=dtype, pin_memory=True).to(self.device, non_blocking=True)
         return filters
 
+    def penalise(self, logits: torch.Tensor, seqs: list[Sequence]) -> torch.Tensor:
+        """The batch's logits with its sequences' penalties, biases and masks."""
+        arrays = penalty_metadata(seqs, logits.size(-1))
+        if not arrays:
+            return logits
+
+        def dev(x):
+            t = torch.empty(x.shape, dtype=torch.from_numpy(x[:0]).dtype, pin_memory=True)
+            t.numpy()[...] = x
+            return t.to(self.device, non_blocking=True)
+
+        if logits.dtype not in (torch.bfloat16, torch.float32):
+            logits = logits.to(torch.bfloat16)
+        return kernels.apply_penalties(logits, **{name: dev(x) for name, x in arrays.items()})
+
     def copy_blocks(self, copies: list[tuple[int, int]]) -> None:
         """Copy whole blocks of every layer's K and V: (source, destination)."""
         if copies:
             kernels.copy_kv_blocks(self.kv_cache, *zip(*copies))
+            if self.kv_scales is not None:  # [.., NB, Hkv, BS, 1]: a block's scales too are one piece
+                kernels.copy_kv_blocks(self.kv_scales.unsqueeze(-1), *zip(*copies))
 
     # --------------------------------------------------------------- run ---
     @torch.inference_mode()
@@ -294,6 +405,11 @@ class ModelRunner:
         v["context_lens"][:bs] = ctx.context_lens
         v["block_tables"].fill_(-1)
         v["block_tables"][:bs, :ctx.block_tables.size(1)] = ctx.block_tables
+        if self.share_prefixes:
+            n = ctx.shared_blocks.size(0)
+            v["cu_groups"][:n + 1] = ctx.cu_groups
+            v["cu_groups"][n + 1:].fill_(bs)  # no rows in the other groups
+            v["shared_blocks"][:n] = ctx.shared_blocks
         self.graphs[graph_bs].replay()
         return self.graph_logits(bs)
 
@@ -320,6 +436,7 @@ class ModelRunner:
             # one logit row per sequence: the last prompt token
             last = get_context().cu_seqlens_q[1:] - 1
             logits = logits[last]
+        logits = self.penalise(logits, seqs)
         token_ids = self.sampler(logits, self.prepare_sample(seqs), generator, **self.prepare_filters(seqs)).tolist()
         reset_context()
         return token_ids
@@ -339,13 +456,17 @@ class ModelRunner:
         slot_mapping = torch.full((max_bs,), -1, dtype=torch.int64, device=dev)
         context_lens = torch.zeros(max_bs, dtype=torch.int64, device=dev)
         block_tables = torch.full((max_bs, max_blocks), -1, dtype=torch.int32, device=dev)
+        groups = dict(cu_groups=torch.zeros(max_bs + 1, dtype=torch.int32, device=dev),
+                      shared_blocks=torch.zeros(max_bs, dtype=torch.int32, device=dev)) if self.share_prefixes else {}
         sizes = [b for b in [1, 2, 4, 8] + list(range(16, max_bs + 1, 16)) if b <= max_bs]
         self.graph_outputs = {}
         pool = None
         for bs in reversed(sizes):
             graph = torch.cuda.CUDAGraph()
             set_context(False, slot_mapping=slot_mapping[:bs], context_lens=context_lens[:bs],
-                        block_tables=block_tables[:bs])
+                        block_tables=block_tables[:bs],
+                        **({} if not groups else dict(cu_groups=groups["cu_groups"][:bs + 1],
+                                                      shared_blocks=groups["shared_blocks"][:bs])))
             fwd = getattr(self.model, "forward_q", None)
             run = (lambda: fwd(input_ids[:bs], positions[:bs])) if fwd is not None else \
                 (lambda: (self.model(input_ids[:bs], positions[:bs]), None, None))
@@ -360,4 +481,4 @@ class ModelRunner:
             torch.cuda.synchronize()
             reset_context()
         self.graph_vars = dict(input_ids=input_ids, positions=positions, slot_mapping=slot_mapping,
-                               context_lens=context_lens, block_tables=block_tables)
+                               context_lens=context_lens, block_tables=block_tables, **groups)

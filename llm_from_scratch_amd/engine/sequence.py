@@ -9,18 +9,25 @@ block and gives a full last block an empty slot list).
 from __future__ import annotations
 
 import math
+from array import array
 from copy import copy
 from dataclasses import dataclass
 from enum import Enum, auto
 from itertools import count
 from typing import Optional
 
+import numpy as np
+
 
 @dataclass
 class SamplingParams:
     """utils/sampler.py:7-23 of the reference, plus the ``max_model_length``
-    field engine/sequence.py:34 reads from it and the filters of
-    kernels.sample_filtered (top_k 0, top_p 1 and min_p 0: none)."""
+    field engine/sequence.py:34 reads from it, the filters of
+    kernels.sample_filtered (top_k 0, top_p 1 and min_p 0: none) and what
+    kernels.apply_penalties does to the logits before: repetition_penalty
+    (1: none) for tokens of the prompt and the completion, presence_penalty and
+    frequency_penalty (0: none) for those of the completion, logit_bias (token ->
+    value) and allowed_token_ids (None: all)."""
     temperature: float = 1.0
     max_tokens: int = 256
     ignore_eos: bool = False
@@ -28,11 +35,21 @@ class SamplingParams:
     top_k: int = 0
     top_p: float = 1.0
     min_p: float = 0.0
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Optional[dict[int, float]] = None
+    allowed_token_ids: Optional[list[int]] = None
 
     def __post_init__(self):
         assert self.temperature > 1e-10, "greedy sampling is not permitted"
         assert 0 <= self.top_k < 2 ** 31 and 0 < self.top_p <= 1 and 0 <= self.min_p <= 1, \
             "top_k must be in [0, 2**31), top_p in (0, 1], min_p in [0, 1]"
+        assert 0 < self.repetition_penalty < math.inf, "repetition_penalty must be > 0"
+        assert math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty), \
+            "presence_penalty and frequency_penalty must be finite"
+        assert not self.logit_bias or len(self.logit_bias) <= 1024, "logit_bias holds at most 1024 tokens"
+        assert self.allowed_token_ids is None or len(self.allowed_token_ids) > 0, "allowed_token_ids allows no token"
 
 
 class SequenceStatus(Enum):
@@ -57,6 +74,10 @@ class Sequence:
         self.block_table: list[int] = []  # -1: a block freed behind the sliding window
         self.num_released_blocks = 0  # from the first block without sinks on
         self.top_k, self.top_p, self.min_p = sp.top_k, sp.top_p, sp.min_p
+        self.repetition_penalty = sp.repetition_penalty
+        self.presence_penalty, self.frequency_penalty = sp.presence_penalty, sp.frequency_penalty
+        self.logit_bias, self.allowed_token_ids = sp.logit_bias, sp.allowed_token_ids
+        self._history = array("i")
         self.temperature = sp.temperature
         self.max_tokens = sp.max_tokens
         self.ignore_eos = sp.ignore_eos
@@ -69,6 +90,7 @@ class Sequence:
         child.seq_id = next(Sequence.counter)
         child.token_ids = copy(self.token_ids)
         child.block_table = copy(self.block_table)
+        child._history = copy(self._history)
         return child
 
     def __len__(self):
@@ -111,6 +133,15 @@ class Sequence:
     def block(self, i):
         assert 0 <= i < self.num_blocks, f"Block index {i} out of range [0, {self.num_blocks})"
         return self.token_ids[i * self.block_size:(i + 1) * self.block_size]
+
+    @property
+    def has_penalties(self):
+        return self.repetition_penalty != 1 or self.presence_penalty != 0 or self.frequency_penalty != 0
+
+    def history(self) -> np.ndarray:
+        """The token ids as int32, from a copy that grows with them."""
+        self._history.extend(self.token_ids[len(self._history):])
+        return np.frombuffer(self._history, np.int32, self.num_tokens).copy()
 
     def append_token(self, token_id):
         self.token_ids.append(token_id)

@@ -1,0 +1,120 @@
+"""Host side of pools in 8 bits, shared prefixes and penalties (CPU only)."""
+import numpy as np
+import pytest
+import torch
+
+from llm_from_scratch_amd.decode_model import DecodeModelConfig
+from llm_from_scratch_amd.engine import ModelRunner, SamplingParams, Sequence
+from llm_from_scratch_amd.engine.model_runner import penalty_metadata, shared_groups
+
+
+def test_shared_groups():
+    a, b = list(range(10)), list(range(100, 110))
+    assert shared_groups([]) == ([0], [])
+    assert shared_groups([a]) == ([0, 1], [0])
+    assert shared_groups([a, b]) == ([0, 1, 2], [0, 0])
+    assert shared_groups([a, a[:6] + [50], a[:6] + [51, 52]]) == ([0, 3], [6])
+    # a row that shares less than half of what the others do begins a run of its own
+    assert shared_groups([a, a[:8] + [50], a[:2] + [60], a[:2] + [61]]) == ([0, 2, 4], [8, 2])
+    assert shared_groups([b, a, a[:3], a[:4]]) == ([0, 1, 4], [0, 3])
+    # freed blocks are shared by nobody
+    assert shared_groups([[1, -1, 3], [1, -1, 3]]) == ([0, 2], [1])
+    assert shared_groups([[-1, 2], [-1, 2]]) == ([0, 1, 2], [0, 0])
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_shared_groups_are_common_beginnings(seed):
+    rng = np.random.default_rng(seed)
+    base = [rng.permutation(50).tolist()[:8] for _ in range(3)]
+    rows = []
+    for _ in range(int(rng.integers(1, 20))):
+        n = int(rng.integers(0, 9))
+        rows.append(base[int(rng.integers(0, 3))][:n] + [int(x) for x in rng.integers(1000, 2000, int(rng.integers(0, 3)))])
+    starts, shared = shared_groups(rows)
+    assert starts[0] == 0 and starts[-1] == len(rows) and all(x < y for x, y in zip(starts, starts[1:]))
+    assert len(shared) == len(starts) - 1
+    for a, b, n in zip(starts, starts[1:], shared):
+        assert all(r[:n] == rows[a][:n] and len(r) >= n for r in rows[a:b])
+        assert n == 0 if b - a == 1 else n > 0
+
+
+def seq(tokens, prompt, **kw):
+    s = Sequence(tokens[:prompt], SamplingParams(**kw))
+    for t in tokens[prompt:]:
+        s.append_token(t)
+    return s
+
+
+def test_penalty_metadata():
+    plain = seq([1, 2, 3], 2)
+    assert penalty_metadata([plain], 100) == {}
+    s = seq([5, 6, 5, 7], 2, repetition_penalty=1.5, frequency_penalty=0.25)
+    m = penalty_metadata([plain, s], 100)
+    assert set(m) == {"tokens", "seq_lens", "prompt_lens", "repetition", "presence", "frequency"}
+    assert m["tokens"].tolist() == [[0, 0, 0, 0], [5, 6, 5, 7]] and m["seq_lens"].tolist() == [0, 4]
+    assert m["prompt_lens"].tolist() == [2, 2] and m["repetition"].tolist() == [1, 1.5]
+    assert m["frequency"].tolist() == [0, 0.25] and m["presence"].tolist() == [0, 0]
+    s.append_token(9)
+    assert penalty_metadata([s], 100)["tokens"].tolist() == [[5, 6, 5, 7, 9]]
+    biased = seq([1], 1, logit_bias={7: 2.0, 70: -1.5})
+    m = penalty_metadata([plain, biased], 100)
+    assert set(m) == {"bias_ids", "bias"}
+    assert m["bias_ids"].tolist() == [[-1, -1], [7, 70]] and m["bias"].tolist() == [[0, 0], [2, -1.5]]
+    some = seq([1], 1, allowed_token_ids=[0, 33, 69, 70, -3])
+    m = penalty_metadata([some, plain], 70)
+    assert set(m) == {"allowed"} and m["allowed"].shape == (2, 3) and m["allowed"].dtype == np.int32
+    assert m["allowed"][0].tolist() == [1, 2, 32] and (m["allowed"][1] == -1).all()
+
+
+def test_history_grows_with_the_sequence_and_forks_apart():
+    s = seq([3, 4], 2, presence_penalty=1.0)
+    assert s.history().tolist() == [3, 4]
+    held = s.history()
+    child = s.fork()
+    for i in range(200):
+        s.append_token(i)
+        child.append_token(1000 + i)
+    assert s.history().tolist() == [3, 4] + list(range(200)) and s.history().dtype == np.int32
+    assert child.history().tolist() == [3, 4] + list(range(1000, 1200)) and held.tolist() == [3, 4]
+    assert child.presence_penalty == 1.0
+
+
+def test_sampling_params():
+    with pytest.raises(AssertionError, match="repetition_penalty"):
+        SamplingParams(repetition_penalty=0)
+    with pytest.raises(AssertionError, match="finite"):
+        SamplingParams(presence_penalty=float("nan"))
+    with pytest.raises(AssertionError, match="1024"):
+        SamplingParams(logit_bias={i: 1.0 for i in range(1025)})
+    with pytest.raises(AssertionError, match="no token"):
+        SamplingParams(allowed_token_ids=[])
+
+
+class Layer(torch.nn.Module):
+    def __init__(self, window=None, scales=True):
+        super().__init__()
+        self.k_cache = self.v_cache = torch.empty(0)
+        self.window = window
+        if scales:
+            self.k_scale = self.v_scale = None
+
+
+def checked(layer, **config):
+    runner = ModelRunner.__new__(ModelRunner)
+    runner.model, runner.config = torch.nn.ModuleList([layer]), config
+    runner.check_config()
+    return runner
+
+
+def test_what_pools_in_8_bits_and_shared_prefixes_go_with():
+    fp8 = torch.float8_e4m3fn
+    assert checked(Layer(), kv_dtype=fp8).fp8_pool and not checked(Layer(window=4)).fp8_pool
+    assert checked(Layer(), share_prefixes=True).share_prefixes
+    with pytest.raises(ValueError, match="bf16"):
+        checked(Layer(), kv_dtype=fp8, share_prefixes=True)
+    for config in (dict(kv_dtype=fp8), dict(share_prefixes=True)):
+        with pytest.raises(ValueError, match="sliding window"):
+            checked(Layer(window=4), **config)
+    with pytest.raises(ValueError, match="no scales"):
+        checked(Layer(scales=False), kv_dtype=fp8)
+    assert DecodeModelConfig().runner_config(kv_dtype=fp8)["kv_dtype"] == fp8
