@@ -9,13 +9,15 @@
 //   x = -infinity where the row's mask has no bit for v
 // and one rounding to the logits' type.
 //
-// A workgroup takes CHUNK tokens of the vocabulary of one row: it counts the
-// history's tokens among them in LDS (integers: any order gives the same), then
-// streams the logits past the counts, eight a thread and step, chunks beginning
-// where a row of out is 16-byte aligned.  Eight logits without a count among them
-// (nearly all) pass as they are, through the mask.  The few biased tokens are
-// written again at the end, after a barrier.  Bound: HBM, a read and a write of the
-// logits.
+// A workgroup takes CHUNK tokens of the vocabulary of one row, from where the row
+// of out is 16-byte aligned.  It streams the logits through the mask, eight a
+// thread and step, and meanwhile counts the history's tokens among them in LDS
+// (integers: any order gives the same), whose first occurrences make a list.
+// After a barrier the few listed and biased tokens are read again and written as
+// the formula has them.  Counting every logit's penalties in the stream instead
+// took 45 us where this takes PEN_KERNEL (256 rows of 150001, histories of 50 to
+// 4096, 64 biases): nearly every wave has some token with a count.  Bound: HBM, a
+// read and a write of the logits.
 #include "common.h"
 
 namespace lfs {
@@ -59,16 +61,20 @@ __device__ __forceinline__ float penalised(float x, bool seen, uint32_t n, float
   return x;
 }
 
-// A token's count: its top bit says that it is in the prompt.  32 bits, or 16
-// where the history is shorter than 2^15, which halves the LDS: two tokens a word.
+// A token's count, with two marks: in the prompt, in the list of biases.  32 bits,
+// or 16 where the history is shorter than 2^14, which halves the LDS: two a word.
 template <bool WIDE>
 struct Counts {
-  static constexpr int PER = WIDE ? 1 : 2;
-  static constexpr uint32_t SEEN = WIDE ? 1u << 31 : 1u << 15;
-  static __device__ __forceinline__ void add(uint32_t* c, uint32_t at, bool prompt) {
+  static constexpr int PER = WIDE ? 1 : 2, BITS = WIDE ? 32 : 16;
+  static constexpr uint32_t SEEN = 1u << (BITS - 1), BIASED = 1u << (BITS - 2), TIMES = BIASED - 1;
+  // returns the token's count before
+  static __device__ __forceinline__ uint32_t add(uint32_t* c, uint32_t at, bool prompt) {
     const int sh = WIDE ? 0 : (at & 1) * 16;
-    if (prompt) atomicOr(&c[at / PER], SEEN << sh);
-    else atomicAdd(&c[at / PER], 1u << sh);
+    const uint32_t old = prompt ? atomicOr(&c[at / PER], SEEN << sh) : atomicAdd(&c[at / PER], 1u << sh);
+    return (old >> sh) & (SEEN | TIMES);
+  }
+  static __device__ __forceinline__ void mark(uint32_t* c, uint32_t at) {
+    atomicOr(&c[at / PER], BIASED << (WIDE ? 0 : (at & 1) * 16));
   }
   static __device__ __forceinline__ uint32_t get(const uint32_t* c, uint32_t at) {
     return WIDE ? c[at] : (c[at / 2] >> ((at & 1) * 16)) & 0xFFFFu;
@@ -81,7 +87,9 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
   using C = Counts<WIDE>;
   // a chunk's tokens from index 8 on; the first chunk's few before the first aligned one from 8 - head
   __shared__ __attribute__((aligned(16))) uint32_t count[(CHUNK + 8) / C::PER];
-  __shared__ int32_t ids[MAX_BIAS];
+  __shared__ uint16_t list[CHUNK + 8];  // indexes of the history's tokens, once each
+  __shared__ __attribute__((aligned(16))) int32_t ids[MAX_BIAS];
+  __shared__ int listed;
   const int b = blockIdx.y, tid = threadIdx.x;
   T* orow = out + (int64_t)b * ldo;
   const T* xrow = logits + (int64_t)b * ld;
@@ -90,11 +98,33 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
   const int v0 = blockIdx.x == 0 ? 0 : body;               // and its first
   const int v1 = min(V, body + CHUNK);                     // and its end
   const int zero = body - 8;                               // token of LDS index 0
-  // the thread's logits and mask words, in flight while the history is counted
+  if (v0 >= v1) return;
+  // the thread's logits and mask words, the first of the history (which of it
+  // counts is known later) and of the list of biases
   constexpr int NQ = 8 * sizeof(T) / 16;  // 16-byte pieces of eight logits
   constexpr int ITER = CHUNK / (PT * 8);
   const uint32_t* mask = in.allowed ? in.allowed + (int64_t)b * in.allowed_stride : nullptr;
   const int nwords = (V + 31) >> 5;
+  const bool counts = in.seq_lens != nullptr;
+  const int32_t* row = in.tokens + (int64_t)b * in.tokens_stride;
+  int32_t h[HIST];
+  auto fetch = [&](int i0, int n) {
+#pragma unroll
+    for (int k = 0; k < HIST; ++k) {
+      const int i = i0 + k * PT + tid;
+      h[k] = i < n ? row[i] : -1;
+    }
+  };
+  if (counts) fetch(0, in.width);
+  constexpr int BU = MAX_BIAS / PT;
+  int id[BU];
+  float by[BU];
+#pragma unroll
+  for (int u = 0; u < BU; ++u) {
+    const int i = tid + u * PT;
+    id[u] = i < in.nbias ? in.bias_ids[(int64_t)b * in.nbias + i] : -1;
+    by[u] = i < in.nbias ? in.bias[(int64_t)b * in.nbias + i] : 0.f;
+  }
   uint4 x[ITER][NQ];
   uint32_t ok[ITER];
 #pragma unroll
@@ -111,90 +141,62 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
   }
   const float rep = in.repetition ? in.repetition[b] : 1.f;
   const float pres = in.presence ? in.presence[b] : 0.f, freq = in.frequency ? in.frequency[b] : 0.f;
-  const bool counts = in.seq_lens != nullptr;
+  if (tid == 0) listed = 0;
+  if (counts)
+    for (int i = tid * 4; i < (CHUNK + 8) / C::PER; i += PT * 4) *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int u = 0; u < BU; ++u) ids[tid + u * PT] = id[u];
+  __syncthreads();
+  int same[BU];  // how often the token is in the list, 0 where it was earlier
+#pragma unroll
+  for (int u = 0; u < BU; ++u) {
+    same[u] = 0;
+    if (id[u] < v0 || id[u] >= v1) continue;
+    if (counts) C::mark(count, id[u] - zero);
+    int n = 0, before = 0;
+    for (int j = 0; j < in.nbias; j += 4) {  // (past the list: -1)
+      const int4 q = *reinterpret_cast<const int4*>(ids + j);
+      const int i = tid + u * PT - j;
+      const int m = (q.x == id[u]) | (q.y == id[u]) << 1 | (q.z == id[u]) << 2 | (q.w == id[u]) << 3;
+      n += __builtin_popcount(m);
+      before |= i >= 4 ? m : i > 0 ? m & ((1 << i) - 1) : 0;
+    }
+    same[u] = before ? 0 : n;
+  }
   if (counts) {
     const int n = max(0, min(in.seq_lens[b], in.width)), np = in.prompt_lens[b];
-    const int32_t* row = in.tokens + (int64_t)b * in.tokens_stride;
-    int32_t h[HIST];
-    auto fetch = [&](int i0) {
-#pragma unroll
-      for (int k = 0; k < HIST; ++k) {
-        const int i = i0 + k * PT + tid;
-        h[k] = i < n ? row[i] : -1;
-      }
-    };
-    fetch(0);
-    for (int i = tid * 4; i < (CHUNK + 8) / C::PER; i += PT * 4) *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
     for (int i0 = 0; i0 < n; i0 += HIST * PT) {
       int32_t now[HIST];
 #pragma unroll
-      for (int k = 0; k < HIST; ++k) now[k] = h[k];
-      fetch(i0 + HIST * PT);
+      for (int k = 0; k < HIST; ++k) now[k] = i0 + k * PT + tid < n ? h[k] : -1;
+      if (i0 + HIST * PT < n) fetch(i0 + HIST * PT, n);
 #pragma unroll
       for (int k = 0; k < HIST; ++k)
-        if (now[k] >= v0 && now[k] < v1) C::add(count, (uint32_t)(now[k] - zero), i0 + k * PT + tid < np);
+        if (now[k] >= v0 && now[k] < v1) {
+          const int at = now[k] - zero;
+          if (C::add(count, at, i0 + k * PT + tid < np) == 0) list[atomicAdd(&listed, 1)] = (uint16_t)at;
+        }
     }
   }
-  auto one = [&](float x, int v) {
-    const uint32_t c = counts ? C::get(count, v - zero) : 0u;
-    return penalised(x, c != 0, c & (C::SEEN - 1), rep, pres, freq);
-  };
   auto allowed = [&](int v) { return mask == nullptr || (mask[v >> 5] >> (v & 31) & 1u); };
-  // the biased tokens' logits are read before anything is written: out may be logits
-  constexpr int BU = MAX_BIAS / PT;
-  float bx[BU];
-#pragma unroll
-  for (int u = 0; u < BU; ++u) {
-    const int i = tid + u * PT;
-    const int id = i < in.nbias ? in.bias_ids[(int64_t)b * in.nbias + i] : -1;
-    ids[i] = id;
-    bx[u] = id >= v0 && id < v1 ? logit_in<T>(xrow[id]) : 0.f;
-  }
-  __syncthreads();
   // tokens before the first aligned one, and past the last eight
   const int tail = body + (max(0, v1 - body) & ~7);
   for (int k = tid; k < (body - v0) + (v1 - tail); k += PT) {
     const int v = k < body - v0 ? v0 + k : tail + k - (body - v0);
-    if (v >= v1) continue;
-    orow[v] = logit_out<T>(allowed(v) ? one(logit_in<T>(xrow[v]), v) : -INFINITY);
+    if (v < v1) orow[v] = allowed(v) ? xrow[v] : logit_out<T>(-INFINITY);
   }
 #pragma unroll
   for (int k = 0; k < ITER; ++k) {
     const int v = body + (k * PT + tid) * 8;
     if (v + 8 > v1) break;
-    bool any = false;
-    if (counts) {
-      const uint4* c = reinterpret_cast<const uint4*>(count + (v - zero) / C::PER);
-      uint4 q = c[0];
-      uint32_t bits = q.x | q.y | q.z | q.w;
-      if constexpr (WIDE) {
-        q = c[1];
-        bits |= q.x | q.y | q.z | q.w;
-      }
-      any = bits != 0;
-    }
-    if (any) {
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        uint32_t w[4] = {x[k][i].x, x[k][i].y, x[k][i].z, x[k][i].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (sizeof(T) == 2)
-            w[e] = pack_bf16x2(one(bf16lo(w[e]), v + 2 * e), one(bf16hi(w[e]), v + 2 * e + 1));
-          else
-            w[e] = __float_as_uint(one(__uint_as_float(w[e]), v + 4 * i + e));
-        }
-        x[k][i] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
       uint32_t w[4] = {x[k][i].x, x[k][i].y, x[k][i].z, x[k][i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if constexpr (sizeof(T) == 2) {
-          const uint32_t lo = (uint32_t)__builtin_amdgcn_sbfe((int)ok[k], 2 * e, 1), hi = (uint32_t)__builtin_amdgcn_sbfe((int)ok[k], 2 * e + 1, 1);
+          const uint32_t lo = (uint32_t)__builtin_amdgcn_sbfe((int)ok[k], 2 * e, 1);
+          const uint32_t hi = (uint32_t)__builtin_amdgcn_sbfe((int)ok[k], 2 * e + 1, 1);
           const uint32_t m = (lo & 0xFFFFu) | (hi & 0xFFFF0000u);
           w[e] = (w[e] & m) | (0xFF80FF80u & ~m);
         } else {
@@ -204,22 +206,27 @@ __global__ __launch_bounds__(PT) void penalties_kernel(const T* logits, int64_t 
       reinterpret_cast<uint4*>(orow + v)[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  if (in.nbias == 0) return;
   __syncthreads();
+  // the row of out now holds the chunk's logits as they came, but where masked
+  auto one = [&](int v, uint32_t c) {
+    return penalised(logit_in<T>(orow[v]), (c & (C::SEEN | C::TIMES)) != 0, c & C::TIMES, rep, pres, freq);
+  };
+  if (counts)
+    for (int i = tid; i < listed; i += PT) {
+      const int at = list[i], v = at + zero;
+      const uint32_t c = C::get(count, at);
+      if ((c & C::BIASED) == 0 && allowed(v)) orow[v] = logit_out<T>(one(v, c));
+    }
 #pragma unroll
   for (int u = 0; u < BU; ++u) {
-    const int i = tid + u * PT;
-    if (i >= in.nbias) break;
-    const int id = ids[i];
-    if (id < v0 || id >= v1 || !allowed(id)) continue;
-    bool first = true;
-    float y = one(bx[u], id);
-    for (int j = 0; j < in.nbias; ++j)
-      if (ids[j] == id) {
-        first &= j >= i;
+    if (same[u] == 0 || !allowed(id[u])) continue;
+    float y = one(id[u], counts ? C::get(count, id[u] - zero) : 0u) + by[u];
+    for (int j = tid + u * PT + 1, n = same[u]; n > 1 && j < in.nbias; ++j)
+      if (ids[j] == id[u]) {
         y += in.bias[(int64_t)b * in.nbias + j];
+        --n;
       }
-    if (first) orow[id] = logit_out<T>(y);
+    orow[id[u]] = logit_out<T>(y);
   }
 }
 
@@ -227,7 +234,7 @@ template <class T, bool WIDE>
 void launch_penalties(const void* x, int64_t ld, void* out, int64_t ldo, int64_t B, int V, const PenaltyIn& in,
                       hipStream_t st) {
   // few rows: small chunks, so that the vocabulary spreads over the CUs
-  constexpr int BIG = 16384, SMALL = 4096;
+  constexpr int BIG = 8192, SMALL = 4096;
   const bool big = B * ((V + BIG - 1) / BIG) >= 512;
   const dim3 grid((unsigned)(V / (big ? BIG : SMALL) + 1), (unsigned)B);
   if (big)
@@ -262,7 +269,7 @@ extern "C" int lfs_apply_penalties(const void* logits, int64_t ld, void* out, in
   const PenaltyIn in{tokens, tokens_stride, width, prompt_lens, seq_lens, repetition, presence, frequency, bias_ids, bias,
                      num_biases, (const uint32_t*)allowed, allowed_stride};
   LFS_REQUIRE((((uintptr_t)out | (uintptr_t)logits) & (is_f32 ? 3u : 1u)) == 0, "apply_penalties: unaligned logits");
-  const bool wide = width >= 1 << 15;
+  const bool wide = width >= 1 << 14;
   hipStream_t st = (hipStream_t)stream;
   if (is_f32 && wide) launch_penalties<float, true>(logits, ld, out, ld_out, B, V, in, st);
   else if (is_f32) launch_penalties<float, false>(logits, ld, out, ld_out, B, V, in, st);
