@@ -438,17 +438,26 @@ def copy_kv_blocks(kv_cache: torch.Tensor, src, dst) -> None:
             _ptr(kv_cache), planes, NB, block, s.buffer_info()[0], d.buffer_info()[0], len(s))
 
 
+# The checks of the calls below in one expression each, and one by one only
+# where that fails: a call's checks took 4-5 us one by one.
 def _fp8_pool(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
     """(NB, BS, Hkv, D) of a pool in 8 bits, checked."""
+    shape = k_cache.shape
+    if len(shape) == 4:
+        NB, BS, Hkv, D = shape
+        scales = (NB, Hkv, BS)
+        if (k_cache.dtype is v_cache.dtype is FP8 and k_scale.dtype is v_scale.dtype is torch.float32
+                and v_cache.shape == shape and k_scale.shape == v_scale.shape == scales
+                and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+                and v_scale.is_contiguous()):
+            return NB, BS, Hkv, D
     for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dtype is not FP8:
-            _dtype(t, FP8, n)
+        _dtype(t, FP8, n)
         assert t.dim() == 4 and t.is_contiguous(), f"{n} must be contiguous [num_blocks, block_size, Hkv, D]"
-    NB, BS, Hkv, D = k_cache.shape
     assert v_cache.shape == k_cache.shape, "k_cache and v_cache must have one shape"
+    NB, BS, Hkv, D = k_cache.shape
     for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        if t.dtype is not torch.float32:
-            _dtype(t, torch.float32, n)
+        _dtype(t, torch.float32, n)
         assert t.shape == (NB, Hkv, BS) and t.is_contiguous(), f"{n} must be contiguous [num_blocks, Hkv, block_size]"
     return NB, BS, Hkv, D
 
@@ -464,10 +473,11 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
     fp32 [num_blocks, Hkv, block_size], contiguous; slot_mapping: int64 [T].
     Slots outside the pool are skipped like -1; a slot may appear once."""
     NB, BS, Hkv, D = _fp8_pool(k_cache, v_cache, k_scale, v_scale)
-    assert key.dim() == 3 and value.shape == key.shape and key.shape[1:] == (Hkv, D), "key and value must be [T, Hkv, D]"
-    assert key.stride(2) == value.stride(2) == 1 and key.stride(1) == value.stride(1) == D, \
-        "heads and dims of key and value must be contiguous"
-    T = key.size(0)
+    assert key.dim() == 3 and value.shape == key.shape, "key and value must be [T, Hkv, D]"
+    T, heads, dim = key.shape
+    assert heads == Hkv and dim == D, "key and value must be [T, Hkv, D]"
+    (ks, kh, kd), (vs, vh, vd) = key.stride(), value.stride()
+    assert kd == vd == 1 and kh == vh == D, "heads and dims of key and value must be contiguous"
     assert slot_mapping.shape == (T,) and slot_mapping.is_contiguous(), "slot_mapping must be contiguous [T]"
     _on_gpu(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
     if not (key.dtype is value.dtype is torch.bfloat16 and slot_mapping.dtype is torch.int64):
@@ -475,7 +485,7 @@ def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Ten
         _dtype(value, torch.bfloat16, "value")
         _dtype(slot_mapping, torch.int64, "slot_mapping")
     _launch("store_kvcache_fp8", _lib.load().lfs_store_kvcache_fp8, key,
-            key.data_ptr(), key.stride(0), value.data_ptr(), value.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+            key.data_ptr(), ks, value.data_ptr(), vs, k_cache.data_ptr(), v_cache.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(), T, Hkv, D, BS, NB)
 
 
@@ -500,7 +510,8 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
     if not block_tables.dtype is cu_seqlens.dtype is torch.int32:
         _dtype(block_tables, torch.int32, "block_tables")
         _dtype(cu_seqlens, torch.int32, "cu_seqlens")
-    k, v = torch.empty(2, total, Hkv, D, dtype=torch.bfloat16, device=k_cache.device).unbind(0)
+    k = torch.empty(total, Hkv, D, dtype=torch.bfloat16, device=k_cache.device)
+    v = torch.empty_like(k)
     _launch("load_kvcache_fp8", _lib.load().lfs_load_kvcache_fp8, k_cache,
             k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
             _row_stride(block_tables), max_blocks, cu_seqlens.data_ptr(), B, total, k.data_ptr(), v.data_ptr(), Hkv, D,
@@ -1148,39 +1159,38 @@ def apply_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     _on_gpu(logits)
     B, V = logits.shape
     dev, rows = logits.get_device(), [prompt_lens, seq_lens, repetition, presence, frequency]
+    size = (B,)
     for i, t in enumerate(rows):
         if t is None:
             continue
-        if t.get_device() != dev:
+        if not (t.get_device() == dev and t.dtype is _PENALTY_TYPES[i] and t.shape == size):
             _on_gpu(logits, t)
-        if t.dtype is not _PENALTY_TYPES[i]:
             _dtype(t, _PENALTY_TYPES[i], _PENALTY_NAMES[i])
-        assert t.shape == (B,), f"{_PENALTY_NAMES[i]} must be [B]"
+            assert t.shape == size, f"{_PENALTY_NAMES[i]} must be [B]"
         if not t.is_contiguous():
             rows[i] = t.contiguous()
-    if not (tokens is None) == (prompt_lens is None) == (seq_lens is None):
-        raise ValueError("tokens, prompt_lens and seq_lens go together")
-    if tokens is None and not repetition is presence is frequency is None:
-        raise ValueError("penalties need tokens, prompt_lens and seq_lens")
+    if tokens is None:
+        if not (prompt_lens is None and seq_lens is None):
+            raise ValueError("tokens, prompt_lens and seq_lens go together")
+        if not (repetition is None and presence is None and frequency is None):
+            raise ValueError("penalties need tokens, prompt_lens and seq_lens")
+        token_args = (None, 0, 0)
+    else:
+        if prompt_lens is None or seq_lens is None:
+            raise ValueError("tokens, prompt_lens and seq_lens go together")
+        tokens = _penalty_matrix(logits, tokens, torch.int32, "tokens", B)
+        token_args = (tokens.data_ptr(), _row_stride(tokens), tokens.size(1))
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
-    for t, n, dt, width in ((tokens, "tokens", torch.int32, None), (bias_ids, "bias_ids", torch.int32, None),
-                            (bias, "bias", torch.float32, None if bias is None else bias_ids.size(-1)),
-                            (allowed, "allowed", torch.int32, -(-V // 32))):
-        if t is None:
-            continue
-        if t.get_device() != dev:
-            _on_gpu(logits, t)
-        if t.dtype is not dt:
-            _dtype(t, dt, n)
-        assert t.dim() == 2 and t.size(0) == B and (width is None or t.size(1) == width), \
-            f"{n} must be [B, {'n' if width is None else width}]"
-    if tokens is not None and tokens.stride(1) != 1:
-        tokens = tokens.contiguous()
+    n = 0
     if bias is not None:
-        bias_ids, bias = bias_ids.contiguous(), bias.contiguous()
-    if allowed is not None and allowed.stride(1) != 1:
-        allowed = allowed.contiguous()
+        bias_ids = _penalty_matrix(logits, bias_ids, torch.int32, "bias_ids", B).contiguous()
+        n = bias_ids.size(1)
+        bias = _penalty_matrix(logits, bias, torch.float32, "bias", B, n).contiguous()
+    mask_args = (None, 0)
+    if allowed is not None:
+        allowed = _penalty_matrix(logits, allowed, torch.int32, "allowed", B, -(-V // 32))
+        mask_args = (allowed.data_ptr(), _row_stride(allowed))
     if out is None:
         out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
     else:
@@ -1191,10 +1201,21 @@ def apply_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         assert out.shape == logits.shape and out.stride(1) == 1, "out must be [B, V] with unit column stride"
     _launch("apply_penalties", _lib.load().lfs_apply_penalties, logits,
             logits.data_ptr(), _row_stride(logits), out.data_ptr(), _row_stride(out), logits.dtype is torch.float32,
-            _ptr(tokens), 0 if tokens is None else _row_stride(tokens), 0 if tokens is None else tokens.size(1),
-            *map(_ptr, rows), _ptr(bias_ids), _ptr(bias), 0 if bias is None else bias.size(1), _ptr(allowed),
-            0 if allowed is None else _row_stride(allowed), B, V)
+            *token_args, *map(_ptr, rows), _ptr(bias_ids), _ptr(bias), n, *mask_args, B, V)
     return out
+
+
+def _penalty_matrix(logits: torch.Tensor, t: torch.Tensor, dtype: torch.dtype, name: str, rows: int,
+                    width: Optional[int] = None) -> torch.Tensor:
+    """t [rows, width], checked, with unit column stride."""
+    if t.get_device() != logits.get_device():
+        _on_gpu(logits, t)
+    if t.dtype is not dtype:
+        _dtype(t, dtype, name)
+    shape = t.shape
+    assert len(shape) == 2 and shape[0] == rows and (width is None or shape[1] == width), \
+        f"{name} must be [B, {'n' if width is None else width}]"
+    return t if t.stride(1) == 1 else t.contiguous()
 
 
 _PENALTY_TYPES = (torch.int32, torch.int32, torch.float32, torch.float32, torch.float32)
