@@ -105,6 +105,20 @@ __device__ __forceinline__ void prefix_unit(const SharedArgs& a, uint8_t* smem, 
     if (r >= rows) return 0;
     return (int)max((int64_t)0, min(min(a.ctx_lens[first + r / a.G], cap), tokens));
   };
+  // lanes 16 x .. 16 x + 15 look after the tile's 16-key group x: block column
+  // and offset, asked for a tile ahead, the first before the rows' lengths are known
+  const int32_t* btrow = a.bt + (int64_t)first * a.bt_stride;
+  const int gkey = 16 * (lane >> 4);
+  int col = (unsigned)(k0 * KT + gkey) / (unsigned)a.BS;
+  int off = k0 * KT + gkey - col * a.BS, entry = -1, eoff = 0;
+  auto ask = [&](int t0) {
+    entry = -1;
+    eoff = off;
+    if (t0 + gkey < tokens) entry = btrow[col];
+    off += KT;
+    while (off >= a.BS) off -= a.BS, ++col;
+  };
+  ask(k0 * KT);
   // keys that any of the workgroup's rows sees: none past them is read
   int kend = max(limit_of(r0 + lane), limit_of(r0 + 64 + lane));
 #pragma unroll
@@ -131,24 +145,11 @@ __device__ __forceinline__ void prefix_unit(const SharedArgs& a, uint8_t* smem, 
   }
   const uint8_t* kb = reinterpret_cast<const uint8_t*>(a.kc) + (int64_t)kh * RB;
   const uint8_t* vb = reinterpret_cast<const uint8_t*>(a.vc) + (int64_t)kh * RB;
-  // lanes 16 x .. 16 x + 15 look after the tile's 16-key group x: block column
-  // and offset, asked for a tile ahead
-  const int32_t* btrow = a.bt + (int64_t)first * a.bt_stride;
-  const int gkey = 16 * (lane >> 4);
-  int64_t col = ((int64_t)k0 * KT + gkey) / a.BS;
-  int off = (int)((int64_t)k0 * KT + gkey - col * a.BS), entry = -1, eoff = 0;
-  auto ask = [&](int t0) {
-    entry = -1;
-    eoff = off;
-    if (t0 + gkey < kend) entry = btrow[col];
-    off += KT;
-    while (off >= a.BS) off -= a.BS, ++col;
-  };
   // copies of the tile at key t0 to buffer buf; returns which of its groups hold
   // visible keys.  A wave copies one group's K and V; one without takes the rows
   // of one with, whose values are finite, and its scores are masked.
   auto fetch = [&](int t0, int buf) -> unsigned {
-    const bool ok = entry >= 0 && (int64_t)entry < a.NB;
+    const bool ok = entry >= 0 && (int64_t)entry < a.NB && t0 + gkey < kend;
     const uint64_t m = __ballot(ok);
     const unsigned use = (unsigned)(m & 1) | (unsigned)(m >> 16 & 1) << 1 | (unsigned)(m >> 32 & 1) << 2 |
                          (unsigned)(m >> 48 & 1) << 3;
@@ -198,7 +199,6 @@ __device__ __forceinline__ void prefix_unit(const SharedArgs& a, uint8_t* smem, 
   unsigned use = 0, next = 0;
   __syncthreads();  // the tiles' LDS is free
   if (k0 < k1) {
-    ask(k0 * KT);
     next = fetch(k0 * KT, 0);
     ask((k0 + 1) * KT);
   }
