@@ -7,13 +7,18 @@
 // decode tile reads its tokens' scales as one run.
 //
 //  store  D / 8 lanes per (token, K or V, kv head): one 16-byte load, the row's
-//         amax by an xor butterfly, one 8-byte store.  A workgroup takes TOK
+//         amax by an xor butterfly, one 8-byte store.  A workgroup takes tok
 //         tokens and writes their scales last, through LDS, a run of tokens a
-//         head.  Bound: HBM, 2 D bytes in and D + 4 out a row.
-//  load   8 values a thread and piece of the same rows back as bf16(code * s).  A workgroup
-//         takes 16 rows of the result, whose slots its first threads find (the
-//         sequence by a binary search, its block by the table).  Bound: HBM, D + 4
-//         bytes in and 2 D out a row.
+//         head.  Bound: HBM, 2 D bytes in and D + 4 out a row: 16383 tokens of 8
+//         heads of 128 in 22.6 us, 4.5 TB/s.
+//  load   8 values a thread and piece of the same rows back as bf16(code * s).  A
+//         workgroup takes 16 rows of the result, whose slots its first threads
+//         find (the sequence by a binary search, its block by the table).  Bound: HBM, D + 4
+//         bytes in and 2 D out a row: 8 sequences of 4000 to 16384 tokens, 8 heads
+//         of 128, blocks of 16 in 93 us, 5.4 TB/s (with 16 values a thread, whose
+//         stores are half lines, 116).
+#include <algorithm>
+
 #include "tile32.h"
 
 namespace lfs {
@@ -21,7 +26,7 @@ namespace {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int SU = 4;  // rows in flight per thread of a store
-constexpr int MAX_ROWS = 4096;
+constexpr int MAX_ROWS = 1024;  // (K or V, head) rows of a workgroup
 
 template <int D, bool VEC>
 __global__ __launch_bounds__(256) void store_kvcache_fp8_kernel(
@@ -172,8 +177,14 @@ extern "C" int lfs_store_kvcache_fp8(const void* key, int64_t k_stride_t, const 
               "store_kvcache_fp8: the caches must be 8-byte aligned");
   LFS_REQUIRE(T < (1ll << 31) / Hkv / 2, "store_kvcache_fp8: too many tokens");
   const bool vec = k_stride_t % 8 == 0 && v_stride_t % 8 == 0 && ((((uintptr_t)key) | ((uintptr_t)value)) & 15u) == 0;
-  LFS_REQUIRE(Hkv <= MAX_ROWS / 8, "store_kvcache_fp8: at most %d kv heads (got %d)", MAX_ROWS / 8, Hkv);
-  const int tok = T >= 2048 && Hkv <= MAX_ROWS / 32 ? 16 : 4;
+  LFS_REQUIRE(Hkv <= MAX_ROWS / 2, "store_kvcache_fp8: at most %d kv heads (got %d)", MAX_ROWS / 2, Hkv);
+  // Tokens a workgroup: as many as give its threads four pieces each where that
+  // makes some hundreds of workgroups, else one each: one piece / four, us a call in
+  // a graph: 4 heads of 64, 16 tokens 2.7 / 3.7, 4096 3.9 / 4.5, 16383 8.7 / 7.6; 8
+  // of 128, 16 2.7 / 3.8, 2048 5.0 / 5.3, 4096 8.4 / 7.3, 16383 27.0 / 22.8.
+  const int pieces = 2 * Hkv * (D / 8);
+  int tok = std::max(1, std::min(16, 1024 / pieces));
+  if (T < (int64_t)640 * tok) tok = std::max(1, std::min(16, 256 / pieces));
   const int64_t wgs = (T + tok - 1) / tok;
 #define LFS_STORE(DD, VEC)                                                                                            \
   hipLaunchKernelGGL((store_kvcache_fp8_kernel<DD, VEC>), dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,     \

@@ -19,7 +19,18 @@
 //          same XCD and find them in its L2.
 //  rest    the walk of pool_wave.h from the prefix's end on, shared by the
 //          balanced split of decode_wave.h.  A group of one sequence has no
-//          prefix here, its whole context is rest.
+//          prefix here, its whole context is rest; from two on it pays (64
+//          sequences behind 4096 tokens each pair, four, eight shares: 145, 88, 52
+//          us of 32 / 8 heads of 128, 162 to 174 by themselves; of 16 / 4 of 64 63,
+//          38, 23 and 57 to 59).
+// What it takes (us, in all; alone the roles 65 and 57): 128 sequences of 64 to 1024
+// tokens behind 16384 shared ones, 32 / 8 heads of 128: 93, of which the merge 11,
+// where the decode that reads every context by itself takes 1220; 64 sequences in
+// 3 groups behind 1536 to 3584 tokens, 16 / 4 of 64: 23 and 47.  Bound: at the first
+// the matrix cores' work beside the reads (a CU has one workgroup of each role), at
+// the second six dependent round trips (boundaries, lengths, table, rows) and the
+// merge's launch.  Each workgroup taking a share of both roles, half of them in
+// either order, took 116 and 32: twice the parts, and twice the scans.
 // Group boundaries are read on the device: a running maximum of cu_groups,
 // clipped to the batch, so that any values keep every access in bounds.
 #include "pool_wave.h"

@@ -35,7 +35,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <int D, bool FP8>
 struct PoolGeom {
   static constexpr int ES = FP8 ? 1 : 2;             // bytes of a value
-  static constexpr int T = FP8 || D == 64 ? 64 : 32;   // tokens per tile
+  // Tokens per tile (8 or 16 KiB).  Codes in heads of 64: 64 sequences of 128 to 4096
+  // tokens 22.7 us, in tiles of 128 26.5 (fewer, longer steps at a range's ends).
+  static constexpr int T = FP8 || D == 64 ? 64 : 32;
   static constexpr int NG = T / 16;                  // 16-token groups
   static constexpr int TU = (T + 63) / 64;           // tokens per lane, one each: its scale, its group's block
   static constexpr int KL = D * ES / 64;             // 16-byte K loads per lane and group
@@ -57,8 +59,8 @@ __device__ __forceinline__ v8bf codes_bf16(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(v8bf, make_uint4(bf16_lo(a), bf16_hi(a), bf16_lo(b), bf16_hi(b)));
 }
 
-// Tokens t0 .. t1 - 1 of a context (t0 a multiple of 16, of T or the block size's
-// end where ONE), for kv head kh: G query heads at q, the partial to rows prow ..
+// Tokens t0 .. t1 - 1 of a context (t0 a multiple of 16; where ONE a tile from t0 on
+// lies in one block), for kv head kh: G query heads at q, the partial to rows prow ..
 // or, where out is given, the normalised output there.
 struct PoolRange {
   const int32_t* btrow;
