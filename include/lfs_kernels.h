@@ -699,7 +699,7 @@ int lfs_scatter_add_weighted(const void* x, int32_t x_is_f32, int64_t ldx, const
  *   s = max(amax over the head's D values, 1e-4) * fp32(1/448),
  *   code = e4m3fn(clamp(x / s, -448, 448))
  * as lfs_act_quant with a group of D.  Two tokens of one slot leave either's
- * values.  D = 64 or 128; caches 8-byte aligned.
+ * values.  D = 64 or 128, at most 512 kv heads; caches 8-byte aligned.
  */
 int lfs_store_kvcache_fp8(const void* key, int64_t k_stride_t, const void* value, int64_t v_stride_t,
                           void* k_cache, void* v_cache, float* k_scale, float* v_scale,
@@ -723,7 +723,8 @@ int lfs_load_kvcache_fp8(const void* k_cache, const void* v_cache, const float* 
  * paged_decode_fp8: lfs_paged_decode over such a pool (keys code * k_scale,
  * values code * v_scale, fp32), which splits the work itself.  Codes and scales
  * of visible tokens must be finite.  k_scale and v_scale 16-byte aligned; a
- * workspace of lfs_paged_decode_fp8_workspace_bytes bytes, 16-byte aligned.
+ * workspace of lfs_paged_decode_fp8_workspace_bytes bytes (0 for B > 8192),
+ * 16-byte aligned.
  */
 int64_t lfs_paged_decode_fp8_workspace_bytes(int64_t B, int32_t num_q_heads, int32_t head_dim);
 int lfs_paged_decode_fp8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -738,9 +739,11 @@ int lfs_paged_decode_fp8(const void* q, const void* k_cache, const void* v_cache
  * have their first blocks in common, which are then read once a group.  Rows
  * cu_groups[g] .. cu_groups[g + 1] - 1 (int32 [num_groups + 1], non-decreasing)
  * are group g; the first shared_blocks[g] (int32) entries of their block tables
- * must be equal.  Rows of no group share nothing; a context may end within the
- * shared blocks.  A workspace of lfs_paged_decode_shared_workspace_bytes bytes,
- * 16-byte aligned.
+ * must be equal (they are read through the group's first row).  Rows of no group
+ * share nothing; a context may end within the shared blocks.  Boundaries are
+ * clipped to the batch, and so are shared blocks to the table.  At most 8192
+ * sequences and groups.  A workspace of lfs_paged_decode_shared_workspace_bytes
+ * bytes, 16-byte aligned.
  */
 int64_t lfs_paged_decode_shared_workspace_bytes(int64_t B, int64_t num_groups, int32_t num_q_heads,
                                                 int32_t num_kv_heads, int32_t head_dim);

@@ -39,7 +39,6 @@ struct PoolGeom {
   // tokens 22.7 us, in tiles of 128 26.5 (fewer, longer steps at a range's ends).
   static constexpr int T = FP8 || D == 64 ? 64 : 32;
   static constexpr int NG = T / 16;                  // 16-token groups
-  static constexpr int TU = (T + 63) / 64;           // tokens per lane, one each: its scale, its group's block
   static constexpr int KL = D * ES / 64;             // 16-byte K loads per lane and group
   static constexpr int DB = D / 16;                  // V values per lane and token
   static constexpr int VD = DB * ES / 4;             // and their dwords
@@ -73,7 +72,7 @@ struct PoolRange {
 template <int D, bool FP8, bool ONE>
 struct PoolWave {
   using Geo = PoolGeom<D, FP8>;
-  static constexpr int NG = Geo::NG, TU = Geo::TU, KL = Geo::KL, DB = Geo::DB, T = Geo::T, ES = Geo::ES, VD = Geo::VD;
+  static constexpr int NG = Geo::NG, KL = Geo::KL, DB = Geo::DB, T = Geo::T, ES = Geo::ES, VD = Geo::VD;
   // Every row is read once: nontemporal, but where a head's codes are half a line,
   // whose other half another wave asks for (64 sequences of 8192 tokens, 16 / 4
   // heads of 64: 65.4 us nontemporal, 61.1 not; of 128 92 and 102).
@@ -81,7 +80,7 @@ struct PoolWave {
   struct Tile {
     u32x4 k[NG][KL];
     uint32_t v[NG][4][VD];
-    float ks[TU], vs[TU];
+    float ks, vs;  // of token `lane`
     int n;         // tokens up to the range's end (at most T)
     uint32_t bad;  // bit g: group g lies in no block of the pool
     bool first, last;  // of its range
@@ -94,9 +93,10 @@ struct PoolWave {
   const float *ksc, *vsc;
   v8bf q[D / 32], qnext[D / 32];
   float scale_log2, acc[DB][4], m_run, l_run;
-  // the tile asked for: its range, place, block ids and offsets, and the next's columns
+  // the tile asked for: its range and place; lanes 16 g .. 16 g + 15 hold the block id
+  // of its 16-token group g and the offset there, and the column of the next's
   PoolRange ask_at;
-  int pos, ask_n, col[TU], off[TU], ids[TU], idoff[TU], sq, sr;
+  int pos, ask_n, col, off, id, idoff, sq, sr;
   bool ask_first, ask_last, more;
 
   __device__ __forceinline__ void init(int lane_, const void* kc_, const void* vc_, const float* ksc_, const float* vsc_,
@@ -117,26 +117,20 @@ struct PoolWave {
     if (ask_first) {
       more = next(ask_at);
       pos = ask_at.t0;
-#pragma unroll
-      for (int u = 0; u < TU; ++u) {
-        const unsigned t = pos + u * 64 + (lane >> 4) * 16, c = t / (unsigned)BS;
-        col[u] = (int)c;
-        off[u] = (int)(t - c * BS);
-      }
+      const unsigned t = pos + (lane >> 4) * 16;
+      col = (int)(t / (unsigned)BS);
+      off = (int)t - col * BS;
     }
     ask_n = more ? min(T, ask_at.t1 - pos) : 0;
     pos += T;
     ask_last = pos >= ask_at.t1;
-#pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      const int end = (int)((unsigned)(ask_at.t1 - 1) / (unsigned)BS);
-      const int id = ask_at.btrow[min(col[u], end)];
-      ids[u] = col[u] <= end ? id : -1;
-      idoff[u] = off[u];
-      col[u] += sq;
-      off[u] += sr;
-      if (off[u] >= BS) off[u] -= BS, ++col[u];
-    }
+    const int end = (int)((unsigned)(ask_at.t1 - 1) / (unsigned)BS);
+    const int at = ask_at.btrow[min(col, end)];
+    id = col <= end ? at : -1;
+    idoff = off;
+    col += sq;
+    off += sr;
+    if (off >= BS) off -= BS, ++col;
   }
   // Load the tile whose ids were asked for.
   __device__ __forceinline__ void load(Tile& t) {
@@ -154,29 +148,23 @@ struct PoolWave {
         qnext[c] = __builtin_bit_cast(v8bf, __builtin_amdgcn_raw_buffer_load_b128(qr, ((j & 7) * D + d) * 2, 0, 0));
       }
     }
-    uint32_t bad = 0;
-    int64_t at[TU];
-#pragma unroll
-    for (int u = 0; u < TU; ++u) {
-      const bool ok = ids[u] >= 0 && (int64_t)ids[u] < NB;
-      const int64_t slot = (int64_t)(ok ? ids[u] : 0) * BS + idoff[u];
-      at[u] = slot * row + (int64_t)kh * (D * ES);
-      if constexpr (FP8) {
-        const int64_t sat = ((int64_t)(ok ? ids[u] : 0) * Hkv + kh) * BS + idoff[u] + (lane & 15);
-        const bool use = ok && u * 64 + lane < n;
-        const float a = ksc[sat], b = vsc[sat];
-        t.ks[u] = use ? a : 0.f;
-        t.vs[u] = use ? b : 0.f;
-      }
-      const uint64_t m = __ballot(!ok);
-#pragma unroll
-      for (int k = 0; k < (NG < 4 ? NG : 4); ++k) bad |= (uint32_t)(m >> (16 * k) & 1) << (u * 4 + k);
+    const bool ok = id >= 0 && (int64_t)id < NB;
+    const int64_t blk = ok ? id : 0, at = (blk * BS + idoff) * row + (int64_t)kh * (D * ES);
+    if constexpr (FP8) {
+      const int64_t sat = (blk * Hkv + kh) * BS + idoff + (lane & 15);
+      const bool use = ok && lane < n;
+      const float a = ksc[sat], b = vsc[sat];
+      t.ks = use ? a : 0.f;
+      t.vs = use ? b : 0.f;
     }
+    const uint64_t m = __ballot(!ok);
+    uint32_t bad = 0;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) bad |= (uint32_t)(m >> (16 * g) & 1) << g;
     t.bad = bad;
     auto base_of = [&](int g) {
-      const int u = g >> 2, l = (g & 3) * 16;
-      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)at[u], l);
-      const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at[u] >> 32), l);
+      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)at, 16 * g);
+      const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at >> 32), 16 * g);
       return (int64_t)((uint64_t)hi << 32 | lo);
     };
     const int kat = j * row + kq * 16, vat = kq * 4 * row + j * (DB * ES);
@@ -228,11 +216,8 @@ struct PoolWave {
   // pw: the wave's LDS slice, 2 T floats (FP8).
   __device__ __forceinline__ void compute(const Tile& t, float* __restrict__ pw) {
     if constexpr (FP8) {
-#pragma unroll
-      for (int u = 0; u < TU; ++u) {
-        pw[u * 64 + lane] = t.ks[u];
-        pw[T + u * 64 + lane] = t.vs[u];
-      }
+      pw[lane] = t.ks;
+      pw[T + lane] = t.vs;
       wave_lds_sync();
     }
     float s[NG][4];

@@ -21,7 +21,11 @@ Interface (nano-vLLM style, as the runner expects):
     logits = model.compute_logits(hidden)             # bf16 [T, vocab]
 
 DecodeModelConfig also gives the attention a sliding window with sinks and
-norms per head (qk_head_norm_rope_store), which the reference has not.
+norms per head (qk_head_norm_rope_store), which the reference has not.  Where
+the runner attaches a pool in 8 bits (k_scale and v_scale beside k_cache and
+v_cache), the attention stores codes and scales and decodes over them
+(forward_fp8); where Context.cu_groups is set, it decodes over shared prefixes
+(paged_attention_decode_shared).
 
 Kernels per layer: add_rmsnorm (+act_quant) -> qkv FP8 GEMM ->
 qk_norm_rope_store -> paged decode (split + merge with the act_quant of its

@@ -24,6 +24,12 @@ RPC):
                       over static buffers (:339-392)
 The decode slot is bt[-1]*BS + last_block_num_tokens - 1 with the corrected
 last_block_num_tokens (a full last block counts BS tokens).
+
+Beyond the reference, in the configuration: "kv_dtype" torch.float8_e4m3fn makes
+a pool in 8 bits (kv_cache holds codes, kv_scales [2, L, NB, Hkv, BS] their
+scales); "share_prefixes" decodes neighbouring sequences whose block tables begin
+alike over what they share (shared_groups).  Before sampling, the logits go
+through the penalties, biases and masks of their sequences (penalise).
 """
 from __future__ import annotations
 

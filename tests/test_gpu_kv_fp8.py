@@ -112,6 +112,25 @@ def test_store_is_act_quant_per_head(Hkv, D, T, BS, layout):
         assert np.array_equal(np.isnan(got_s), np.isnan(want_s))
 
 
+@pytest.mark.parametrize("Hkv,D,T", [(4, 64, 10301), (8, 128, 2601), (3, 64, 16385), (33, 128, 700), (512, 64, 5)])
+def test_store_many_tokens_and_heads(Hkv, D, T):
+    """Several pieces a thread, and more heads than a workgroup has pieces for."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    key, value = (torch.randn(T, Hkv, D, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    NB, BS = -(-T // 16) + 1, 16
+    pool = poisoned(NB, BS, Hkv, D)
+    slots = torch.randperm(NB * BS, generator=g, device=DEV)[:T]
+    K.store_kvcache_fp8(key, value, *pool, slots)
+    for x, cache, scale in ((key, pool[0], pool[2]), (value, pool[1], pool[3])):
+        codes, s = K.act_quant(x.view(T, Hkv * D), block_size=D)  # bit for bit the oracle's (tests/test_gpu_fp8.py)
+        assert torch.equal(cache.view(torch.uint8).flatten(0, 1)[slots].view(T, -1), codes.view(torch.uint8))
+        assert torch.equal(scale.transpose(1, 2).flatten(0, 1)[slots], s)
+        assert int(torch.isnan(scale).sum()) == (NB * BS - T) * Hkv
+    if Hkv == 512:
+        with pytest.raises(ValueError, match="512 kv heads"):
+            K.store_kvcache_fp8(key.repeat(1, 2, 1), value.repeat(1, 2, 1), *poisoned(1, 16, 1024, 64), slots)
+
+
 @pytest.mark.parametrize("Hkv,D", [(4, 64), (8, 128), (3, 64), (1, 128)])
 @pytest.mark.parametrize("BS", [16, 48, 256])
 def test_load_is_the_rounded_product(Hkv, D, BS):

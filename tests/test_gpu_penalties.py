@@ -59,7 +59,8 @@ def check(logits, tokens=None, prompts=None, lens=None, rep=None, pres=None, fre
         fine = np.isfinite(want)
         assert np.array_equal(out[b][~fine], want[~fine], equal_nan=True), b
         tol = half * np.abs(want) + (4 + len(pairs)) * 2.0 ** -24 * size + 1e-38
-        bad = np.flatnonzero(~(np.abs(out[b] - want) <= tol) & fine)
+        with np.errstate(invalid="ignore"):
+            bad = np.flatnonzero(~(np.abs(out[b] - want) <= tol) & fine)
         assert not len(bad), (b, bad[:5], out[b][bad[:5]], want[bad[:5]])
     return got
 
@@ -109,6 +110,19 @@ def test_histories(V):
           rep=np.full(9, 1.3), pres=np.full(9, 0.4), freq=np.full(9, 0.01))
     check(logits_of(rng, 2, V), tokens[:2], np.array([0, 0]), np.array([-4, 0]), rep=[1.5, 1.5], pres=[1, 1], freq=[1, 1])
     check(logits_of(rng, 2, V), tokens[:2, :0], np.array([0, 0]), np.array([3, 0]), rep=[1.5, 1.5])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("L", [900, 17000])
+def test_large_batches(dtype, L):
+    """Large chunks, with counts of either width, biases and masks, rows at odd
+    addresses."""
+    rng = np.random.default_rng(L)
+    B, V = 24, 90001
+    tokens = (V * (rng.integers(0, 300, (B, L)) / 300) ** 3).astype(int)
+    check(logits_of(rng, B, V, dtype), tokens, rng.integers(0, L, B), rng.integers(0, L + 1, B), rep=rng.uniform(0.5, 2, B),
+          pres=rng.uniform(0, 2, B), freq=rng.uniform(0, 0.1, B), ids=rng.integers(0, V, (B, 30)),
+          bias=rng.normal(0, 9, (B, 30)), allowed=rng.random((B, V)) < 0.6)
 
 
 def test_prompt_tokens_are_repeated_but_not_counted():

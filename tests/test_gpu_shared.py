@@ -88,6 +88,7 @@ def test_groups(Hq, Hkv, D, BS):
     for groups in (
         [(2, [2 * BS + n for n in (1, 15, 16, 17, 63, 64, 65, 130)])],
         [(0, [1, 100]), (3, [3 * BS + 7] * 3), (1, []), (5, [5 * BS + 300, 5 * BS, 5 * BS + 1]), (2, [2 * BS + 40])],
+        [(3, [2 * BS + 5, 7, BS + 1]), (2, [BS + 15, BS + 3, 0])],
         [(4, [4 * BS + 9, 3 * BS, BS + 1, 1, 0, 4 * BS - 1, 5 * BS]), (1, [0, 0]), (2, [BS, 3])],
     ):
         check(rng, groups, BS, Hq, Hkv, D, str(groups)[:60])
