@@ -752,18 +752,25 @@ def _shared_workspace(device: int, *shape: int) -> int:
 
 def _decode_args(q: torch.Tensor, context_lens: torch.Tensor, block_tables: torch.Tensor, need: int,
                  workspace: Optional[torch.Tensor], quant: bool):
-    """Checks of what a decode takes beside the pool; its workspace and outputs."""
+    """Checks of what a decode takes beside the pool; its workspace and outputs,
+    and the batch, the table's row stride and width."""
     B, Hq, D = q.shape
-    assert block_tables.dim() == 2 and block_tables.size(0) == B and block_tables.stride(1) == 1, \
-        "block_tables must be [B, max_blocks]"
-    assert context_lens.shape == (B,) and context_lens.is_contiguous(), "context_lens must be contiguous [B]"
-    if not (q.dtype is torch.bfloat16 and context_lens.dtype is torch.int64 and block_tables.dtype is torch.int32):
+    tables = block_tables.shape
+    if not (q.dtype is torch.bfloat16 and q.is_contiguous() and len(tables) == 2 and tables[0] == B
+            and block_tables.dtype is torch.int32 and context_lens.dtype is torch.int64 and context_lens.shape == (B,)
+            and context_lens.is_contiguous()):
         _dtype(q, torch.bfloat16, "q")
+        assert q.is_contiguous(), "q must be contiguous [B, Hq, D]"
+        assert block_tables.dim() == 2 and block_tables.size(0) == B, "block_tables must be [B, max_blocks]"
+        assert context_lens.shape == (B,) and context_lens.is_contiguous(), "context_lens must be contiguous [B]"
         _dtype(context_lens, torch.int64, "context_lens")
         _dtype(block_tables, torch.int32, "block_tables")
+    row, unit = block_tables.stride()
+    assert unit == 1, "block_tables must be [B, max_blocks] with unit column stride"
     if workspace is not None:
         _on_gpu(q, workspace)
         assert workspace.is_contiguous(), "workspace must be contiguous"
+        need = workspace.nbytes
     elif need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     o, oq, os_ = torch.empty_like(q), None, None
@@ -771,22 +778,21 @@ def _decode_args(q: torch.Tensor, context_lens: torch.Tensor, block_tables: torc
         assert Hq * D % 128 == 0, "the quantised output needs Hq * D to be a multiple of 128"
         oq = torch.empty(B, Hq * D, dtype=FP8, device=q.device)
         os_ = torch.empty(B, Hq * D // 128, dtype=torch.float32, device=q.device)
-    return workspace, o, oq, os_
+    return _ptr(workspace), need, o, oq, os_, (row if B > 1 else tables[1]), tables[1]
 
 
 def _decode_fp8(q, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables, scale, workspace, quant):
-    assert q.dim() == 3 and q.is_contiguous(), "q must be contiguous [B, Hq, D]"
+    assert q.dim() == 3, "q must be [B, Hq, D]"
     NB, BS, Hkv, Dk = _fp8_pool(k_cache, v_cache, k_scale, v_scale)
     B, Hq, D = q.shape
     assert Dk == D, "head_dim mismatch between q and the caches"
     _on_gpu(q, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables)
-    workspace, o, oq, os_ = _decode_args(q, context_lens, block_tables, _fp8_workspace(q.get_device(), B, Hq, D),
-                                         workspace, quant)
+    ws, ws_bytes, o, oq, os_, row, width = _decode_args(q, context_lens, block_tables,
+                                                        _fp8_workspace(q.get_device(), B, Hq, D), workspace, quant)
     _launch("paged_attention_decode", _lib.load().lfs_paged_decode_fp8, q,
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            context_lens.data_ptr(), block_tables.data_ptr(), _row_stride(block_tables), o.data_ptr(), _ptr(workspace),
-            0 if workspace is None else workspace.nbytes, B, Hq, Hkv, D, BS, NB, block_tables.size(1),
-            1.0 / math.sqrt(D) if scale is None else scale, _ptr(oq), _ptr(os_))
+            context_lens.data_ptr(), block_tables.data_ptr(), row, o.data_ptr(), ws, ws_bytes, B, Hq, Hkv, D, BS, NB,
+            width, 1.0 / math.sqrt(D) if scale is None else scale, _ptr(oq), _ptr(os_))
     return (o, oq, os_) if quant else o
 
 
@@ -807,11 +813,12 @@ def paged_attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cach
     grid depends only on the shapes, so the call can be captured in a HIP graph,
     with a ``workspace`` of ``paged_decode_shared_workspace_bytes`` bytes of its
     own; the groups may change between replays."""
-    assert q.dim() == 3 and q.is_contiguous(), "q must be contiguous [B, Hq, D]"
-    assert k_cache.dim() == 4 and k_cache.is_contiguous() and v_cache.is_contiguous() \
-        and v_cache.shape == k_cache.shape, "caches must be contiguous [num_blocks, block_size, Hkv, D]"
+    assert q.dim() == 3, "q must be [B, Hq, D]"
+    shape = k_cache.shape
+    assert len(shape) == 4 and v_cache.shape == shape and k_cache.is_contiguous() and v_cache.is_contiguous(), \
+        "caches must be contiguous [num_blocks, block_size, Hkv, D]"
     B, Hq, D = q.shape
-    NB, BS, Hkv, Dk = k_cache.shape
+    NB, BS, Hkv, Dk = shape
     assert Dk == D, "head_dim mismatch between q and the caches"
     assert shared_blocks.dim() == 1 and shared_blocks.is_contiguous(), "shared_blocks must be contiguous [num_groups]"
     NG = shared_blocks.size(0)
@@ -822,12 +829,11 @@ def paged_attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cach
         _dtype(v_cache, torch.bfloat16, "v_cache")
         _dtype(cu_groups, torch.int32, "cu_groups")
         _dtype(shared_blocks, torch.int32, "shared_blocks")
-    workspace, o, oq, os_ = _decode_args(q, context_lens, block_tables,
-                                         _shared_workspace(q.get_device(), B, NG, Hq, Hkv, D), workspace, quant)
+    ws, ws_bytes, o, oq, os_, row, width = _decode_args(
+        q, context_lens, block_tables, _shared_workspace(q.get_device(), B, NG, Hq, Hkv, D), workspace, quant)
     _launch("paged_attention_decode_shared", _lib.load().lfs_paged_decode_shared, q,
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(),
-            _row_stride(block_tables), cu_groups.data_ptr(), shared_blocks.data_ptr(), NG, o.data_ptr(),
-            _ptr(workspace), 0 if workspace is None else workspace.nbytes, B, Hq, Hkv, D, BS, NB, block_tables.size(1),
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), row,
+            cu_groups.data_ptr(), shared_blocks.data_ptr(), NG, o.data_ptr(), ws, ws_bytes, B, Hq, Hkv, D, BS, NB, width,
             1.0 / math.sqrt(D) if scale is None else scale, _ptr(oq), _ptr(os_))
     return (o, oq, os_) if quant else o
 
