@@ -774,7 +774,10 @@ __global__ __launch_bounds__(128) void paged_decode_merge_quant_group(
 }
 
 // tp[b] = sum of count(b') for b' < b, b <= B <= BAL_MAXB, in LDS (each thread a
-// run of sequences); wsum: one int per wave.
+// run of sequences, from scan_first on); wsum: one int per wave.
+__device__ __forceinline__ int scan_first(int B) {
+  return min(B, (int)threadIdx.x * ((B + (int)blockDim.x - 1) / (int)blockDim.x));
+}
 template <class Count>
 __device__ __forceinline__ void scan_tiles(int* tp, int* wsum, int B, Count&& count) {
   const int tid = threadIdx.x, nthr = blockDim.x, wave = tid >> 6, lane = tid & 63;

@@ -41,6 +41,7 @@ namespace {
 
 constexpr int SMEM = 2 * 4 * (BAL_MAXB + 8);  // scans of groups and sequences, then the tiles
 constexpr int PROWS = RW * NW;                // rows of a prefix unit
+constexpr int KNOWN = 512;                    // sequences whose prefix and length stay in LDS
 
 struct SharedArgs {
   const uint16_t *q, *kc, *vc;
@@ -77,8 +78,11 @@ __device__ __forceinline__ void scan_starts(const SharedArgs& a, int* starts, in
 }
 
 // Tokens of group g's prefix, of n sequences.
+__device__ __forceinline__ int64_t prefix_of(const SharedArgs& a, int blocks, int n) {
+  return n < 2 ? 0 : (int64_t)min(max(blocks, 0), a.max_blocks) * a.BS;
+}
 __device__ __forceinline__ int64_t prefix_tokens(const SharedArgs& a, int g, int n) {
-  return n < 2 ? 0 : (int64_t)min(max(a.shared[g], 0), a.max_blocks) * a.BS;
+  return prefix_of(a, n < 2 ? 0 : a.shared[g], n);
 }
 // Its 128-row tiles and 64-key tiles.
 __device__ __forceinline__ int row_tiles(const SharedArgs& a, int n) { return (n * a.G + PROWS - 1) / PROWS; }
@@ -310,10 +314,12 @@ template <int D>
 __device__ __forceinline__ void prefix_role(const SharedArgs& a, uint8_t* smem, int* wsum, int w) {
   int* starts = reinterpret_cast<int*>(smem);
   int* units = starts + BAL_MAXB + 8;
+  // the thread's first group's blocks are in flight while the boundaries are scanned
+  const int g0 = scan_first(a.NG), blocks0 = g0 < a.NG ? a.shared[g0] : 0;
   scan_starts(a, starts, wsum);
   scan_tiles(units, wsum, a.NG, [&](int g) {
     const int n = starts[g + 1] - starts[g];
-    return row_tiles(a, n) * a.Hkv * key_tiles(prefix_tokens(a, g, n));
+    return row_tiles(a, n) * a.Hkv * key_tiles(prefix_of(a, g == g0 ? blocks0 : a.shared[g], n));
   });
   if (w == 0)
     for (int i = threadIdx.x; i <= a.NG; i += 256) a.starts[i] = starts[i], a.punits[i] = units[i];
@@ -353,18 +359,21 @@ __device__ __forceinline__ void prefix_role(const SharedArgs& a, uint8_t* smem, 
 // The walk works on virtual workgroups of hg waves, one per kv head of a group of
 // heads: 4 / hg of them here.
 template <int D, bool ONE>
-__device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, int* wsum, int w) {
+__device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, int* known, int* wsum, int w) {
   constexpr int T = PoolGeom<D, false>::T;
   int* starts = reinterpret_cast<int*>(smem);
   int* tp = starts + BAL_MAXB + 8;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int64_t cap = (int64_t)a.max_blocks * a.BS;
+  const int b0 = scan_first(a.B);
+  const int64_t len0 = b0 < a.B ? a.ctx_lens[b0] : 0;  // in flight while the boundaries are scanned
   scan_starts(a, starts, wsum);
   scan_tiles(tp, wsum, a.B, [&](int b) {
     int64_t tokens;
     const int g = group_of(a, starts, b, tokens);
     if (w == 0) a.group[b] = g;
-    const int64_t L = min(a.ctx_lens[b], cap) - tokens;
+    const int64_t Lc = min(b == b0 ? len0 : a.ctx_lens[b], cap), L = Lc - tokens;
+    if (b < KNOWN) known[2 * b] = (int)tokens, known[2 * b + 1] = (int)max((int64_t)0, Lc);
     return L > 0 ? (int)((L + T - 1) / T) : 0;
   });
   if (w == 0)
@@ -399,10 +408,16 @@ __device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, in
           const int kh = grp * a.hg + head, i1 = (int)(i0 + (stop - u));
           u = stop;
           if (kh >= a.Hkv) continue;
-          int64_t tokens;
-          group_of(a, starts, b, tokens);
-          const int start = __builtin_amdgcn_readfirstlane((int)tokens);
-          const int L = __builtin_amdgcn_readfirstlane((int)min(a.ctx_lens[b], cap));
+          int start, L;
+          if (b < KNOWN) {
+            start = __builtin_amdgcn_readfirstlane(known[2 * b]);
+            L = __builtin_amdgcn_readfirstlane(known[2 * b + 1]);
+          } else {
+            int64_t tokens;
+            group_of(a, starts, b, tokens);
+            start = __builtin_amdgcn_readfirstlane((int)tokens);
+            L = __builtin_amdgcn_readfirstlane((int)min(a.ctx_lens[b], cap));
+          }
           r.btrow = a.bt + (int64_t)b * a.bt_stride;
           r.q = a.q + ((int64_t)b * a.Hkv + kh) * a.G * D;
           r.out = nullptr;
@@ -418,11 +433,11 @@ __device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, in
 template <int D, bool ONE>
 __global__ __launch_bounds__(256, 2) void paged_shared_kernel(SharedArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[SMEM];
-  __shared__ int wsum[NW];
+  __shared__ int known[2 * KNOWN], wsum[NW];
   static_assert(SMEM >= 4 * KT * 2 * D, "K and V tiles, two each");
   const int w = blockIdx.x;
   if (w < a.nprefix) prefix_role<D>(a, smem, wsum, w);
-  else rest_role<D, ONE>(a, smem, wsum, w - a.nprefix);
+  else rest_role<D, ONE>(a, smem, known, wsum, w - a.nprefix);
 }
 
 // One wave per 64 elements of an output row: the weights of up to 64 parts at a
