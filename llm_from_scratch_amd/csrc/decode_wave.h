@@ -773,18 +773,25 @@ __global__ __launch_bounds__(128) void paged_decode_merge_quant_group(
   }
 }
 
-// tp[b] = sum of count(b') for b' < b, b <= B <= BAL_MAXB, in LDS (each thread a
-// run of sequences, from scan_first on); wsum: one int per wave.
+// tp[b] = sum of count(b') for b' < b, b <= B <= BAL_MAXB, in LDS, each thread a run
+// of sequences (lo .. hi - 1): scan_tiles leaves the sums of each run there and
+// returns what all have; place_tiles adds what lies before them and calls
+// visit(b, tp[b], tp[b + 1]), so that whoever looks for the sequence of a tile finds
+// it without a search.  wsum: one int per wave.
+struct TileScan {
+  int lo, hi, before, total;
+};
 __device__ __forceinline__ int scan_first(int B) {
   return min(B, (int)threadIdx.x * ((B + (int)blockDim.x - 1) / (int)blockDim.x));
 }
 template <class Count>
-__device__ __forceinline__ void scan_tiles(int* tp, int* wsum, int B, Count&& count) {
+__device__ __forceinline__ TileScan scan_tiles(int* tp, int* wsum, int B, Count&& count) {
   const int tid = threadIdx.x, nthr = blockDim.x, wave = tid >> 6, lane = tid & 63;
-  const int per = (B + nthr - 1) / nthr;
-  const int lo = min(B, tid * per), hi = min(B, lo + per);
+  TileScan s;
+  s.lo = scan_first(B);
+  s.hi = min(B, s.lo + (B + nthr - 1) / nthr);
   int run = 0;
-  for (int i = lo; i < hi; ++i) tp[i + 1] = run += count(i);
+  for (int i = s.lo; i < s.hi; ++i) tp[i + 1] = run += count(i);
   int incl = run;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -793,10 +800,23 @@ __device__ __forceinline__ void scan_tiles(int* tp, int* wsum, int B, Count&& co
   }
   if (lane == 63) wsum[wave] = incl;
   __syncthreads();
-  int excl = incl - run;
-  for (int w = 0; w < wave; ++w) excl += wsum[w];
-  for (int i = lo; i < hi; ++i) tp[i + 1] += excl;
-  if (tid == 0) tp[0] = 0;
+  s.before = incl - run;
+  s.total = 0;
+  for (int w = 0; w < nthr >> 6; ++w) {
+    if (w < wave) s.before += wsum[w];
+    s.total += wsum[w];
+  }
+  return s;
+}
+template <class Visit>
+__device__ __forceinline__ void place_tiles(int* tp, const TileScan& s, Visit&& visit) {
+  int at = s.before;
+  for (int i = s.lo; i < s.hi; ++i) {
+    const int next = tp[i + 1] += s.before;
+    visit(i, at, next);
+    at = next;
+  }
+  if (threadIdx.x == 0) tp[0] = 0;
   __syncthreads();
 }
 

@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256) void paged_fp8_kernel(
   constexpr int T = PoolGeom<D, true>::T;
   __shared__ __attribute__((aligned(16))) float scales[4][2 * T];
   __shared__ int tp[SCAN ? BAL_MAXB + 1 : 1], lens[SCAN ? BAL_MAXB : 1];
-  __shared__ int wsum[4];
+  __shared__ int wsum[4], found;
   const int tid = threadIdx.x, wpg = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int cap = max_blocks * BS;
@@ -65,25 +65,22 @@ __global__ __launch_bounds__(256) void paged_fp8_kernel(
         },
         scales[wave], ws_o, ws_ml);
   } else {
-    scan_tiles(tp, wsum, B, [&](int b) {
+    const TileScan scan = scan_tiles(tp, wsum, B, [&](int b) {
       const int L = (int)max((int64_t)0, min(ctx_lens[b], (int64_t)cap));
       lens[b] = L;
       return (L + T - 1) / T;
     });
-    if (blockIdx.x == 0)
-      for (int i = tid; i <= B; i += blockDim.x) tp_out[i] = tp[i];
-    const unsigned total = (unsigned)ngroups * (unsigned)tp[B], nwg = gridDim.x;
+    const unsigned total = (unsigned)ngroups * (unsigned)scan.total, nwg = gridDim.x;
     const unsigned Ct = max(1u, (total + nwg - 1) / nwg);
     unsigned u = blockIdx.x * Ct;
     const unsigned u_end = min(total, u + Ct);
+    place_tiles(tp, scan, [&](int i, int before, int after) {
+      if ((unsigned)ngroups * (unsigned)before <= u && u < (unsigned)ngroups * (unsigned)after) found = i;
+    });
+    if (blockIdx.x == 0)
+      for (int i = tid; i <= B; i += blockDim.x) tp_out[i] = tp[i];
     if (u >= u_end) return;
-    int b = 0, b_hi = B - 1;  // the largest b with ngroups * tp[b] <= u
-    while (b < b_hi) {
-      const int mid = (b + b_hi + 1) >> 1;
-      if ((unsigned)ngroups * (unsigned)tp[mid] <= u) b = mid;
-      else b_hi = mid - 1;
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
+    int b = __builtin_amdgcn_readfirstlane(found);
     w.run(
         [&](PoolRange& r) {
           while (u < u_end) {

@@ -41,7 +41,7 @@ namespace {
 
 constexpr int SMEM = 2 * 4 * (BAL_MAXB + 8);  // scans of groups and sequences, then the tiles
 constexpr int PROWS = RW * NW;                // rows of a prefix unit
-constexpr int KNOWN = 512;                    // sequences whose prefix and length stay in LDS
+constexpr int KNOWN = 512;                    // sequences whose prefix and length stay in LDS, groups whose blocks do
 
 struct SharedArgs {
   const uint16_t *q, *kc, *vc;
@@ -56,8 +56,18 @@ struct SharedArgs {
   float scale_log2;
 };
 
-// starts[g]: running maximum of the boundaries clipped to 0 .. B, in LDS.
-__device__ __forceinline__ void scan_starts(const SharedArgs& a, int* starts, int* wmax) {
+// What a workgroup keeps in LDS beside its scans.
+struct SharedLds {
+  int wsum[NW], found[NW];
+  int blocks[KNOWN];       // shared by a group
+  int prefix[2 * KNOWN];   // of a sequence: tokens of its group's prefix, length
+};
+
+// starts[g]: running maximum of the boundaries clipped to 0 .. B, in LDS, with the
+// first groups' shared blocks.
+__device__ __forceinline__ void scan_starts(const SharedArgs& a, int* starts, SharedLds& s) {
+  int* wmax = s.wsum;
+  for (int g = threadIdx.x; g < min(a.NG, KNOWN); g += 256) s.blocks[g] = a.shared[g];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, n = a.NG + 1;
   const int per = (n + 255) / 256, lo = min(n, tid * per), hi = min(n, lo + per);
   int run = 0;
@@ -84,12 +94,16 @@ __device__ __forceinline__ int64_t prefix_of(const SharedArgs& a, int blocks, in
 __device__ __forceinline__ int64_t prefix_tokens(const SharedArgs& a, int g, int n) {
   return prefix_of(a, n < 2 ? 0 : a.shared[g], n);
 }
+// (after scan_starts)
+__device__ __forceinline__ int64_t prefix_tokens(const SharedArgs& a, const SharedLds& s, int g, int n) {
+  return g < KNOWN ? prefix_of(a, s.blocks[g], n) : prefix_tokens(a, g, n);
+}
 // Its 128-row tiles and 64-key tiles.
 __device__ __forceinline__ int row_tiles(const SharedArgs& a, int n) { return (n * a.G + PROWS - 1) / PROWS; }
 __device__ __forceinline__ int key_tiles(int64_t tokens) { return (int)((tokens + KT - 1) / KT); }
 
 // The group of sequence b (-1: none) and its prefix.
-__device__ __forceinline__ int group_of(const SharedArgs& a, const int* starts, int b, int64_t& tokens) {
+__device__ __forceinline__ int group_of(const SharedArgs& a, const SharedLds& s, const int* starts, int b, int64_t& tokens) {
   tokens = 0;
   if (a.NG == 0) return -1;
   int lo = 0, hi = a.NG;  // the last boundary at or before b
@@ -99,7 +113,7 @@ __device__ __forceinline__ int group_of(const SharedArgs& a, const int* starts, 
     else hi = mid - 1;
   }
   if (lo == a.NG || starts[lo] > b) return -1;
-  tokens = prefix_tokens(a, lo, starts[lo + 1] - starts[lo]);
+  tokens = prefix_tokens(a, s, lo, starts[lo + 1] - starts[lo]);
   return lo;
 }
 
@@ -311,33 +325,29 @@ __device__ __forceinline__ void prefix_unit(const SharedArgs& a, uint8_t* smem, 
 }
 
 template <int D>
-__device__ __forceinline__ void prefix_role(const SharedArgs& a, uint8_t* smem, int* wsum, int w) {
+__device__ __forceinline__ void prefix_role(const SharedArgs& a, uint8_t* smem, SharedLds& s, int w) {
   int* starts = reinterpret_cast<int*>(smem);
   int* units = starts + BAL_MAXB + 8;
-  // the thread's first group's blocks are in flight while the boundaries are scanned
-  const int g0 = scan_first(a.NG), blocks0 = g0 < a.NG ? a.shared[g0] : 0;
-  scan_starts(a, starts, wsum);
-  scan_tiles(units, wsum, a.NG, [&](int g) {
+  scan_starts(a, starts, s);
+  const TileScan scan = scan_tiles(units, s.wsum, a.NG, [&](int g) {
     const int n = starts[g + 1] - starts[g];
-    return row_tiles(a, n) * a.Hkv * key_tiles(prefix_of(a, g == g0 ? blocks0 : a.shared[g], n));
+    return row_tiles(a, n) * a.Hkv * key_tiles(prefix_tokens(a, s, g, n));
+  });
+  const unsigned total = scan.total, Ct = max(1u, (total + a.nprefix - 1) / a.nprefix);
+  unsigned u = w * Ct;
+  const unsigned u_end = min(total, u + Ct);
+  place_tiles(units, scan, [&](int g, int before, int after) {
+    if ((unsigned)before <= u && u < (unsigned)after) s.found[0] = g;
   });
   if (w == 0)
     for (int i = threadIdx.x; i <= a.NG; i += 256) a.starts[i] = starts[i], a.punits[i] = units[i];
-  const unsigned total = units[a.NG], Ct = max(1u, (total + a.nprefix - 1) / a.nprefix);
-  unsigned u = w * Ct;
-  const unsigned u_end = min(total, u + Ct);
   if (u >= u_end) return;
-  int g = 0, hi = a.NG - 1;  // the largest g with units[g] <= u: it has some
-  while (g < hi) {
-    const int mid = (g + hi + 1) >> 1;
-    if ((unsigned)units[mid] <= u) g = mid;
-    else hi = mid - 1;
-  }
+  int g = s.found[0];
   unsigned base = units[g];
   int first = starts[g], end = starts[g + 1];
   while (true) {
     const int n = end - first, rts = row_tiles(a, n);
-    const int64_t tokens = prefix_tokens(a, g, n);
+    const int64_t tokens = prefix_tokens(a, s, g, n);
     const unsigned nt = key_tiles(tokens), pairs = rts * a.Hkv;
     while (u < base + pairs * nt && u < u_end) {
       const unsigned pair = (u - base) / nt, k0 = (u - base) - pair * nt;
@@ -359,7 +369,7 @@ __device__ __forceinline__ void prefix_role(const SharedArgs& a, uint8_t* smem, 
 // The walk works on virtual workgroups of hg waves, one per kv head of a group of
 // heads: 4 / hg of them here.
 template <int D, bool ONE>
-__device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, int* known, int* wsum, int w) {
+__device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, SharedLds& s, int w) {
   constexpr int T = PoolGeom<D, false>::T;
   int* starts = reinterpret_cast<int*>(smem);
   int* tp = starts + BAL_MAXB + 8;
@@ -367,30 +377,31 @@ __device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, in
   const int64_t cap = (int64_t)a.max_blocks * a.BS;
   const int b0 = scan_first(a.B);
   const int64_t len0 = b0 < a.B ? a.ctx_lens[b0] : 0;  // in flight while the boundaries are scanned
-  scan_starts(a, starts, wsum);
-  scan_tiles(tp, wsum, a.B, [&](int b) {
+  scan_starts(a, starts, s);
+  const TileScan scan = scan_tiles(tp, s.wsum, a.B, [&](int b) {
     int64_t tokens;
-    const int g = group_of(a, starts, b, tokens);
+    const int g = group_of(a, s, starts, b, tokens);
     if (w == 0) a.group[b] = g;
     const int64_t Lc = min(b == b0 ? len0 : a.ctx_lens[b], cap), L = Lc - tokens;
-    if (b < KNOWN) known[2 * b] = (int)tokens, known[2 * b + 1] = (int)max((int64_t)0, Lc);
+    if (b < KNOWN) s.prefix[2 * b] = (int)tokens, s.prefix[2 * b + 1] = (int)max((int64_t)0, Lc);
     return L > 0 ? (int)((L + T - 1) / T) : 0;
+  });
+  const int sub = wave / a.hg, head = wave - sub * a.hg, per = NW / a.hg;
+  const unsigned total = (unsigned)a.ngroups * (unsigned)scan.total, nwg = a.nrest * per;
+  const unsigned Ct = max(1u, (total + nwg - 1) / nwg), v = w * per + sub;
+  place_tiles(tp, scan, [&](int b, int before, int after) {
+    for (int k = 0; k < per; ++k) {
+      const unsigned at = (w * per + k) * Ct;
+      if ((unsigned)a.ngroups * (unsigned)before <= at && at < (unsigned)a.ngroups * (unsigned)after) s.found[k] = b;
+    }
   });
   if (w == 0)
     for (int i = threadIdx.x; i <= a.B; i += 256) a.stiles[i] = tp[i];
-  const int sub = wave / a.hg, head = wave - sub * a.hg, per = NW / a.hg;
   if (sub >= per) return;  // hg == 3
-  const unsigned total = (unsigned)a.ngroups * (unsigned)tp[a.B], nwg = a.nrest * per;
-  const unsigned Ct = max(1u, (total + nwg - 1) / nwg), v = w * per + sub;
   unsigned u = v * Ct;
   const unsigned u_end = min(total, u + Ct);
   if (u >= u_end) return;
-  int b = 0, hi = a.B - 1;
-  while (b < hi) {
-    const int mid = (b + hi + 1) >> 1;
-    if ((unsigned)a.ngroups * (unsigned)tp[mid] <= u) b = mid;
-    else hi = mid - 1;
-  }
+  int b = s.found[sub];
   b = __builtin_amdgcn_readfirstlane(b);
   PoolWave<D, false, ONE> wv;
   wv.init(lane, a.kc, a.vc, nullptr, nullptr, a.Hkv, a.G, a.BS, a.NB, a.scale_log2);
@@ -410,11 +421,11 @@ __device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, in
           if (kh >= a.Hkv) continue;
           int start, L;
           if (b < KNOWN) {
-            start = __builtin_amdgcn_readfirstlane(known[2 * b]);
-            L = __builtin_amdgcn_readfirstlane(known[2 * b + 1]);
+            start = __builtin_amdgcn_readfirstlane(s.prefix[2 * b]);
+            L = __builtin_amdgcn_readfirstlane(s.prefix[2 * b + 1]);
           } else {
             int64_t tokens;
-            group_of(a, starts, b, tokens);
+            group_of(a, s, starts, b, tokens);
             start = __builtin_amdgcn_readfirstlane((int)tokens);
             L = __builtin_amdgcn_readfirstlane((int)min(a.ctx_lens[b], cap));
           }
@@ -433,11 +444,11 @@ __device__ __forceinline__ void rest_role(const SharedArgs& a, uint8_t* smem, in
 template <int D, bool ONE>
 __global__ __launch_bounds__(256, 2) void paged_shared_kernel(SharedArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[SMEM];
-  __shared__ int known[2 * KNOWN], wsum[NW];
+  __shared__ SharedLds lds;
   static_assert(SMEM >= 4 * KT * 2 * D, "K and V tiles, two each");
   const int w = blockIdx.x;
-  if (w < a.nprefix) prefix_role<D>(a, smem, wsum, w);
-  else rest_role<D, ONE>(a, smem, known, wsum, w - a.nprefix);
+  if (w < a.nprefix) prefix_role<D>(a, smem, lds, w);
+  else rest_role<D, ONE>(a, smem, lds, w - a.nprefix);
 }
 
 // One wave per 64 elements of an output row: the weights of up to 64 parts at a
