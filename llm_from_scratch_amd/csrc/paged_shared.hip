@@ -28,7 +28,7 @@
 // where the decode that reads every context by itself takes 1220; 64 sequences in
 // 3 groups behind 1536 to 3584 tokens, 16 / 4 of 64: 23 and 47.  Bound: at the first
 // the matrix cores' work beside the reads (a CU has one workgroup of each role), at
-// the second six dependent round trips (boundaries, lengths, table, rows) and the
+// the second five dependent round trips (boundaries, lengths, table, rows) and the
 // merge's launch.  Each workgroup taking a share of both roles, half of them in
 // either order, took 116 and 32: twice the parts, and twice the scans.
 // Group boundaries are read on the device: a running maximum of cu_groups,
