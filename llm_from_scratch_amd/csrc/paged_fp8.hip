@@ -18,22 +18,26 @@
 namespace lfs {
 namespace {
 
-// SCAN: a fixed grid shares the tiles of the batch (paged_decode_balanced's
-// split); else a workgroup per (sequence, group of kv heads) walks the whole
-// context.
+// A workgroup's four waves are 4 / hg shares of hg adjacent kv heads each.
+// SCAN: a fixed grid's shares split the tiles of the batch evenly
+// (paged_decode_balanced's split); else a share per (sequence, group of kv heads)
+// walks the whole context.  (With a workgroup a share, whose LDS lets two onto a CU,
+// one kv head took 33 us where it takes 27: 64 sequences of 128 to 8192 tokens, 8 /
+// 1 heads of 128.)
 template <int D, bool ONE, bool SCAN>
 __global__ __launch_bounds__(256) void paged_fp8_kernel(
     const uint16_t* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
     const float* __restrict__ ksc, const float* __restrict__ vsc, const int64_t* __restrict__ ctx_lens,
     const int32_t* __restrict__ bt, int64_t bt_stride, float* __restrict__ ws_o, float* __restrict__ ws_ml,
     int* __restrict__ tp_out, uint16_t* __restrict__ out, int Hkv, int G, int BS, int64_t NB, int max_blocks, int B,
-    float scale_log2, int ngroups) {
+    float scale_log2, int ngroups, int hg) {
   constexpr int T = PoolGeom<D, true>::T;
   __shared__ __attribute__((aligned(16))) float scales[4][2 * T];
   __shared__ int tp[SCAN ? BAL_MAXB + 1 : 1], lens[SCAN ? BAL_MAXB : 1];
-  __shared__ int wsum[4], found;
-  const int tid = threadIdx.x, wpg = blockDim.x >> 6;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  __shared__ int wsum[4], found[4];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int per = 4 / hg, sub = wave / hg, head = wave - sub * hg;
+  const unsigned v = blockIdx.x * per + sub;  // the share (sub == per: none, of 3 heads' fourth wave)
   const int cap = max_blocks * BS;
   PoolWave<D, true, ONE> w;
   w.init(lane, kc, vc, ksc, vsc, Hkv, G, BS, NB, scale_log2);
@@ -44,12 +48,12 @@ __global__ __launch_bounds__(256) void paged_fp8_kernel(
     r.q = q + h * G * D;
     r.t0 = i0 * T, r.t1 = min(L, i1 * T), r.kh = kh;
     r.out = r.t0 == 0 && r.t1 >= L ? out + h * G * D : nullptr;
-    r.prow = (slot * wpg + wave) * G;
+    r.prow = (slot * hg + head) * G;
   };
   if constexpr (!SCAN) {
-    const int b = (int)(blockIdx.x / (unsigned)ngroups), grp = (int)(blockIdx.x - (unsigned)b * ngroups);
-    const int kh = grp * wpg + wave, L = (int)min(ctx_lens[b], (int64_t)cap);
-    if (kh >= Hkv) return;
+    const int b = (int)(v / (unsigned)ngroups), grp = (int)(v - (unsigned)b * ngroups), kh = grp * hg + head;
+    if (sub >= per || b >= B || kh >= Hkv) return;
+    const int L = (int)max((int64_t)0, min(ctx_lens[b], (int64_t)cap));
     if (L <= 0) {
       uint16_t* o = out + ((int64_t)b * Hkv + kh) * G * D;
       for (int i = lane; i < G * D / 2; i += 64) reinterpret_cast<uint32_t*>(o)[i] = 0;
@@ -70,17 +74,20 @@ __global__ __launch_bounds__(256) void paged_fp8_kernel(
       lens[b] = L;
       return (L + T - 1) / T;
     });
-    const unsigned total = (unsigned)ngroups * (unsigned)scan.total, nwg = gridDim.x;
-    const unsigned Ct = max(1u, (total + nwg - 1) / nwg);
-    unsigned u = blockIdx.x * Ct;
-    const unsigned u_end = min(total, u + Ct);
+    const unsigned total = (unsigned)ngroups * (unsigned)scan.total, shares = gridDim.x * per;
+    const unsigned Ct = max(1u, (total + shares - 1) / shares);
     place_tiles(tp, scan, [&](int i, int before, int after) {
-      if ((unsigned)ngroups * (unsigned)before <= u && u < (unsigned)ngroups * (unsigned)after) found = i;
+      for (int k = 0; k < per; ++k) {
+        const unsigned at = (blockIdx.x * per + k) * Ct;
+        if ((unsigned)ngroups * (unsigned)before <= at && at < (unsigned)ngroups * (unsigned)after) found[k] = i;
+      }
     });
     if (blockIdx.x == 0)
       for (int i = tid; i <= B; i += blockDim.x) tp_out[i] = tp[i];
-    if (u >= u_end) return;
-    int b = __builtin_amdgcn_readfirstlane(found);
+    unsigned u = v * Ct;
+    const unsigned u_end = min(total, u + Ct);
+    if (sub >= per || u >= u_end) return;
+    int b = __builtin_amdgcn_readfirstlane(found[sub]);
     w.run(
         [&](PoolRange& r) {
           while (u < u_end) {
@@ -92,12 +99,12 @@ __global__ __launch_bounds__(256) void paged_fp8_kernel(
             }
             const unsigned grp = (u - base) / nb, i0 = (u - base) - grp * nb;
             const unsigned stop = min(u_end, base + (grp + 1) * nb);
-            const int kh = grp * wpg + wave;
+            const int kh = grp * hg + head;
             const int i1 = (int)(i0 + (stop - u));
             u = stop;
             if (kh >= Hkv) continue;
             range(r, b, kh, __builtin_amdgcn_readfirstlane(lens[b]), (int)i0, i1,
-                  (int64_t)blockIdx.x + (int64_t)b * ngroups + grp);
+                  (int64_t)v + (int64_t)b * ngroups + grp);
             return true;
           }
           return false;
@@ -143,12 +150,13 @@ extern "C" int lfs_paged_decode_fp8(const void* q, const void* k_cache, const vo
   float* ws_o = (float*)workspace;
   float* ws_ml = ws_o + rows * D;
   int* tp = (int*)(ws_ml + rows * 2);
-  const dim3 grid((unsigned)(scan ? bg.nwg : B * bg.ngroups)), block((unsigned)(64 * bg.wpg));
+  const int64_t per = 4 / bg.wpg;  // shares a workgroup
+  const dim3 grid((unsigned)(scan ? bg.nwg / per : (B * bg.ngroups + per - 1) / per)), block(256);
   hipStream_t st = (hipStream_t)stream;
 #define LFS_FP8(DD, ONE, SCAN)                                                                                        \
   hipLaunchKernelGGL((paged_fp8_kernel<DD, ONE, SCAN>), grid, block, 0, st, (const uint16_t*)q, (const uint8_t*)k_cache, \
                      (const uint8_t*)v_cache, k_scale, v_scale, context_lens, block_tables, bt_stride, ws_o, ws_ml, tp, \
-                     (uint16_t*)out, Hkv, G, BS, num_blocks, max_blocks, (int)B, scale * 1.4426950408889634f, bg.ngroups)
+                     (uint16_t*)out, Hkv, G, BS, num_blocks, max_blocks, (int)B, scale * 1.4426950408889634f, bg.ngroups, bg.wpg)
   if (D == 64) {
     if (!scan) LFS_FP8(64, false, false);
     else if (one) LFS_FP8(64, true, true);

@@ -51,7 +51,7 @@ struct SharedArgs {
   const int32_t *cu, *shared;
   float *po, *pml, *so, *sml;  // partials: prefix, rest
   int *starts, *punits, *stiles, *group;  // [NG + 1], [NG + 1], [B + 1], [B]: for the merge
-  int Hkv, G, BS, NG, B, max_blocks, tile, hg, ngroups, nprefix, nrest;
+  int Hkv, G, BS, NG, B, max_blocks, hg, ngroups, nprefix, nrest;
   int64_t NB;
   float scale_log2;
 };

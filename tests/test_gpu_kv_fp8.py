@@ -281,6 +281,8 @@ def test_decode_batches_of_none_and_short_tables():
     cut = [[x[:32] for x in s] for s in seqs]
     close(decode(q, pool, lens_of(seqs) * 100, bt[:, :2]), q, cut, 0.125, "cut")
     assert (decode(q, pool, lens_of(seqs), bt[:, :0]) == 0).all()
+    far = torch.tensor([2 ** 62, -2 ** 32 + 5], device=DEV)
+    close(decode(q, pool, far, bt[:, :2]), q, [cut[0], [x[:0] for x in cut[1]]], 0.125, "far")
     close(decode(q, pool, -lens_of(seqs), bt), q, [[x[:0] for x in s] for s in seqs], 0.125, "below zero")
 
 

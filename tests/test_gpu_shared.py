@@ -199,6 +199,8 @@ def test_scale_stride_and_empty_batches():
     cut = [[x[:64] for x in s] for s in seqs]  # contexts past their tables are cut there
     close(K.paged_attention_decode_shared(q, kc, vc, lens * 50, bt[:, :2], *meta), q, cut, 0.125, "cut")
     assert (K.paged_attention_decode_shared(q, kc, vc, -lens, bt, *meta) == 0).all()
+    far = torch.tensor([2 ** 62, -2 ** 32 + 5, 2 ** 33], device=DEV)
+    close(K.paged_attention_decode_shared(q, kc, vc, far, bt[:, :2], *meta), q, [cut[0], [x[:0] for x in cut[1]], cut[2]], 0.125)
 
 
 def test_pool_past_32_bits():
