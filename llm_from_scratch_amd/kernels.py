@@ -1159,7 +1159,9 @@ def apply_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
                                          v / 32 is set
     then one rounding to the logits' type.  Token ids outside [0, V) are ignored
     (-1: none).  Returns a new tensor, or ``out`` (which may be ``logits``)."""
-    assert logits.dim() == 2 and logits.stride(1) == 1, "logits must be [B, V] with unit column stride"
+    assert logits.dim() == 2, "logits must be [B, V] with unit column stride"
+    ld, unit = logits.stride()
+    assert unit == 1, "logits must be [B, V] with unit column stride"
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"logits must be torch.bfloat16 or torch.float32, got {logits.dtype}")
     _on_gpu(logits)
@@ -1184,44 +1186,53 @@ def apply_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     else:
         if prompt_lens is None or seq_lens is None:
             raise ValueError("tokens, prompt_lens and seq_lens go together")
-        tokens = _penalty_matrix(logits, tokens, torch.int32, "tokens", B)
-        token_args = (tokens.data_ptr(), _row_stride(tokens), tokens.size(1))
+        tokens, row, width = _penalty_matrix(dev, logits, tokens, torch.int32, "tokens", B)
+        token_args = (tokens.data_ptr(), row, width)
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
     n = 0
     if bias is not None:
-        bias_ids = _penalty_matrix(logits, bias_ids, torch.int32, "bias_ids", B).contiguous()
-        n = bias_ids.size(1)
-        bias = _penalty_matrix(logits, bias, torch.float32, "bias", B, n).contiguous()
+        bias_ids, row, n = _penalty_matrix(dev, logits, bias_ids, torch.int32, "bias_ids", B)
+        bias, brow, _ = _penalty_matrix(dev, logits, bias, torch.float32, "bias", B, n)
+        if row != n:
+            bias_ids = bias_ids.contiguous()
+        if brow != n:
+            bias = bias.contiguous()
     mask_args = (None, 0)
     if allowed is not None:
-        allowed = _penalty_matrix(logits, allowed, torch.int32, "allowed", B, -(-V // 32))
-        mask_args = (allowed.data_ptr(), _row_stride(allowed))
+        allowed, row, _ = _penalty_matrix(dev, logits, allowed, torch.int32, "allowed", B, -(-V // 32))
+        mask_args = (allowed.data_ptr(), row)
     if out is None:
         out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
+        ldo = V
     else:
         if out.get_device() != dev:
             _on_gpu(logits, out)
         if out.dtype is not logits.dtype:
             _dtype(out, logits.dtype, "out")
-        assert out.shape == logits.shape and out.stride(1) == 1, "out must be [B, V] with unit column stride"
+        ldo, unit = out.stride() if out.dim() == 2 else (0, 0)
+        assert out.shape == logits.shape and unit == 1, "out must be [B, V] with unit column stride"
     _launch("apply_penalties", _lib.load().lfs_apply_penalties, logits,
-            logits.data_ptr(), _row_stride(logits), out.data_ptr(), _row_stride(out), logits.dtype is torch.float32,
+            logits.data_ptr(), ld if B > 1 else V, out.data_ptr(), ldo if B > 1 else V, logits.dtype is torch.float32,
             *token_args, *map(_ptr, rows), _ptr(bias_ids), _ptr(bias), n, *mask_args, B, V)
     return out
 
 
-def _penalty_matrix(logits: torch.Tensor, t: torch.Tensor, dtype: torch.dtype, name: str, rows: int,
-                    width: Optional[int] = None) -> torch.Tensor:
-    """t [rows, width], checked, with unit column stride."""
-    if t.get_device() != logits.get_device():
+def _penalty_matrix(dev: int, logits: torch.Tensor, t: torch.Tensor, dtype: torch.dtype, name: str, rows: int,
+                    width: Optional[int] = None):
+    """(t [rows, width] with unit column stride, its row stride, width), checked."""
+    if t.get_device() != dev:
         _on_gpu(logits, t)
     if t.dtype is not dtype:
         _dtype(t, dtype, name)
     shape = t.shape
     assert len(shape) == 2 and shape[0] == rows and (width is None or shape[1] == width), \
         f"{name} must be [B, {'n' if width is None else width}]"
-    return t if t.stride(1) == 1 else t.contiguous()
+    row, unit = t.stride()
+    if unit != 1:
+        t = t.contiguous()
+        row = shape[1]
+    return t, (row if rows > 1 else shape[1]), shape[1]
 
 
 _PENALTY_TYPES = (torch.int32, torch.int32, torch.float32, torch.float32, torch.float32)

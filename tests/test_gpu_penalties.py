@@ -196,6 +196,30 @@ def test_layouts(dtype, V):
     assert torch.equal(check(one.expand(B, V), **history, **more), check(one.repeat(B, 1), **history, **more))
 
 
+@pytest.mark.parametrize("V", [1, 77, 9001])
+def test_single_rows_of_any_stride(V):
+    """One row whose stride is not its width: of a transposed column (1), of
+    every third row (3 V); as logits, as out, as tokens and as a mask."""
+    rng = np.random.default_rng(V)
+    tokens = rng.integers(0, V, (1, 20))
+    more = dict(prompts=np.full(1, 3), lens=np.full(1, 20), rep=np.full(1, 1.5), pres=np.full(1, 0.5),
+                freq=np.full(1, 0.1), allowed=rng.random((1, V)) < 0.8)
+    flat = logits_of(rng, 1, V).view(V)
+    want = check(flat.view(1, V), tokens, **more)
+    for stride in (1, 3 * V):
+        one = flat.as_strided((1, V), (stride, 1))
+        assert torch.equal(check(one, tokens, **more), want)
+        out = torch.empty(V, dtype=flat.dtype, device=DEV).as_strided((1, V), (stride, 1))
+        check(one, tokens, **more, out=out)
+        assert torch.equal(out, want)
+        bits = dev(words(more["allowed"]), np.int32)
+        got = K.apply_penalties(
+            one, dev(tokens, np.int32).as_strided((1, 20), (stride, 1)), dev(more["prompts"], np.int32),
+            dev(more["lens"], np.int32), dev(more["rep"], np.float32), dev(more["pres"], np.float32),
+            dev(more["freq"], np.float32), allowed=bits.as_strided(bits.shape, (stride, 1)))
+        assert torch.equal(got, want)
+
+
 def test_rows_past_32_bits():
     V, B = 150000, 15000
     x = torch.empty(B, V, dtype=torch.bfloat16, device=DEV)
