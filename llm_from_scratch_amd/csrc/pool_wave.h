@@ -109,6 +109,13 @@ struct PoolWave {
     sr = T - sq * BS;
   }
 
+  // Begin the range in ask_at: its first tile's place and column.
+  __device__ __forceinline__ void begin() {
+    pos = ask_at.t0;
+    const unsigned t = pos + (lane >> 4) * 16;
+    col = (int)(t / (unsigned)BS);
+    off = (int)t - col * BS;
+  }
   // Of the next tile (of the range under way, else of the one that next() fills
   // in) ask for the block ids; columns past the range's are not read.
   template <class Next>
@@ -116,11 +123,11 @@ struct PoolWave {
     ask_first = pos >= ask_at.t1;
     if (ask_first) {
       more = next(ask_at);
-      pos = ask_at.t0;
-      const unsigned t = pos + (lane >> 4) * 16;
-      col = (int)(t / (unsigned)BS);
-      off = (int)t - col * BS;
+      begin();  // without another range the last one again, of which nothing is then used
     }
+    ask_tile();
+  }
+  __device__ __forceinline__ void ask_tile() {
     ask_n = more ? min(T, ask_at.t1 - pos) : 0;
     pos += T;
     ask_last = pos >= ask_at.t1;
@@ -325,11 +332,12 @@ struct PoolWave {
   template <class Next>
   __device__ __forceinline__ void run(Next&& next, float* __restrict__ pw, float* __restrict__ ws_o,
                                       float* __restrict__ ws_ml) {
-    ask_at.t1 = 0;
-    pos = 0;
-    more = true;
-    ask(next);
-    if (!more) return;
+    // A wave may have no range at all (its heads lie past the last): ask_at then
+    // holds nothing that could be read.
+    if (!next(ask_at)) return;
+    more = ask_first = true;
+    begin();
+    ask_tile();
     Tile a, b;
     load(a);
     ask(next);

@@ -272,6 +272,39 @@ def test_decode_many_sequences():
         assert diff <= 0.05
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(10, 5, 64), (6, 6, 128), (14, 7, 64), (40, 10, 128), (9, 9, 64)])
+@pytest.mark.parametrize("BS", [16, 64])
+def test_decode_of_heads_that_fill_no_last_group(Hq, Hkv, D, BS):
+    """Waves work on four kv heads at a time; in the last group some of them have
+    none, for their whole share of the batch (one long sequence) or for a part of
+    it (short ones)."""
+    rng = np.random.default_rng(Hq + D + BS)
+    for lens in ([5000], [1], [0, 1, 15, 65, 300, 0, 700, 64, 2049], rng.integers(1, 90, 70).tolist()):
+        pool, bt, seqs = filled(rng, lens, BS, Hkv, D)
+        q = queries(rng, len(lens), Hq, D)
+        print(f"fp8 decode {Hq}/{Hkv}x{D} blocks of {BS}, {len(lens)} sequences", flush=True)
+        o = decode(q, pool, lens_of(seqs), bt)
+        close(o, q, seqs, D ** -0.5, f"{len(lens)} sequences")
+        if Hq * D % 128 == 0:
+            o2, oq, os_ = decode(q, pool, lens_of(seqs), bt, quant=True)
+            wq, ws = K.act_quant(o.view(len(lens), -1))
+            assert torch.equal(o, o2) and np.array_equal(bits(oq), bits(wq)) and torch.equal(os_, ws)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 4, 128), (6, 3, 128), (5, 5, 64)])
+def test_decode_many_sequences_of_several_heads(Hq, Hkv, D):
+    """Past the balanced split's batches, with groups of three and four heads."""
+    rng = np.random.default_rng(Hq + D)
+    B = 8200
+    lens = rng.integers(0, 70, 64)
+    pool, bt, seqs = filled(rng, lens.tolist(), 16, Hkv, D)
+    q = queries(rng, B, Hq, D)
+    at = torch.arange(B, device=DEV) % 64
+    o = decode(q, pool, lens_of(seqs)[at], bt[at])
+    rows = list(range(64)) + [4097, 8191, 8192, 8199]
+    close(o[rows], q[rows], [seqs[r % 64] for r in rows], D ** -0.5)
+
+
 def test_decode_batches_of_none_and_short_tables():
     rng = np.random.default_rng(11)
     pool, bt, seqs = filled(rng, [40, 40], 16, 2, 64)

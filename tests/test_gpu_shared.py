@@ -103,6 +103,18 @@ def test_large_groups(Hq, Hkv, D):
     check(rng, groups, 64, Hq, Hkv, D)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(10, 5, 64), (6, 6, 128), (14, 7, 64), (40, 10, 128), (9, 9, 64)])
+@pytest.mark.parametrize("BS", [16, 64])
+def test_heads_that_fill_no_last_group(Hq, Hkv, D, BS):
+    """Waves walk what sequences have for themselves four kv heads at a time; in
+    the last group some of them have none, for their whole share (one long
+    sequence) or for a part of it (short ones behind prefixes)."""
+    rng = np.random.default_rng(Hq + D + BS)
+    for groups in ([(0, [5000])], [(3, [3 * BS + 4000])], [(2, (2 * BS + rng.integers(1, 200, 9)).tolist()), (0, [1, 65])],
+                   [(1, [BS + 70] * 40), (4, [4 * BS + 3] * 20)]):
+        check(rng, groups, BS, Hq, Hkv, D, str(groups)[:60])
+
+
 def test_equals_the_plain_decode():
     """The same batch through paged_attention_decode, to the tolerance of both."""
     rng = np.random.default_rng(4)
