@@ -115,6 +115,24 @@ def test_heads_that_fill_no_last_group(Hq, Hkv, D, BS):
         check(rng, groups, BS, Hq, Hkv, D, str(groups)[:60])
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(12, 4, 64), (32, 8, 128), (8, 1, 128)])
+def test_weights_of_a_prefix_keep_16_bits(Hq, Hkv, D):
+    """Values of either sign that nearly cancel show a weight's rounding beside
+    the output's: no more than 2^-16 of sum w |v|, as over a pool in 8 bits, and
+    2^-12 of it for fp32 scores, exponentials and sums."""
+    rng = np.random.default_rng(Hq * D)
+    for groups in ([(1, [16, 16, 5, 2])], [(4, [64, 64, 50, 80, 200])], [(130, [2080, 2080, 2090])]):
+        kc, vc, bt, lens, meta, seqs = branches(rng, groups, 16, Hkv, D)
+        vc.copy_(torch.where(vc > 0, 1.0, vc).where(~(vc < 0), -1.0))
+        seqs = [[k, np.sign(v)] for k, v in seqs]
+        q = bf16(rng, len(seqs), Hq, D)
+        o = K.paged_attention_decode_shared(q, kc, vc, lens, bt, *meta).double().cpu().numpy()
+        for b, (k, v) in enumerate(seqs):
+            want, a = P.window_attention(q[b:b + 1].double().cpu().numpy(), k, v, [len(k) - 1], D ** -0.5, len(k) + 1, 0)
+            err, tol = np.abs(o[b] - want[0]), 2.0 ** -8 * np.abs(want[0]) + (2.0 ** -12 + 2.0 ** -16) * a[0]
+            assert (err <= tol).all(), f"{groups} row {b}: worst {(err / tol).max():.3g}"
+
+
 def test_equals_the_plain_decode():
     """The same batch through paged_attention_decode, to the tolerance of both."""
     rng = np.random.default_rng(4)
