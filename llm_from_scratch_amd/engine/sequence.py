@@ -9,6 +9,7 @@ block and gives a full last block an empty slot list).
 from __future__ import annotations
 
 import math
+import operator
 from array import array
 from copy import copy
 from dataclasses import dataclass
@@ -19,6 +20,35 @@ from typing import Optional
 import numpy as np
 
 
+PENALTY_LIMIT = 1e30  # finite logits stay finite in fp32 with penalties and biases up to it
+
+
+def check_penalties(sp) -> tuple[Optional[dict[int, float]], Optional[np.ndarray]]:
+    """logit_bias and allowed_token_ids as a Sequence holds them, checked with the
+    penalties."""
+    assert 0 < sp.repetition_penalty < math.inf, "repetition_penalty must be > 0"
+    assert 1 / PENALTY_LIMIT <= sp.repetition_penalty <= PENALTY_LIMIT, \
+        f"repetition_penalty must be in [{1 / PENALTY_LIMIT:g}, {PENALTY_LIMIT:g}]"
+    assert abs(sp.presence_penalty) <= PENALTY_LIMIT and abs(sp.frequency_penalty) <= PENALTY_LIMIT, \
+        f"presence_penalty and frequency_penalty must be finite, at most {PENALTY_LIMIT:g} in size"
+    bias = allowed = None
+    if sp.logit_bias:
+        assert len(sp.logit_bias) <= 1024, "logit_bias holds at most 1024 tokens"
+        bias = {operator.index(t): float(v) for t, v in sp.logit_bias.items()}
+        assert all(-2 ** 31 <= t < 2 ** 31 for t in bias), "logit_bias tokens must fit 32 bits"
+        assert all(abs(v) <= PENALTY_LIMIT or v == -math.inf for v in bias.values()), \
+            f"logit_bias values must be at most {PENALTY_LIMIT:g} in size, or -infinity"
+    if sp.allowed_token_ids is not None:
+        ids = sp.allowed_token_ids
+        if not (isinstance(ids, np.ndarray) and ids.dtype.kind in "iu"):
+            ids = [operator.index(t) for t in ids]
+            assert all(-2 ** 63 <= t < 2 ** 63 for t in ids), "allowed_token_ids must fit 64 bits"
+        allowed = np.array(ids, np.int64)
+        assert allowed.size > 0, "allowed_token_ids allows no token"
+        assert allowed.ndim == 1, "allowed_token_ids must be one row"
+    return bias, allowed
+
+
 @dataclass
 class SamplingParams:
     """utils/sampler.py:7-23 of the reference, plus the ``max_model_length``
@@ -27,7 +57,9 @@ class SamplingParams:
     kernels.apply_penalties does to the logits before: repetition_penalty
     (1: none) for tokens of the prompt and the completion, presence_penalty and
     frequency_penalty (0: none) for those of the completion, logit_bias (token ->
-    value) and allowed_token_ids (None: all)."""
+    value, -infinity for a token never drawn) and allowed_token_ids (None: all;
+    a list, set or array of whole numbers).  Tokens outside the vocabulary are
+    ignored."""
     temperature: float = 1.0
     max_tokens: int = 256
     ignore_eos: bool = False
@@ -45,11 +77,7 @@ class SamplingParams:
         assert self.temperature > 1e-10, "greedy sampling is not permitted"
         assert 0 <= self.top_k < 2 ** 31 and 0 < self.top_p <= 1 and 0 <= self.min_p <= 1, \
             "top_k must be in [0, 2**31), top_p in (0, 1], min_p in [0, 1]"
-        assert 0 < self.repetition_penalty < math.inf, "repetition_penalty must be > 0"
-        assert math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty), \
-            "presence_penalty and frequency_penalty must be finite"
-        assert not self.logit_bias or len(self.logit_bias) <= 1024, "logit_bias holds at most 1024 tokens"
-        assert self.allowed_token_ids is None or len(self.allowed_token_ids) > 0, "allowed_token_ids allows no token"
+        check_penalties(self)
 
 
 class SequenceStatus(Enum):
@@ -76,7 +104,7 @@ class Sequence:
         self.top_k, self.top_p, self.min_p = sp.top_k, sp.top_p, sp.min_p
         self.repetition_penalty = sp.repetition_penalty
         self.presence_penalty, self.frequency_penalty = sp.presence_penalty, sp.frequency_penalty
-        self.logit_bias, self.allowed_token_ids = sp.logit_bias, sp.allowed_token_ids
+        self.logit_bias, self.allowed_token_ids = check_penalties(sp)
         self._history = array("i")
         self.temperature = sp.temperature
         self.max_tokens = sp.max_tokens

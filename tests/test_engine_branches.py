@@ -118,3 +118,36 @@ def test_what_pools_in_8_bits_and_shared_prefixes_go_with():
     with pytest.raises(ValueError, match="no scales"):
         checked(Layer(scales=False), kv_dtype=fp8)
     assert DecodeModelConfig().runner_config(kv_dtype=fp8)["kv_dtype"] == fp8
+
+
+def test_sampling_params_that_would_fail_later():
+    """What the logits cannot take is refused where it is given, not in a step."""
+    inf = float("inf")
+    for bad in ({2 ** 31: 1.0}, {-2 ** 31 - 1: 1.0}, {3: inf}, {3: float("nan")}, {3: 1e39}, {3: -1e31}):
+        with pytest.raises(AssertionError, match="logit_bias"):
+            SamplingParams(logit_bias=bad)
+    for bad in ({"3": 1.0}, {3.0: 1.0}, {3: None}):
+        with pytest.raises(TypeError):
+            SamplingParams(logit_bias=bad)
+    for bad in ([1.5], "12", [None]):
+        with pytest.raises(TypeError):
+            SamplingParams(allowed_token_ids=bad)
+    for bad in ([2 ** 63], np.zeros((2, 2), np.int64), set()):
+        with pytest.raises(AssertionError, match="allowed_token_ids"):
+            SamplingParams(allowed_token_ids=bad)
+    for bad in (dict(repetition_penalty=1e-46), dict(repetition_penalty=1e39), dict(frequency_penalty=1e39),
+                dict(presence_penalty=-inf)):
+        with pytest.raises(AssertionError, match="penalty"):
+            SamplingParams(**bad)
+    # parameters changed after they were made are checked when a sequence takes them
+    sp = SamplingParams()
+    sp.logit_bias = {2 ** 31: 1.0}
+    with pytest.raises(AssertionError, match="logit_bias"):
+        Sequence([1], sp)
+
+
+@pytest.mark.parametrize("ids", [{0, 33, 69}, (0, 33, 69), np.array([69, 33, 0], np.int32), {69: 1, 33: 1, 0: 1},
+                                 torch.tensor([0, 33, 69]), [np.int64(0), 33, 69, 2 ** 40]])
+def test_allowed_tokens_of_any_kind(ids):
+    m = penalty_metadata([seq([1], 1, allowed_token_ids=ids, logit_bias={np.int64(7): -float("inf")})], 70)
+    assert m["allowed"].tolist() == [[1, 2, 32]] and m["bias"].tolist() == [[-np.inf]]
