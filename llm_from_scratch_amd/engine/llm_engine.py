@@ -54,6 +54,8 @@ class LLMEngine:
             eos=config.get("eos", 50256),
             sliding_window=window,
             num_sink_tokens=sinks)
+        # of the logits, where the configuration or the model says so
+        self.vocab_size = config.get("vocab_size", getattr(getattr(model, "cfg", None), "vocab_size", None))
         self.tokenizer = tokenizer
         self.generator = generator
         self.verbose = verbose
@@ -72,7 +74,10 @@ class LLMEngine:
         if isinstance(prompt, str):
             assert self.tokenizer is not None, "string prompts need a tokenizer"
             prompt = self.tokenizer.encode(prompt)
-        self.scheduler.add_sequence(Sequence(list(prompt), sampling_params))
+        seq = Sequence(list(prompt), sampling_params)
+        if self.vocab_size is not None:
+            seq.check_tokens(self.vocab_size)
+        self.scheduler.add_sequence(seq)
 
     def fork(self, seq_id: int, n: int = 1) -> list[int]:
         """n branches of a running sequence, between steps: each goes on from its

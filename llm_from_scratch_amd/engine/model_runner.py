@@ -122,7 +122,8 @@ def shared_groups(tables: list[list[int]]) -> tuple[list[int], list[int]]:
 
 def penalty_metadata(seqs: list[Sequence], vocab: int) -> dict:
     """Host arrays of what the batch's logits go through before sampling
-    (kernels.apply_penalties): of each kind, if any of its sequences has it."""
+    (kernels.apply_penalties): of each kind, if any of its sequences has it.  A
+    sequence that is left no token is refused: its draw would be one it rules out."""
     B = len(seqs)
     out = {}
     if any(s.has_penalties for s in seqs):
@@ -134,6 +135,9 @@ def penalty_metadata(seqs: list[Sequence], vocab: int) -> dict:
                    prompt_lens=np.array([s.num_prompt_tokens for s in seqs], np.int32))
         for name in ("repetition", "presence", "frequency"):
             out[name] = np.array([getattr(s, name + "_penalty") for s in seqs], np.float32)
+    for s in seqs:
+        if s.num_completion_tokens == 0:
+            s.check_tokens(vocab)
     if any(s.logit_bias for s in seqs):
         pairs = [list((s.logit_bias or {}).items()) for s in seqs]
         out["bias_ids"] = np.full((B, max(map(len, pairs))), -1, np.int32)
@@ -148,7 +152,10 @@ def penalty_metadata(seqs: list[Sequence], vocab: int) -> dict:
             if s.allowed_token_ids is not None:
                 ids = np.asarray(s.allowed_token_ids, np.int64)
                 bits = np.zeros(words * 32, np.uint8)
-                bits[ids[(ids >= 0) & (ids < vocab)]] = 1
+                ids = ids[(ids >= 0) & (ids < vocab)]
+                if ids.size == 0:  # replaced since
+                    s.check_tokens(vocab)
+                bits[ids] = 1
                 allowed[b] = np.packbits(bits, bitorder="little").view(np.int32)
         out["allowed"] = allowed
     return out

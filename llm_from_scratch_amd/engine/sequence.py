@@ -59,7 +59,7 @@ class SamplingParams:
     frequency_penalty (0: none) for those of the completion, logit_bias (token ->
     value, -infinity for a token never drawn) and allowed_token_ids (None: all;
     a list, set or array of whole numbers).  Tokens outside the vocabulary are
-    ignored."""
+    ignored, but one at least must be left to draw (Sequence.check_tokens)."""
     temperature: float = 1.0
     max_tokens: int = 256
     ignore_eos: bool = False
@@ -165,6 +165,20 @@ class Sequence:
     @property
     def has_penalties(self):
         return self.repetition_penalty != 1 or self.presence_penalty != 0 or self.frequency_penalty != 0
+
+    def check_tokens(self, vocab: int) -> None:
+        """Of ``vocab`` tokens, logit_bias and allowed_token_ids must leave one."""
+        if not self.logit_bias and self.allowed_token_ids is None:
+            return
+        banned = {t for t, v in (self.logit_bias or {}).items() if v == -math.inf and 0 <= t < vocab}
+        if self.allowed_token_ids is None:
+            left = vocab > len(banned)
+        else:
+            ids = np.asarray(self.allowed_token_ids, np.int64)
+            ids = ids[(ids >= 0) & (ids < vocab)]
+            left = ids.size > 0 and (not banned or not banned.issuperset(ids.tolist()))
+        if not left:
+            raise ValueError(f"logit_bias and allowed_token_ids leave none of the {vocab} tokens")
 
     def history(self) -> np.ndarray:
         """The token ids as int32, from a copy that grows with them."""

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from llm_from_scratch_amd.decode_model import DecodeModelConfig
-from llm_from_scratch_amd.engine import ModelRunner, SamplingParams, Sequence
+from llm_from_scratch_amd.engine import ModelRunner, SamplingParams, Sequence, llm_engine
 from llm_from_scratch_amd.engine.model_runner import penalty_metadata, shared_groups
 
 
@@ -151,3 +151,40 @@ def test_sampling_params_that_would_fail_later():
 def test_allowed_tokens_of_any_kind(ids):
     m = penalty_metadata([seq([1], 1, allowed_token_ids=ids, logit_bias={np.int64(7): -float("inf")})], 70)
     assert m["allowed"].tolist() == [[1, 2, 32]] and m["bias"].tolist() == [[-np.inf]]
+
+
+def test_a_sequence_must_be_left_a_token(monkeypatch):
+    banned = -float("inf")
+    none = [dict(allowed_token_ids=[5000, -1]), dict(allowed_token_ids=[3, 5000], logit_bias={3: banned}),
+            dict(logit_bias={t: banned for t in range(70)})]
+    some = [dict(allowed_token_ids=[5000, 69]), dict(allowed_token_ids=[3, 4], logit_bias={3: banned}),
+            dict(logit_bias={t: banned for t in range(1, 80)}), dict(allowed_token_ids=[3], logit_bias={3: -1e30})]
+    for kw in none:
+        with pytest.raises(ValueError, match="none of the 70 tokens"):
+            penalty_metadata([seq([1], 1), seq([1], 1, **kw)], 70)
+    for kw in some:
+        penalty_metadata([seq([1], 1), seq([1], 1, **kw)], 70)
+    s = seq([1, 2], 1, allowed_token_ids=[4])
+    s.allowed_token_ids = [70]  # between steps
+    with pytest.raises(ValueError, match="none of the 70 tokens"):
+        penalty_metadata([s], 70)
+
+    # the engine refuses the prompt, so that the batch goes on without it
+    class Runner:
+        num_available_kv_blocks = 4
+
+        def __init__(self, *args):
+            pass
+
+    monkeypatch.setattr(llm_engine, "ModelRunner", Runner)
+    monkeypatch.setattr(Sequence, "block_size", Sequence.block_size)
+    model = torch.nn.Module()
+    model.cfg = DecodeModelConfig(vocab_size=70)
+    for eng in (llm_engine.LLMEngine(model, {}), llm_engine.LLMEngine(torch.nn.Module(), dict(vocab_size=70))):
+        for kw in none:
+            with pytest.raises(ValueError, match="none of the 70 tokens"):
+                eng.add_prompt([1, 2], SamplingParams(**kw))
+        assert not eng.scheduler.waiting
+        for kw in some:
+            eng.add_prompt([1, 2], SamplingParams(**kw))
+        assert len(eng.scheduler.waiting) == len(some)
