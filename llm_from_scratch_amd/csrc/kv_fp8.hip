@@ -27,6 +27,7 @@ namespace {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int SU = 4;  // rows in flight per thread of a store
 constexpr int MAX_ROWS = 1024;  // (K or V, head) rows of a workgroup
+constexpr int64_t MAX_WGS = (1 << 24) - 1;  // of 256 threads: a launch takes less than 2^32
 
 template <int D, bool VEC>
 __global__ __launch_bounds__(256) void store_kvcache_fp8_kernel(
@@ -186,6 +187,7 @@ extern "C" int lfs_store_kvcache_fp8(const void* key, int64_t k_stride_t, const 
   int tok = std::max(1, std::min(16, 1024 / pieces));
   if (T < (int64_t)640 * tok) tok = std::max(1, std::min(16, 256 / pieces));
   const int64_t wgs = (T + tok - 1) / tok;
+  LFS_REQUIRE(wgs <= MAX_WGS, "store_kvcache_fp8: too many tokens");
 #define LFS_STORE(DD, VEC)                                                                                            \
   hipLaunchKernelGGL((store_kvcache_fp8_kernel<DD, VEC>), dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,     \
                      (const uint16_t*)key, k_stride_t, (const uint16_t*)value, v_stride_t, (uint8_t*)k_cache,         \
@@ -218,6 +220,7 @@ extern "C" int lfs_load_kvcache_fp8(const void* k_cache, const void* v_cache, co
               "load_kvcache_fp8: caches, k and v must be 16-byte aligned");
   LFS_REQUIRE(Hkv <= 65536, "load_kvcache_fp8: too many kv heads (%d)", Hkv);
   const int64_t wgs = (total + LT - 1) / LT;
+  LFS_REQUIRE(wgs <= MAX_WGS, "load_kvcache_fp8: too many rows");
 #define LFS_LOAD(DD)                                                                                                  \
   hipLaunchKernelGGL((load_kvcache_fp8_kernel<DD>), dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,           \
                      (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, block_tables, bt_stride,     \

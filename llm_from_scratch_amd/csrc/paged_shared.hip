@@ -591,6 +591,8 @@ extern "C" int lfs_paged_decode_shared(const void* q, const void* k_cache, const
   LFS_REQUIRE(((B * G + PROWS - 1) / PROWS + std::min(B / 2, num_groups)) * Hkv * ((tokens + KT - 1) / KT) < (1ll << 31) &&
                   B * a.ngroups * ((tokens + T - 1) / T) < (1ll << 31),
               "paged_decode_shared: too many context tiles");
+  const int64_t E = B * Hq * D;
+  LFS_REQUIRE(E <= (1ll << 32) - 128, "paged_decode_shared: too many outputs");  // a thread each, less than 2^32 a launch
   const int64_t prows = prefix_rows(B, Hq), srows = rest_rows(B, Hq);
   a.q = (const uint16_t*)q, a.kc = (const uint16_t*)k_cache, a.vc = (const uint16_t*)v_cache;
   a.ctx_lens = context_lens, a.bt = block_tables, a.bt_stride = bt_stride;
@@ -613,7 +615,6 @@ extern "C" int lfs_paged_decode_shared(const void* q, const void* k_cache, const
 #undef LFS_SHARED
   const int rc2 = check_launch("paged_decode_shared");
   if (rc2) return rc2;
-  const int64_t E = B * Hq * D;
   if (D == 64)
     hipLaunchKernelGGL((paged_shared_merge<64>), dim3((unsigned)((E + 127) / 128)), dim3(128), 0, st, a, (uint16_t*)out,
                        (uint8_t*)q_out, q_scale, E);

@@ -119,3 +119,15 @@ def test_penalty_refusals(lib):
     refused(lib, call(n=1025, ids=16, bias=16), b"1024")
     refused(lib, call(allowed=16, mst=3), b"too few words")
     assert call(B=0, x=None) == 0
+
+
+def test_calls_past_the_threads_of_a_launch_are_refused(lib):
+    """2^32 threads: the host's error, not the launch's."""
+    for T, Hkv in ((1 << 28, 1), ((1 << 28) - 15, 2)):
+        refused(lib, lib.lfs_load_kvcache_fp8(16, 16, 16, 16, 16, 4, 4, 16, 1, T, 16, 16, Hkv, 64, 16, 8, None), b"too many rows")
+    refused(lib, lib.lfs_store_kvcache_fp8(16, 64, 16, 64, 16, 16, 16, 16, 16, 1 << 28, 1, 64, 16, 8, None),
+            b"too many tokens")
+    B, Hq, Hkv, D = 8192, 8192, 1024, 64
+    need = lib.lfs_paged_decode_shared_workspace_bytes(B, 1, Hq, Hkv, D)
+    refused(lib, lib.lfs_paged_decode_shared(16, 16, 16, 16, 16, 4, 16, 16, 1, 16, 16, need, B, Hq, Hkv, D, 16, 8, 4, 0.1,
+                                             None, None, None), b"too many outputs")
