@@ -698,8 +698,9 @@ int lfs_scatter_add_weighted(const void* x, int32_t x_is_f32, int64_t ldx, const
  * (bf16 [T, Hkv, D], heads and dims contiguous, any token stride):
  *   s = max(amax over the head's D values, 1e-4) * fp32(1/448),
  *   code = e4m3fn(clamp(x / s, -448, 448))
- * as lfs_act_quant with a group of D.  Two tokens of one slot leave either's
- * values.  D = 64 or 128, at most 512 kv heads; caches 8-byte aligned.
+ * as lfs_act_quant with a group of D.  A slot may appear once: two tokens of one
+ * slot would leave codes and scales of both, mixed.  D = 64 or 128, at most 512
+ * kv heads; caches 8-byte aligned.
  */
 int lfs_store_kvcache_fp8(const void* key, int64_t k_stride_t, const void* value, int64_t v_stride_t,
                           void* k_cache, void* v_cache, float* k_scale, float* v_scale,

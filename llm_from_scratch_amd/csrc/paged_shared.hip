@@ -13,24 +13,26 @@
 //          order; a workgroup takes an equal run of them.  A wave has 32 rows, the
 //          waves share 64-key K and V tiles in LDS, the next tile's copies in
 //          flight: the products, swizzles and copies of prefill.hip (tile32.h),
-//          without the causal mask and with the keys' range cut in runs.
+//          without the causal mask, with the keys' range cut in runs and with
+//          weights of 16 bits (outputs as exact as paged_attention_decode's).
 //          Consecutive workgroups hold consecutive runs of one (kv head, 128
 //          rows), so those of the next 128 rows on the same keys often run on the
 //          same XCD and find them in its L2.
 //  rest    the walk of pool_wave.h from the prefix's end on, shared by the
 //          balanced split of decode_wave.h.  A group of one sequence has no
-//          prefix here, its whole context is rest; from two on it pays (64
-//          sequences behind 4096 tokens each pair, four, eight shares: 145, 88, 52
-//          us of 32 / 8 heads of 128, 162 to 174 by themselves; of 16 / 4 of 64 63,
-//          38, 23 and 57 to 59).
-// What it takes (us, in all; alone the roles 65 and 57): 128 sequences of 64 to 1024
-// tokens behind 16384 shared ones, 32 / 8 heads of 128: 93, of which the merge 11,
+//          prefix here, its whole context is rest; from two on it pays, but for
+//          pairs with heads of 64 (64 sequences behind 4096 tokens each pair, four,
+//          eight shares: 161, 95, 54 us of 32 / 8 heads of 128, 151 to 174 by
+//          themselves; of 16 / 4 of 64 69, 42, 25 and 57 to 58).
+// What it takes (us, in all; alone the roles 79-84 and 57): 128 sequences of 64 to 1024
+// tokens behind 16384 shared ones, 32 / 8 heads of 128: 100, of which the merge 11,
 // where the decode that reads every context by itself takes 1220; 64 sequences in
-// 3 groups behind 1536 to 3584 tokens, 16 / 4 of 64: 23 and 47.  Bound: at the first
+// 3 groups behind 1536 to 3584 tokens, 16 / 4 of 64: 24 and 47.  Bound: at the first
 // the matrix cores' work beside the reads (a CU has one workgroup of each role), at
 // the second five dependent round trips (boundaries, lengths, table, rows) and the
 // merge's launch.  Each workgroup taking a share of both roles, half of them in
-// either order, took 116 and 32: twice the parts, and twice the scans.
+// either order, took 116 and 32 where this took 93 and 23 (weights of 8 bits then): twice the
+// parts, and twice the scans.
 // Group boundaries are read on the device: a running maximum of cu_groups,
 // clipped to the batch, so that any values keep every access in bounds.
 #include "pool_wave.h"

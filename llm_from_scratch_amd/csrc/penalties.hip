@@ -15,9 +15,9 @@
 // (integers: any order gives the same), whose first occurrences make a list.
 // After a barrier the few listed and biased tokens are read again and written as
 // the formula has them.  Counting every logit's penalties in the stream instead
-// took 45 us where this takes 40 (4.0 TB/s; 256 rows of 150001, histories of 50 to
+// took 45 us where this took 40 on that card (256 rows of 150001, histories of 50 to
 // 4096, 64 biases): nearly every wave has some token with a count.  Bound: HBM, a
-// read and a write of the logits.
+// read and a write of the logits; 40-44 us on several cards, 3.7-4.0 TB/s.
 #include "common.h"
 
 namespace lfs {

@@ -92,8 +92,9 @@ class LLMEngine:
 
     def pack_kv_cache(self) -> int:
         """Move the blocks in use to the start of the pool, between steps;
-        returns their number n: kv_cache[:, :, :n] then holds every running
-        sequence's keys and values."""
+        returns their number n: kv_cache[:, :, :n] of the runner then holds every
+        running sequence's keys and values, with kv_scales[:, :, :n] those of a pool
+        in 8 bits."""
         self.model_runner.copy_blocks(self.scheduler.pack())
         return len(self.scheduler.block_manager.used_block_ids)
 

@@ -1146,7 +1146,7 @@ def apply_penalties(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
                     bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Logits with penalties for the tokens of each row's history, biases and a
-    mask of allowed tokens: what goes to sample_gumbel or sample_filtered.
+    mask of allowed tokens: in bf16 what sample_gumbel and sample_filtered take.
 
     logits: bf16 or fp32 [B, V] (unit column stride).  Row b's history is
     tokens[b, :seq_lens[b]] (int32 [B, L] and [B]), its first prompt_lens[b]
